@@ -19,7 +19,9 @@ BUILD = os.path.join(ROOT, "build", "hgk" + ("-" + str(abs(hash(" ".join(EXTRA))
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 ARCH = os.environ.get("HGK_ARCH", "gfx950")
 FLAGS = ["-O3", "-std=c++17", "-fPIC", f"--offload-arch={ARCH}", "-I" + os.path.join(ROOT, "include"),
-         "-Wno-unused-result"] + EXTRA
+         "-Wno-unused-result",
+         # no packed fp32 arithmetic: some of its forms have given wrong results on this part
+         "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"] + EXTRA
 
 
 def sources():
