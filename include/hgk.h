@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define HGK_ABI_VERSION 39
+#define HGK_ABI_VERSION 40
 
 enum { HGK_F32 = 0, HGK_BF16 = 1 };
 enum { HGK_OK = 0, HGK_ERR_ARG = -1, HGK_ERR_UNSUPPORTED = -2, HGK_ERR_HIP = -3 };
@@ -657,6 +657,61 @@ int hgk_topk_select(hgk_stream_t stream, const float* values, int rows, long L, 
 int hgk_adam_step(hgk_stream_t stream, float* param, const float* grad, float* exp_avg,
                   float* exp_avg_sq, long n, float lr, float beta1, float beta2, float eps,
                   float weight_decay, float* step_state);
+
+/* ---- feed-forward block over rows of channels (ABI 40) ----
+ * Rows are pixels of an NHWC map (or tokens): dense [M][C]. Weights are [out][in], element type
+ * `dtype` like the activations; gradients have the type of what they are gradients of. Every
+ * pointer on a 16-byte border. Sums are fp32 (int32 in the 8-bit products); M = 0 is allowed (a
+ * weight gradient over no rows is zero).
+ * Activations of the gated product: x sigmoid(x), x Phi(x) (erf), max(x, 0), sigmoid(x). */
+enum { HGK_ACT_SILU = 0, HGK_ACT_GELU = 1, HGK_ACT_RELU = 2, HGK_ACT_SIGMOID = 3, HGK_ACT_COUNT = 4 };
+/* h [M][F] = act(x wg^T) * (x wu^T); x [M][C], wg / wu [F][C]. workspace: hgk_gated_workspace()
+ * bytes (0 unless rows of C elements are no multiple of 16 bytes). */
+size_t hgk_gated_workspace(int dtype, long M, int C, int F, int backward);
+int hgk_gated_fwd(hgk_stream_t stream, int dtype, const void* x, const void* wg, const void* wu,
+                  void* h, long M, int C, int F, int act, void* workspace, size_t ws_bytes);
+/* its backward from dh [M][F]; nothing is kept from the forward (both products are computed again).
+ * dx [M][C] nullable; dwg / dwu [F][C] both or neither. Overwrites its outputs. */
+int hgk_gated_bwd(hgk_stream_t stream, int dtype, const void* x, const void* wg, const void* wu,
+                  const void* dh, void* dx, void* dwg, void* dwu, long M, int C, int F, int act,
+                  void* workspace, size_t ws_bytes);
+/* Dropout mask of a [rows][C] tensor, a function of (seed, offset + *step, row / rows_per_mask,
+ * channel) only: 16 bits an element of Philox4x32-10 (counter: 8-channel group of the mask row |
+ * offset, key: seed); dropped when below floor(65536 p + 1/2), else scaled by the inverse of the
+ * probability that is in fact kept. step: nullable device counter, so that a captured graph draws
+ * another mask at each replay. Dropped values are selected away (an infinity there does not reach y).
+ * y = D(x) + res (res nullable, may alias y, as may x). Its backward is the same call on dy without res. */
+int hgk_dropout_add(hgk_stream_t stream, int dtype, const void* x, const void* res, void* y, long rows,
+                    int C, long rows_per_mask, double p, unsigned long long seed,
+                    unsigned long long offset, const unsigned long long* step);
+/* y [M][N] = res + D(x w^T), x [M][K], w [N][K], res nullable, D as hgk_dropout_add's with
+ * rows_per_mask = 1 over y's elements, in the product's epilogue. */
+size_t hgk_linear_workspace(int dtype, long M, int K, int N, int dropout, int backward);
+int hgk_linear_fwd(hgk_stream_t stream, int dtype, const void* x, const void* w, const void* res,
+                   void* y, long M, int K, int N, double p, unsigned long long seed,
+                   unsigned long long offset, const unsigned long long* step, void* workspace,
+                   size_t ws_bytes);
+/* dx [M][K], dw [N][K] (each nullable) from dy [M][N], the mask drawn again; the residual's
+ * gradient is dy itself. */
+int hgk_linear_bwd(hgk_stream_t stream, int dtype, const void* x, const void* w, const void* dy,
+                   void* dx, void* dw, long M, int K, int N, double p, unsigned long long seed,
+                   unsigned long long offset, const unsigned long long* step, void* workspace,
+                   size_t ws_bytes);
+/* scale[r] = max |x[r]| / 127 (fp32), q[r][k] = rint(x[r][k] / scale[r]) (a row of zeros: 0; a row
+ * that holds an infinity or a NaN: scale NaN). x [rows][K] of `dtype`, q int8. */
+int hgk_quantize_rows_i8(hgk_stream_t stream, int dtype, const void* x, void* q, float* scale, long rows,
+                         int K);
+/* y [M][N] (of `dtype`, like x [M][K]) = s_m wscale_n sum_k q[m][k] wq[n][k] + bias[n] + res[m][n],
+ * with q and s_m of hgk_quantize_rows_i8; wq [N][K] int8, K <= 2^17 (exact int32 sums); bias (fp32)
+ * and res nullable */
+size_t hgk_linear_i8_workspace(long M, int K, int N, int gated);
+int hgk_linear_i8(hgk_stream_t stream, int dtype, const void* x, const void* wq, const float* wscale,
+                  const float* bias, const void* res, void* y, long M, int K, int N,
+                  void* workspace, size_t ws_bytes);
+/* h [M][F] = act(G) * U of two such products */
+int hgk_gated_i8(hgk_stream_t stream, int dtype, const void* x, const void* wqg, const float* sg,
+                 const void* wqu, const float* su, void* h, long M, int C, int F, int act,
+                 void* workspace, size_t ws_bytes);
 
 #ifdef __cplusplus
 }

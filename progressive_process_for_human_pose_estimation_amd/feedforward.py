@@ -1,0 +1,437 @@
+"""A gated feed-forward block over the channels of a feature map on HIP kernels (csrc/hgk_ffn.hip,
+hgk_dropout.hip, hgk_linear_i8.hip), for training and, in 8-bit integers, for serving.
+
+    gated_linear(x, w_gate, w_up, activation)             act(x w_gate^T) * (x w_up^T)
+    linear_dropout_add(x, w, residual, p, seed, offset)   residual + dropout(x w^T)
+    dropout_add(x, residual, p, seed, offset)             residual + dropout(x)
+    quantize_rows(x)                                      int8 rows and a scale for each
+    linear_i8(x, w, w_scale, bias, residual)              the product in 8-bit integers
+    gated_linear_i8(x, wg, sg, wu, su, activation)        the gated product in 8-bit integers
+    Dropout, GatedFeedForward, GatedFeedForwardI8         the modules made of them
+
+Activations are channels-last: [..., C] fp32 or bf16 on the GPU (an NCHW map in channels_last
+memory is `x.permute(0, 2, 3, 1)`, without a copy). Weights are [out, in] in the activations' type;
+gradients have the type of what they belong to. Sums are fp32 (int32 in the 8-bit products), rounded
+once. Other strides, and views that do not start on a 16-byte border, are copied first.
+
+Dropout's mask is a function of (seed, offset, element) and never stored: the backward draws it
+again. An element is dropped with probability p to the nearest 2^-16 and the rest is scaled by the
+inverse of the probability that is kept. The same (seed, offset) gives the same mask: pass another
+offset for each use. `step`, an int64 GPU tensor of one element, is added to the offset on the
+device, so that a captured graph draws other masks at each replay; it must not change between a
+forward and its backward. Everything here can be captured; there is no CPU fallback.
+"""
+import math
+
+import torch
+import torch.nn as nn
+
+from . import hgk as H
+
+ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
+_DTYPES = {torch.float32: H.F32, torch.bfloat16: H.BF16}
+_U64 = 1 << 64
+
+
+def _code(what, x):
+    dt = _DTYPES.get(x.dtype)
+    if dt is None:
+        raise H.HgkError(f"{what}: unsupported dtype {x.dtype} (float32 or bfloat16)")
+    return dt
+
+
+def _act(activation):
+    a = ACTIVATIONS.get(activation)
+    if a is None:
+        raise H.HgkError(f"unknown activation {activation!r}: expected one of {sorted(ACTIVATIONS)}")
+    return a
+
+
+def _dense(t):
+    """t as the kernels read it: dense, on a 16-byte border"""
+    if not t.is_contiguous():
+        t = t.contiguous()
+    return t.clone() if t.data_ptr() & 15 else t
+
+
+def _check(what, x, k, *others):
+    """x [..., k] and the other operands: on one GPU, in x's type (None: any)"""
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise H.HgkError(f"{what}: expected rows of {k} channels, got shape {tuple(x.shape)}")
+    for t, dtype in others:
+        if t is None:
+            continue
+        if t.device != x.device:
+            raise H.HgkError(f"{what}: operands on {x.device} and {t.device}")
+        if t.dtype != dtype:
+            raise H.HgkError(f"{what}: expected {dtype}, got {t.dtype}")
+
+
+def _gpu(what, x):
+    if not x.is_cuda:
+        raise H.HgkError(f"{what}: tensors must live on the GPU")
+
+
+def _check_weights(what, *ws):
+    w = ws[0]
+    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1 or any(v.shape != w.shape for v in ws):
+        raise H.HgkError(f"{what}: weights are [out, in], got {[tuple(v.shape) for v in ws]}")
+
+
+def _check_dropout(p, seed, offset, step, device):
+    if not 0.0 <= p <= 1.0:
+        raise H.HgkError(f"dropout: p = {p} is no probability")
+    if not (0 <= seed < _U64 and 0 <= offset < _U64):
+        raise H.HgkError("dropout: seed and offset are whole numbers of 64 bits")
+    if step is not None and (step.dtype != torch.int64 or step.numel() != 1 or step.device != device):
+        raise H.HgkError(f"dropout: step is an int64 tensor of one element on {device}")
+
+
+def _grads(*ts):
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+class _on:
+    """The device of a tensor made current for a call, where it is not already."""
+
+    def __init__(self, t):
+        self.guard = None
+        if t.device.index != torch.cuda.current_device():
+            self.guard = torch.cuda.device(t.device)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+        return torch.cuda.current_stream().cuda_stream
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+        return False
+
+
+def _workspace(n, x):
+    """(pointer, bytes, owner) of a scratch buffer of the call's stream"""
+    if not n:
+        return None, 0, None
+    ws = torch.empty(n, dtype=torch.uint8, device=x.device)
+    return ws.data_ptr(), n, ws
+
+
+# ---- the gated product ----
+def _gated_fwd(x, wg, wu, act):
+    F, C = wg.shape
+    M, dt, lib = x.numel() // C, _DTYPES[x.dtype], H.lib()
+    with _on(x) as st:
+        h = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
+        wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, 0), x)
+        H.check(lib.hgk_gated_fwd(st, dt, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), M, C,
+                                  F, act, wp, n))
+    return h
+
+
+class _Gated(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, act):
+        x, wg, wu = _dense(x), _dense(wg), _dense(wu)
+        ctx.save_for_backward(x, wg, wu)
+        ctx.act = act
+        return _gated_fwd(x, wg, wu, act)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dh):
+        x, wg, wu = ctx.saved_tensors
+        F, C = wg.shape
+        M, dt, lib = x.numel() // C, _DTYPES[x.dtype], H.lib()
+        with _on(x) as st:
+            dh = _dense(dh)
+            dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+            dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+            dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if dw else (None, None)
+            wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, 1), x)
+            H.check(lib.hgk_gated_bwd(st, dt, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), dh.data_ptr(),
+                                      H.ptr(dx), H.ptr(dwg), H.ptr(dwu), M, C, F, ctx.act, wp, n))
+        return dx, dwg, dwu, None
+
+
+def gated_linear(x, w_gate, w_up, activation="silu"):
+    """act(x w_gate^T) * (x w_up^T): x [..., C], w_gate and w_up [F, C] -> [..., F]. Both products, the
+    activation and the product of the two in one kernel; the backward computes them again and keeps
+    nothing but the inputs. activation: silu, gelu (erf), relu, sigmoid."""
+    _check_weights("gated_linear", w_gate, w_up)
+    _check("gated_linear", x, w_gate.shape[1], (w_gate, x.dtype), (w_up, x.dtype))
+    _code("gated_linear", x)
+    act = _act(activation)
+    _gpu("gated_linear", x)
+    if _grads(x, w_gate, w_up):
+        return _Gated.apply(x, w_gate, w_up, act)
+    return _gated_fwd(_dense(x), _dense(w_gate), _dense(w_up), act)
+
+
+# ---- product, dropout and residual ----
+def _linear_fwd(x, w, res, p, seed, offset, step):
+    N, K = w.shape
+    M, dt, lib = x.numel() // K, _DTYPES[x.dtype], H.lib()
+    with _on(x) as st:
+        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+        wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, p > 0, 0), x)
+        H.check(lib.hgk_linear_fwd(st, dt, x.data_ptr(), w.data_ptr(), H.ptr(res), y.data_ptr(), M, K, N,
+                                   p, seed, offset, H.ptr(step), wp, n))
+    return y
+
+
+class _Linear(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, res, p, seed, offset, step):
+        x, w = _dense(x), _dense(w)
+        ctx.save_for_backward(x, w, step)
+        ctx.drop = (p, seed, offset)
+        return _linear_fwd(x, w, None if res is None else _dense(res), p, seed, offset, step)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, w, step = ctx.saved_tensors
+        p, seed, offset = ctx.drop
+        N, K = w.shape
+        M, dt, lib = x.numel() // K, _DTYPES[x.dtype], H.lib()
+        dx = dw = None
+        if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
+            with _on(x) as st:
+                g = _dense(dy)
+                dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+                dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
+                wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, p > 0, 1), x)
+                H.check(lib.hgk_linear_bwd(st, dt, x.data_ptr(), w.data_ptr(), g.data_ptr(), H.ptr(dx),
+                                           H.ptr(dw), M, K, N, p, seed, offset, H.ptr(step), wp, n))
+        return dx, dw, dy if ctx.needs_input_grad[2] else None, None, None, None, None
+
+
+def linear_dropout_add(x, w, residual=None, p=0.0, seed=0, offset=0, step=None):
+    """residual + dropout(x w^T): x [..., K], w [N, K], residual [..., N] or None -> [..., N]; dropout
+    and residual in the product's epilogue. The mask is dropout_add's over the output."""
+    _check_weights("linear_dropout_add", w)
+    _check("linear_dropout_add", x, w.shape[1], (w, x.dtype), (residual, x.dtype))
+    _code("linear_dropout_add", x)
+    if residual is not None and residual.shape != (*x.shape[:-1], w.shape[0]):
+        raise H.HgkError(f"linear_dropout_add: residual of shape {tuple(residual.shape)}")
+    _check_dropout(p, seed, offset, step, x.device)
+    _gpu("linear_dropout_add", x)
+    if _grads(x, w, residual):
+        return _Linear.apply(x, w, residual, p, seed, offset, step)
+    return _linear_fwd(_dense(x), _dense(w), None if residual is None else _dense(residual), p, seed,
+                       offset, step)
+
+
+# ---- dropout ----
+def _dropout(x, res, rows_per_mask, p, seed, offset, step):
+    C = x.shape[-1]
+    with _on(x) as st:
+        y = torch.empty_like(x)
+        if x.numel():
+            H.check(H.lib().hgk_dropout_add(st, _DTYPES[x.dtype], x.data_ptr(), H.ptr(res), y.data_ptr(),
+                                            x.numel() // C, C, rows_per_mask, p, seed, offset,
+                                            H.ptr(step)))
+    return y
+
+
+class _DropoutAdd(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, res, rows_per_mask, p, seed, offset, step):
+        ctx.save_for_backward(step)
+        ctx.args = (rows_per_mask, p, seed, offset)
+        return _dropout(_dense(x), None if res is None else _dense(res), rows_per_mask, p, seed, offset, step)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        step, = ctx.saved_tensors
+        dx = _dropout(_dense(dy), None, *ctx.args, step) if ctx.needs_input_grad[0] else None
+        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
+
+
+def dropout_add(x, residual=None, p=0.5, seed=0, offset=0, step=None, rows_per_mask=1):
+    """residual + dropout(x) over [..., C]. rows_per_mask: that many consecutive rows share a mask row
+    (H * W of an NHWC map drops whole channels of each image); what is dropped is selected away, so
+    an infinity or NaN there does not reach the result."""
+    if x.dim() < 1:
+        raise H.HgkError("dropout_add: expected [..., C]")
+    _check("dropout_add", x, x.shape[-1], (residual, x.dtype))
+    _code("dropout_add", x)
+    if residual is not None and residual.shape != x.shape:
+        raise H.HgkError(f"dropout_add: residual of shape {tuple(residual.shape)} to {tuple(x.shape)}")
+    if rows_per_mask < 1:
+        raise H.HgkError(f"dropout_add: rows_per_mask = {rows_per_mask}")
+    _check_dropout(p, seed, offset, step, x.device)
+    _gpu("dropout_add", x)
+    if _grads(x, residual):
+        return _DropoutAdd.apply(x, residual, rows_per_mask, p, seed, offset, step)
+    return _dropout(_dense(x), None if residual is None else _dense(residual), rows_per_mask, p, seed,
+                    offset, step)
+
+
+# ---- 8-bit integers ----
+@torch.no_grad()
+def quantize_rows(x):
+    """(q int8 [..., K], scale fp32 [...]): scale = max |row| / 127, q = rint(row / scale). A row of
+    zeros has scale 0; a row that holds an infinity or a NaN has scale NaN."""
+    _check("quantize_rows", x, x.shape[-1] if x.dim() else 0)
+    dt = _code("quantize_rows", x)
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise H.HgkError("quantize_rows: expected [..., K]")
+    _gpu("quantize_rows", x)
+    x = _dense(x)
+    with _on(x) as st:
+        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+        s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+        H.check(H.lib().hgk_quantize_rows_i8(st, dt, x.data_ptr(), q.data_ptr(), s.data_ptr(), s.numel(),
+                                             x.shape[-1]))
+    return q, s
+
+
+def _scale(what, s, n):
+    if s is not None and tuple(s.shape) != (n,):
+        raise H.HgkError(f"{what}: expected {n} values, got shape {tuple(s.shape)}")
+    return None if s is None else _dense(s)
+
+
+@torch.no_grad()
+def linear_i8(x, w, w_scale, bias=None, residual=None):
+    """x w^T (+ bias + residual) in 8-bit integers: x [..., K] fp32 / bf16 is quantised row by row
+    (quantize_rows), w is int8 [N, K] with w_scale fp32 [N] (quantize_rows of the weights), bias fp32
+    [N], residual [..., N] in x's type, which is the result's. The integer sums are exact (K <=
+    131072). No gradient."""
+    _check_weights("linear_i8", w)
+    N, K = w.shape
+    _check("linear_i8", x, K, (w, torch.int8), (w_scale, torch.float32), (bias, torch.float32),
+           (residual, x.dtype))
+    dt = _code("linear_i8", x)
+    if residual is not None:
+        if residual.shape != (*x.shape[:-1], N):
+            raise H.HgkError(f"linear_i8: residual of shape {tuple(residual.shape)}")
+    w_scale, bias = _scale("linear_i8", w_scale, N), _scale("linear_i8", bias, N)
+    _gpu("linear_i8", x)
+    x, w = _dense(x), _dense(w)
+    residual = None if residual is None else _dense(residual)
+    M, lib = x.numel() // K, H.lib()
+    with _on(x) as st:
+        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
+        wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, K, N, 0), x)
+        H.check(lib.hgk_linear_i8(st, dt, x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), H.ptr(bias),
+                                  H.ptr(residual), y.data_ptr(), M, K, N, wp, n))
+    return y
+
+
+@torch.no_grad()
+def gated_linear_i8(x, w_gate, gate_scale, w_up, up_scale, activation="silu"):
+    """gated_linear with both products in 8-bit integers (see linear_i8): w_gate and w_up int8 [F, C]
+    with a scale for each row. No gradient."""
+    _check_weights("gated_linear_i8", w_gate, w_up)
+    F, C = w_gate.shape
+    _check("gated_linear_i8", x, C, (w_gate, torch.int8), (w_up, torch.int8), (gate_scale, torch.float32),
+           (up_scale, torch.float32))
+    dt = _code("gated_linear_i8", x)
+    act = _act(activation)
+    sg, su = _scale("gated_linear_i8", gate_scale, F), _scale("gated_linear_i8", up_scale, F)
+    _gpu("gated_linear_i8", x)
+    x, wg, wu = _dense(x), _dense(w_gate), _dense(w_up)
+    M, lib = x.numel() // C, H.lib()
+    with _on(x) as st:
+        h = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
+        wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, C, F, 1), x)
+        H.check(lib.hgk_gated_i8(st, dt, x.data_ptr(), wg.data_ptr(), sg.data_ptr(), wu.data_ptr(),
+                                 su.data_ptr(), h.data_ptr(), M, C, F, act, wp, n))
+    return h
+
+
+# ---- modules ----
+class _Masks(nn.Module):
+    """The (seed, offset, step) of a module's dropout. The seed is drawn from torch's generator at
+    construction (torch.manual_seed governs it); every training call takes the next offset. Under
+    graph capture the host's offset is frozen, so a device counter moves on at each replay and the
+    call keeps the value that it saw for its backward."""
+
+    def __init__(self, p):
+        super().__init__()
+        if not 0.0 <= p <= 1.0:
+            raise H.HgkError(f"dropout: p = {p} is no probability")
+        self.p = p
+        self.seed = int(torch.randint(0, 2 ** 62, (1,)).item())
+        self.calls = 0
+        self.register_buffer("step", torch.zeros(1, dtype=torch.int64), persistent=False)
+
+    def next_mask(self, x):
+        """keyword arguments of the next use, on x's device"""
+        if not self.training or self.p == 0.0:
+            return {"p": 0.0}
+        self.calls = (self.calls + 1) & 0xffffffff
+        step = None
+        if x.is_cuda and torch.cuda.is_current_stream_capturing():
+            if self.step.device != x.device:
+                raise H.HgkError(f"dropout: move the module to {x.device} before capturing it")
+            self.step.add_(1 << 32)
+            step = self.step.clone()
+        return {"p": self.p, "seed": self.seed, "offset": self.calls, "step": step}
+
+
+class Dropout(_Masks):
+    """nn.Dropout over channels-last [..., C] with the skip added in the same pass: forward(x,
+    residual=None). channels=True drops whole channels of each image of an NHWC map (nn.Dropout2d)."""
+
+    def __init__(self, p=0.5, channels=False):
+        super().__init__(p)
+        self.channels = channels
+
+    def forward(self, x, residual=None):
+        kw = self.next_mask(x)
+        if kw["p"] == 0.0 and residual is None:
+            return x
+        rows = 1
+        if self.channels:
+            if x.dim() < 3:
+                raise H.HgkError("Dropout(channels=True): expected an NHWC map")
+            rows = max(1, math.prod(x.shape[1:-1]))
+        return dropout_add(x, residual, rows_per_mask=rows, **kw)
+
+
+class GatedFeedForward(_Masks):
+    """x + dropout(w_down (act(w_gate x) * (w_up x))) over channels-last [..., channels]. Parameters
+    are fp32 [out, in] with nn.Linear's initialisation and are cast to x's type in each call, so that
+    bf16 maps train fp32 masters. quantized() gives the block in 8-bit integers for serving."""
+
+    def __init__(self, channels, hidden, activation="silu", p=0.0, residual=True):
+        super().__init__(p)
+        _act(activation)
+        self.activation, self.residual = activation, residual
+        self.w_gate = nn.Parameter(torch.empty(hidden, channels))
+        self.w_up = nn.Parameter(torch.empty(hidden, channels))
+        self.w_down = nn.Parameter(torch.empty(channels, hidden))
+        for w in (self.w_gate, self.w_up, self.w_down):
+            nn.init.kaiming_uniform_(w, a=math.sqrt(5))
+
+    def forward(self, x):
+        h = gated_linear(x, self.w_gate.to(x.dtype), self.w_up.to(x.dtype), self.activation)
+        return linear_dropout_add(h, self.w_down.to(x.dtype), x if self.residual else None,
+                                  **self.next_mask(x))
+
+    def quantized(self):
+        return GatedFeedForwardI8(self)
+
+
+class GatedFeedForwardI8(nn.Module):
+    """A GatedFeedForward served in 8-bit integers: weights quantised once, with a scale for each
+    output channel; activations row by row in each call. No dropout, no gradients."""
+
+    def __init__(self, block):
+        super().__init__()
+        self.activation, self.residual = block.activation, block.residual
+        for name in ("gate", "up", "down"):
+            q, s = quantize_rows(getattr(block, "w_" + name).detach())
+            self.register_buffer("w_" + name, q)
+            self.register_buffer(name + "_scale", s)
+
+    @torch.no_grad()
+    def forward(self, x):
+        h = gated_linear_i8(x, self.w_gate, self.gate_scale, self.w_up, self.up_scale, self.activation)
+        return linear_i8(h, self.w_down, self.down_scale, residual=x if self.residual else None)

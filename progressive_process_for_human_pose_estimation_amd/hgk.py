@@ -13,13 +13,15 @@ LIB_PATH = os.path.join(_PKG, "libhgk.so")
 
 F32, BF16 = 0, 1
 UP_BILINEAR_AC, UP_NEAREST = 0, 1
-ABI_VERSION = 39
+ABI_VERSION = 40
 
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
 _c_long = ctypes.c_long
 _c_float = ctypes.c_float
 _c_size_t = ctypes.c_size_t
+_c_double = ctypes.c_double
+_c_u64 = ctypes.c_ulonglong
 _c_intp = ctypes.POINTER(ctypes.c_int)
 
 
@@ -257,6 +259,24 @@ SIGNATURES = {
                                        _c_int, _c_float, _c_int]),
     "hgk_adam_step": (_c_int, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_long, _c_float,
                                _c_float, _c_float, _c_float, _c_float, _c_void_p]),
+    "hgk_gated_workspace": (_c_size_t, [_c_int, _c_long, _c_int, _c_int, _c_int]),
+    "hgk_gated_fwd": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_long, _c_int, _c_int, _c_int,
+                               _c_void_p, _c_size_t]),
+    "hgk_gated_bwd": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 7 + [_c_long, _c_int, _c_int, _c_int,
+                               _c_void_p, _c_size_t]),
+    "hgk_dropout_add": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_long, _c_int, _c_long,
+                                 _c_double, _c_u64, _c_u64, _c_void_p]),
+    "hgk_linear_workspace": (_c_size_t, [_c_int, _c_long] + [_c_int] * 4),
+    "hgk_linear_fwd": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_long, _c_int, _c_int,
+                                _c_double, _c_u64, _c_u64, _c_void_p, _c_void_p, _c_size_t]),
+    "hgk_linear_bwd": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 5 + [_c_long, _c_int, _c_int,
+                                _c_double, _c_u64, _c_u64, _c_void_p, _c_void_p, _c_size_t]),
+    "hgk_quantize_rows_i8": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_long, _c_int]),
+    "hgk_linear_i8_workspace": (_c_size_t, [_c_long, _c_int, _c_int, _c_int]),
+    "hgk_linear_i8": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_long, _c_int, _c_int,
+                               _c_void_p, _c_size_t]),
+    "hgk_gated_i8": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 6 + [_c_long, _c_int, _c_int, _c_int,
+                              _c_void_p, _c_size_t]),
 }
 
 _lib = None

@@ -1,0 +1,154 @@
+"""The feed-forward operators without a GPU: what the C ABI and the Python layer refuse, and the test
+oracle against published vectors and differences."""
+import numpy as np
+import pytest
+import torch
+
+import feedforward_oracle as R
+from progressive_process_for_human_pose_estimation_amd import feedforward as F
+from progressive_process_for_human_pose_estimation_amd import hgk as H
+
+A = 1 << 20  # an address on a 16-byte border: never read, the calls are refused before any launch
+
+
+def refused(rc, text):
+    msg = H.lib().hgk_last_error().decode()
+    assert rc == -1 and text in msg, (rc, msg)
+
+
+def test_philox_vectors():
+    """Known answers of Philox4x32-10 (published with the generator)"""
+    z = R.philox(np.zeros((1, 4), np.uint64), (0, 0))[0]
+    assert [int(v) for v in z] == [0x6627e8d5, 0xe169c58d, 0xbc57ac4c, 0x9b00dbd8]
+    f = R.philox(np.full((1, 4), 0xffffffff, np.uint64), (0xffffffff, 0xffffffff))[0]
+    assert [int(v) for v in f] == [0x408f276d, 0x41c83b0e, 0xa20bc7c6, 0x6d5451fd]
+
+
+def test_oracle_mask_share_and_sharing():
+    k = R.kept(4096, 64, 0.25, 7, 3)
+    # 262144 independent draws: five standard deviations of the share
+    assert abs(float(k.double().mean()) - 0.75) < 5 * (0.25 * 0.75 / k.numel()) ** 0.5
+    assert not torch.equal(k, R.kept(4096, 64, 0.25, 7, 4)) and not torch.equal(k, R.kept(4096, 64, 0.25, 8, 3))
+    c = R.kept(100, 13, 0.5, 1, 2, rows_per_mask=30)
+    assert torch.equal(c[0], c[29]) and not torch.equal(c[:30], c[30:60])
+    assert bool(R.kept(9, 9, 0.0, 1, 2).all()) and not bool(R.kept(9, 9, 1.0, 1, 2).any())
+
+
+@pytest.mark.parametrize("name", sorted(F.ACTIVATIONS))
+def test_oracle_gradients_against_differences(name):
+    g = torch.Generator().manual_seed(5)
+    x, wg, wu, dh = (torch.randn(*s, generator=g, dtype=torch.float64) for s in ((5, 7), (6, 7), (6, 7), (5, 6)))
+    (_, _), (dx, _), (dwg, _), (dwu, _) = R.gated(x, wg, wu, name, torch.float32, dh)
+    for t, d in ((0, dx), (1, dwg), (2, dwu)):
+        args = [x, wg, wu]
+        v = torch.randn(args[t].shape, generator=g, dtype=torch.float64)
+        e = 1e-6
+        f = [float((R.gated(*[a + s * e * v if i == t else a for i, a in enumerate(args)], name,
+                            torch.float32)[0] * dh).sum()) for s in (1, -1)]
+        # central difference: e^2 times a third derivative of order 1e2, rounding 1e-16 / e
+        assert abs((f[0] - f[1]) / (2 * e) - float((d * v).sum())) < 1e-6
+
+
+def test_abi_refusals():
+    L = H.load_library()
+    big = 1 << 40
+    refused(L.hgk_gated_fwd(None, 0, None, A, A, A, 4, 8, 8, 0, None, 0), "null")
+    refused(L.hgk_gated_fwd(None, 0, A + 4, A, A, A, 4, 8, 8, 0, None, 0), "16-byte")
+    refused(L.hgk_gated_fwd(None, 0, A, A, A, A, 4, 8, 8, 4, None, 0), "activation")
+    refused(L.hgk_gated_fwd(None, 0, A, A, A, A, 4, 0, 8, 0, None, 0), "bad sizes")
+    refused(L.hgk_gated_fwd(None, 0, A, A, A, A, -1, 8, 8, 0, None, 0), "bad sizes")
+    refused(L.hgk_gated_fwd(None, 7, A, A, A, A, 4, 8, 8, 0, None, 0), "dtype")
+    refused(L.hgk_gated_fwd(None, 1, A, A, A, A, 4, 9, 8, 0, A, 16), "too small")
+    refused(L.hgk_gated_bwd(None, 0, A, A, A, A, A, A, None, 4, 8, 8, 0, A, big), "both")
+    refused(L.hgk_gated_bwd(None, 0, A, A, A, A, A, A, A, 4, 8, 8, 0, None, big), "too small")
+    refused(L.hgk_gated_bwd(None, 0, A, A, A, A, A, A, A, 4, 8, 8, 0, A, 16), "too small")
+    refused(L.hgk_dropout_add(None, 0, A, None, A, 4, 8, 1, 1.5, 0, 0, None), "probability")
+    refused(L.hgk_dropout_add(None, 0, A, None, A, 4, 8, 1, float("nan"), 0, 0, None), "probability")
+    refused(L.hgk_dropout_add(None, 0, A, None, A, 4, 8, 0, 0.5, 0, 0, None), "rows_per_mask")
+    refused(L.hgk_dropout_add(None, 0, None, None, A, 4, 8, 1, 0.5, 0, 0, None), "null")
+    refused(L.hgk_dropout_add(None, 0, A, None, A, 4, 0, 1, 0.5, 0, 0, None), "bad sizes")
+    refused(L.hgk_dropout_add(None, 5, A, None, A, 4, 8, 1, 0.5, 0, 0, None), "dtype")
+    refused(L.hgk_linear_fwd(None, 0, A, None, None, A, 4, 8, 8, 0.0, 0, 0, None, None, 0), "null")
+    refused(L.hgk_linear_fwd(None, 0, A, A, A + 2, A, 4, 8, 8, 0.0, 0, 0, None, None, 0), "16-byte")
+    refused(L.hgk_linear_fwd(None, 0, A, A, None, A, 4, 8, 8, -0.1, 0, 0, None, None, 0), "probability")
+    refused(L.hgk_linear_bwd(None, 1, A, A, A, A, A, 4, 8, 8, 0.5, 0, 0, None, A, 16), "too small")
+    refused(L.hgk_quantize_rows_i8(None, 0, A, A, A, 4, (1 << 17) + 1), "bad sizes")
+    refused(L.hgk_quantize_rows_i8(None, 0, A, None, A, 4, 8), "null")
+    refused(L.hgk_linear_i8(None, 0, A, A, A, None, None, A, 4, (1 << 17) + 1, 8, A, big), "bad sizes")
+    refused(L.hgk_linear_i8(None, 0, A, A, A, None, None, A, 4, 8, 8, A, 8), "too small")
+    refused(L.hgk_linear_i8(None, 0, A, A, None, None, None, A, 4, 8, 8, A, big), "null")
+    refused(L.hgk_gated_i8(None, 0, A, A, A, A, A, A, 4, 8, 8, 9, A, big), "activation")
+    refused(L.hgk_gated_i8(None, 0, A, A + 8, A, A, A, A, 4, 8, 8, 0, A, big), "16-byte")
+
+
+def test_no_rows_launches_nothing():
+    L = H.load_library()
+    assert L.hgk_gated_fwd(None, 0, None, None, None, None, 0, 8, 8, 0, None, 0) == 0
+    assert L.hgk_dropout_add(None, 0, None, None, None, 0, 8, 1, 0.5, 0, 0, None) == 0
+    assert L.hgk_linear_fwd(None, 0, None, None, None, None, 0, 8, 8, 0.0, 0, 0, None, None, 0) == 0
+    assert L.hgk_linear_i8(None, 0, None, None, None, None, None, None, 0, 8, 8, None, 0) == 0
+
+
+def test_workspaces():
+    L = H.load_library()
+    assert L.hgk_gated_workspace(1, 4096, 256, 1024, 0) == 0       # rows of whole 16-byte chunks
+    assert L.hgk_gated_workspace(1, 4096, 257, 1024, 0) >= 4096 * 264 * 2 + 2 * 1024 * 264 * 2
+    assert L.hgk_gated_workspace(1, 4096, 256, 1024, 1) >= 2 * 4096 * 1024 * 2
+    assert L.hgk_linear_i8_workspace(100, 64, 64, 0) >= 100 * 64 + 100 * 4
+    for bad in ((7, 4, 8, 8, 0), (0, 0, 8, 8, 0), (0, 4, 0, 8, 1)):
+        assert L.hgk_gated_workspace(*bad) == 0
+
+
+def t(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+BAD = [
+    (lambda: F.gated_linear(t(4, 8), t(6, 8), t(6, 8)), "GPU"),
+    (lambda: F.gated_linear(t(4, 8), t(6, 8), t(5, 8)), "weights"),
+    (lambda: F.gated_linear(t(4, 8), t(6, 8, 1), t(6, 8, 1)), "weights"),
+    (lambda: F.gated_linear(t(4, 9), t(6, 8), t(6, 8)), "rows of 8"),
+    (lambda: F.gated_linear(t(4, 8), t(6, 8), t(6, 8), "tanh"), "activation"),
+    (lambda: F.gated_linear(t(4, 8), t(6, 8), t(6, 8, dtype=torch.bfloat16)), "expected"),
+    (lambda: F.gated_linear(t(4, 8).half(), t(6, 8).half(), t(6, 8).half()), "dtype"),
+    (lambda: F.gated_linear(t(4, 8), t(6, 8, dtype=torch.float32).to("meta"), t(6, 8)), "operands on"),
+    (lambda: F.linear_dropout_add(t(4, 8), t(6, 8)), "GPU"),
+    (lambda: F.linear_dropout_add(t(4, 8), t(6, 8), t(1, 6)), "residual"),
+    (lambda: F.linear_dropout_add(t(4, 8), t(6, 8), p=1.01), "probability"),
+    (lambda: F.linear_dropout_add(t(4, 8), t(6, 8), p=0.1, seed=1 << 64), "64 bits"),
+    (lambda: F.linear_dropout_add(t(4, 8), t(6, 8), p=0.1, step=t(1)), "step"),
+    (lambda: F.dropout_add(t(4, 8)), "GPU"),
+    (lambda: F.dropout_add(torch.tensor(1.0)), "expected"),
+    (lambda: F.dropout_add(t(4, 8), t(4, 7)), "residual"),
+    (lambda: F.dropout_add(t(4, 8), rows_per_mask=0), "rows_per_mask"),
+    (lambda: F.dropout_add(t(4, 8), p=-0.1), "probability"),
+    (lambda: F.dropout_add(t(4, 8), offset=-1), "64 bits"),
+    (lambda: F.quantize_rows(t(4, 8)), "GPU"),
+    (lambda: F.quantize_rows(t(4, 8, dtype=torch.int32)), "dtype"),
+    (lambda: F.linear_i8(t(4, 8), t(6, 8, dtype=torch.int8), t(6)), "GPU"),
+    (lambda: F.linear_i8(t(4, 8), t(6, 8), t(6)), "expected"),
+    (lambda: F.linear_i8(t(4, 8), t(6, 8, dtype=torch.int8), t(5)), "6 values"),
+    (lambda: F.linear_i8(t(4, 8), t(6, 8, dtype=torch.int8), t(6), residual=t(4, 5)), "residual"),
+    (lambda: F.gated_linear_i8(t(4, 8), t(6, 8, dtype=torch.int8), t(6), t(6, 8, dtype=torch.int8), t(7)), "6 values"),
+    (lambda: F.Dropout(2.0), "probability"),
+    (lambda: F.GatedFeedForward(8, 16, activation="tanh"), "activation"),
+]
+
+
+@pytest.mark.parametrize("i", range(len(BAD)))
+def test_python_refusals(i):
+    call, text = BAD[i]
+    with pytest.raises(H.HgkError, match=text):
+        call()
+
+
+def test_module_masks_advance_and_follow_the_seed():
+    torch.manual_seed(3)
+    a = F.GatedFeedForward(8, 16, p=0.1)
+    torch.manual_seed(3)
+    b = F.GatedFeedForward(8, 16, p=0.1)
+    assert a.seed == b.seed and torch.equal(a.w_gate, b.w_gate)
+    m = [a.next_mask(t(2, 8)) for _ in range(3)]
+    assert len({v["offset"] for v in m}) == 3 and all(v["seed"] == a.seed for v in m)
+    assert a.eval().next_mask(t(2, 8)) == {"p": 0.0}
+    assert set(a.state_dict()) == {"w_gate", "w_up", "w_down"}
