@@ -90,6 +90,9 @@ const char* hgk_last_error(void);
  *                           total, go to ONE halo launch whose splits run over the concatenated
  *                           tiles (each slab read-modified-written once per launch, not per use;
  *                           the other uses take the implicit GEMM multi launch); default 128; 0 = off
+ *   HGK_ROUTE_FFN_TILE      feed-forward products (hgk_gated_*, hgk_linear_*, *_i8) on tiles of 128
+ *                           (128) or 256 rows and columns (256) wherever the tiled kernel runs;
+ *                           0 (default): by the sizes
  * hgk_set_route returns the previous value (HGK_ERR_ARG for an unknown knob); a negative value
  * restores the default. */
 enum {
@@ -109,7 +112,8 @@ enum {
   HGK_ROUTE_IMG_NARROW = 13,
   HGK_ROUTE_WG_RING = 14,
   HGK_ROUTE_WG_HALO_MULTI = 15,
-  HGK_ROUTE_COUNT = 16
+  HGK_ROUTE_FFN_TILE = 16,
+  HGK_ROUTE_COUNT = 17
 };
 long hgk_set_route(int knob, long value);
 long hgk_get_route(int knob);

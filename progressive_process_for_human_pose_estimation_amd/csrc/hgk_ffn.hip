@@ -16,34 +16,12 @@
 
 namespace hgk {
 
-struct GemmPlan {
-  bool big;  // 256-row / column tiles
-  int tiles_m, tiles_n, splits;
-  long slab;  // bytes
-};
-
-// cols: output columns of a tile are `per` times narrower in a gated tile
-static GemmPlan plan_gemm(int dtype, long M, long N, int per, int steps, int batch, bool can_split) {
-  GemmPlan p;
-  const long big = ((M + 255) / 256) * ((N + 256 / per - 1) / (256 / per)) * batch;
-  p.big = dtype == HGK_BF16 && big >= 256;
-  const int b = p.big ? 256 : 128;
-  p.tiles_m = (int)((M + b - 1) / b);
-  p.tiles_n = (int)((N + b / per - 1) / (b / per));
-  const long tiles = (long)p.tiles_m * p.tiles_n * batch;
-  p.splits = 1;
-  if (can_split && tiles * 2 <= (p.big ? 256 : kFillGroups))
-    p.splits = (int)std::max(1l, std::min<long>((p.big ? 256 : kFillGroups) / tiles, steps / 4));
-  p.slab = p.splits > 1 ? (long)p.splits * batch * M * N * 4 : 0;
-  return p;
-}
-
 template <int DT, typename T, int LM, int LN, int EPI>
 static void run_tiles(hipStream_t st, const GemmArgs& a, bool big) {
   const dim3 grid((unsigned)((long)a.tiles_m * a.tiles_n * a.batch * a.splits));
   if constexpr (DT == G_BF16) {
     if (big) {
-      hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 256, 256, 2, 4, EPI, 2>), grid, dim3(512), 0, st, a);
+      hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 256, 256, 4, 2, EPI, 2>), grid, dim3(512), 0, st, a);
       return;
     }
   }
@@ -59,7 +37,7 @@ static int run_product(hipStream_t st, GemmArgs& a, const GemmPlan& p, char* sla
   if (p.splits > 1) {
     run_tiles<DT, T, LM, LN, E_SLAB>(st, a, p.big);
     HGK_LAUNCH_CHECK();
-    const long n = (long)a.batch * a.M * ((a.N + 3) / 4);
+    const long n = (long)a.batch * a.M * ((a.N + 7) / 8);
     hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
   } else {
     run_tiles<DT, T, LM, LN, E_OUT>(st, a, p.big);
@@ -112,7 +90,7 @@ static GatedWs gated_ws(int dtype, long M, int C, int F, bool bwd) {
   GatedWs w;
   const int es = es_of(dtype), q = 16 / es, ks = 128 / es;
   w.Cp = (int)up_to(C, q);
-  w.Fp = (int)up_to(F, q);
+  w.Fp = (int)up_to(F, 8);
   w.pad = w.Cp != C;
   Carve c;
   w.x = w.wg = w.wu = w.dg = w.du = w.slab = 0;
@@ -124,8 +102,8 @@ static GatedWs gated_ws(int dtype, long M, int C, int F, bool bwd) {
   if (bwd) {
     w.dg = c.take(M * w.Fp * es);
     w.du = c.take(M * w.Fp * es);
-    w.dx = plan_gemm(dtype, M, C, 1, 2 * (int)((F + ks - 1) / ks), 1, true);
-    w.dw = plan_gemm(dtype, F, C, 1, (int)((M + ks - 1) / ks), 2, true);
+    w.dx = plan_gemm(dtype == HGK_BF16, M, C, 1, 2 * (int)((F + ks - 1) / ks), 1, true);
+    w.dw = plan_gemm(dtype == HGK_BF16, F, C, 1, (int)((M + ks - 1) / ks), 2, true);
     w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
   }
   w.total = c.at;
@@ -166,13 +144,12 @@ static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* 
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
   a.out = h;
-  a.ldo = F;
   a.act = act;
-  a.vec = F % 4 == 0;
+  a.vec = F % 8 == 0;
   if (M <= kSkinnyRows) {
     run_skinny<DT, T, true>(st, a);
   } else {
-    const GemmPlan p = plan_gemm(dtype, M, F, 2, a.spseg, 1, false);
+    const GemmPlan p = plan_gemm(dtype == HGK_BF16, M, F, 2, a.spseg, 1, false);
     a.tiles_m = p.tiles_m;
     a.tiles_n = p.tiles_n;
     run_tiles<DT, T, L_ROW, L_ROW, E_GATED>(st, a, p.big);
@@ -196,8 +173,8 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
   a.out1 = ws + w.du;
   a.npad = w.Fp;
   a.act = act;
-  a.vec = F % 4 == 0;
-  const GemmPlan p = plan_gemm(dtype, M, F, 2, a.spseg, 1, false);
+  a.vec = F % 8 == 0;
+  const GemmPlan p = plan_gemm(dtype == HGK_BF16, M, F, 2, a.spseg, 1, false);
   a.tiles_m = p.tiles_m;
   a.tiles_n = p.tiles_n;
   run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p.big);
@@ -217,8 +194,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
     b.spseg = (F + ks - 1) / ks;
     b.nseg = 2;
     b.out = dx;
-    b.ldo = C;
-    b.vec = C % 4 == 0;
+    b.vec = C % 8 == 0;
     if (int rc = run_product<DT, T, L_ROW, L_COL>(st, b, w.dx, ws + w.slab)) return rc;
   }
   if (dwg) {
@@ -235,8 +211,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
     b.batch = 2;
     b.out = dwg;
     b.out1 = dwu;
-    b.ldo = C;
-    b.vec = C % 4 == 0;
+    b.vec = C % 8 == 0;
     if (int rc = run_product<DT, T, L_COL, L_COL>(st, b, w.dw, ws + w.slab)) return rc;
   }
   return HGK_OK;
@@ -262,12 +237,12 @@ static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) 
     w.x = c.take(M * w.Kp * es);
     w.w = c.take((long)N * w.Kp * es);
   }
-  w.fwd = plan_gemm(dtype, M, N, 1, (int)((w.Kp + ks - 1) / ks), 1, true);
+  w.fwd = plan_gemm(dtype == HGK_BF16, M, N, 1, (int)((w.Kp + ks - 1) / ks), 1, true);
   if (bwd) {
     if (drop) w.dz = c.take(M * N * es);
     if (w.pad_n) w.dzp = c.take(M * w.Np * es);
-    w.dx = plan_gemm(dtype, M, K, 1, (N + ks - 1) / ks, 1, true);
-    w.dw = plan_gemm(dtype, N, K, 1, (int)((M + ks - 1) / ks), 1, true);
+    w.dx = plan_gemm(dtype == HGK_BF16, M, K, 1, (N + ks - 1) / ks, 1, true);
+    w.dw = plan_gemm(dtype == HGK_BF16, N, K, 1, (int)((M + ks - 1) / ks), 1, true);
     w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
   } else {
     w.slab = c.take(w.fwd.slab);
@@ -295,9 +270,8 @@ static int linear_fwd(hipStream_t st, const void* x, const void* wt, const void*
   a.km = a.kn = w.Kp;
   a.spseg = (int)up_to((long)w.Kp * sizeof(T), 128) / 128;
   a.out = y;
-  a.ldo = N;
   a.res = res;
-  a.vec = N % 4 == 0;
+  a.vec = N % 8 == 0;
   a.drop = d.thr != 0;
   a.d = d;
   if (M <= kSkinnyRows) {
@@ -346,8 +320,7 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
     b.kn = N;
     b.spseg = (N + ks - 1) / ks;
     b.out = dx;
-    b.ldo = K;
-    b.vec = K % 4 == 0;
+    b.vec = K % 8 == 0;
     b.alpha = alpha;
     if (int rc = run_product<DT, T, L_ROW, L_COL>(st, b, w.dx, ws + w.slab)) return rc;
   }
@@ -362,8 +335,7 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
     b.km = b.kn = (int)M;
     b.spseg = (int)((M + ks - 1) / ks);
     b.out = dw;
-    b.ldo = K;
-    b.vec = K % 4 == 0;
+    b.vec = K % 8 == 0;
     b.alpha = alpha;
     if (int rc = run_product<DT, T, L_COL, L_COL>(st, b, w.dw, ws + w.slab)) return rc;
   }

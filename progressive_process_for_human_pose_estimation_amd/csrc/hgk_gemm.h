@@ -18,7 +18,7 @@
 // a lane picks, the LDS side is written in order.
 //
 // The matrix instruction's A operand is the N side and its B operand the M side: a lane then holds
-// 4 consecutive n of one row m, which an epilogue loads and stores as one vector.
+// 4 consecutive n of one row m.
 //
 // Ends: rows / columns past the last are clamped to the last (their results are not stored); k
 // past the end reads a page of zeros on BOTH sides (a NaN times zero would not vanish).
@@ -88,16 +88,15 @@ struct GemmArgs {
   int spseg, nseg;    // K-steps per segment, segments
   int tiles_m, tiles_n, batch, splits;
   // epilogue
-  void* out;
+  void* out;          // rows of N, like res and dh
   void* out1;         // second batch's / du
   float* slab;
-  long ldo;           // elements per output row
-  const void* res;    // residual, rows of ldo
-  const void* dh;     // E_GATED_BWD: incoming gradient, rows of N
+  const void* res;    // residual
+  const void* dh;     // E_GATED_BWD: incoming gradient
   int npad;           // E_GATED_BWD: columns [N, npad) of dg / du are written as zero
   const float *row_scale, *col_scale, *col_scale1, *bias;
   float alpha;        // E_OUT: factor of the sum
-  int act, vec;       // vec: out / res / dh rows may be accessed in vectors of 4
+  int act, vec;       // vec: N % 8 == 0, rows are read and written in groups of 8
   int drop;           // apply `d`
   DropArgs d;
 };
@@ -140,62 +139,58 @@ __device__ __forceinline__ void act_slope(int act, float g, float& a, float& s) 
   }
 }
 
-// 4 consecutive elements of a row, n .. n + 3, those past N skipped
+// 8 consecutive elements of a row as they lie in memory (16 bytes of bf16, 32 of fp32)
 template <typename T>
-__device__ __forceinline__ void load4(const T* p, int n, int N, bool vec, float* f) {
-  if (vec && n + 4 <= N) {
-    if constexpr (sizeof(T) == 4) {
-      const float4 v = *reinterpret_cast<const float4*>(p + n);
-      f[0] = v.x; f[1] = v.y; f[2] = v.z; f[3] = v.w;
-    } else {
-      const uint2 v = *reinterpret_cast<const uint2*>(p + n);
-      f[0] = __uint_as_float(v.x << 16); f[1] = __uint_as_float(v.x & 0xffff0000u);
-      f[2] = __uint_as_float(v.y << 16); f[3] = __uint_as_float(v.y & 0xffff0000u);
-    }
+struct Raw8 {
+  uint4 v[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T* p) {
+  Raw8<T> r;
+#pragma unroll
+  for (int i = 0; i < (int)sizeof(T) / 2; ++i) r.v[i] = reinterpret_cast<const uint4*>(p)[i];
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ void unpack_raw8(const Raw8<T>& r, float* f) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) unpack16<float>(__builtin_bit_cast(float4, r.v[i]), f + 4 * i);
+  } else {
+    unpack16<bf16_t>(r.v[0], f);
+  }
+}
+// elements n .. n + 7 of a row of N; vec: N % 8 == 0 (a group lies inside or outside as a whole)
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int n, int N, bool vec, float* f) {
+  if (vec) {
+    unpack_raw8<T>(load_raw8<T>(p + n), f);
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = n + e < N ? to_f(p[n + e]) : 0.f;
+    for (int e = 0; e < 8; ++e) f[e] = n + e < N ? to_f(p[n + e]) : 0.f;
   }
 }
 template <typename T>
-__device__ __forceinline__ void store4(T* p, int n, int N, bool vec, const float* f) {
-  if (vec && n + 4 <= N) {
+__device__ __forceinline__ void store8(T* p, int n, int N, bool vec, const float* f) {
+  if (vec) {
     if constexpr (sizeof(T) == 4) {
-      *reinterpret_cast<float4*>(p + n) = make_float4(f[0], f[1], f[2], f[3]);
+      store16<float>(p + n, pack16<float>(f));
+      store16<float>(p + n + 4, pack16<float>(f + 4));
     } else {
-      bf16x2_t a = {(__bf16)f[0], (__bf16)f[1]}, b = {(__bf16)f[2], (__bf16)f[3]};
-      *reinterpret_cast<uint2*>(p + n) =
-          make_uint2(__builtin_bit_cast(uint32_t, a), __builtin_bit_cast(uint32_t, b));
+      store16<bf16_t>(p + n, pack16<bf16_t>(f));
     }
   } else {
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
+    for (int e = 0; e < 8; ++e)
       if (n + e < N) p[n + e] = from_f<T>(f[e]);
   }
 }
-
-// factor, bias, dropout and residual of 4 consecutive outputs n .. n + 3 of row m, and the store
-template <typename T>
-__device__ __forceinline__ void finish4(const GemmArgs& a, void* out, int m, int n, float* f, uint64_t off) {
+// dropout of the 8 outputs of one group of row m
+__device__ __forceinline__ void drop8(const GemmArgs& a, int m, int n, float* f, uint64_t off) {
+  const uint64_t gid = (uint64_t)m * ((a.N + 7) >> 3) + (n >> 3);
+  const uint32_t k = drop_mask8(gid, off, a.d.seed, a.d.thr);
 #pragma unroll
-  for (int e = 0; e < 4; ++e) f[e] *= a.alpha;
-  if (a.bias) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] += n + e < a.N ? a.bias[n + e] : 0.f;
-  }
-  if (a.drop) {
-    const uint64_t gid = (uint64_t)m * ((a.N + 7) >> 3) + (n >> 3);
-    const uint32_t k = drop_mask8(gid, off, a.d.seed, a.d.thr) >> (n & 4);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] = (k >> e) & 1u ? f[e] * a.d.scale : 0.f;
-  }
-  if (a.res) {
-    float q[4];
-    load4<T>((const T*)a.res + (long)m * a.ldo, n, a.N, a.vec, q);
-#pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] += q[e];
-  }
-  store4<T>((T*)out + (long)m * a.ldo, n, a.N, a.vec, f);
+  for (int e = 0; e < 8; ++e) f[e] = (k >> e) & 1u ? f[e] * a.d.scale : 0.f;
 }
 
 // COL tiles: the rows that one half-wave reads together (8 lg + 0 .. 3 of two lane groups) land on
@@ -389,68 +384,116 @@ void gemm_kernel(GemmArgs a) {
     }
   }
 
-  // ---- epilogue: a lane holds n .. n + 3 of row m ----
+  // ---- epilogue. The sums go through LDS 16 rows of a wave at a time, so that a lane gets 8
+  // consecutive columns of one row (a dropout group, a 16-byte vector of bf16): rows are then
+  // read and written in whole lines. Stored from the fragment layout (8 bytes a lane, 16 rows an
+  // instruction) the 256-wide tile of a [32768][1024] result took 45 us a tile. ----
   constexpr bool FAST = sizeof(T) == 2;
+  constexpr int CW = DUAL ? WTN / 2 : WTN;          // output columns of a wave
+  constexpr int GP = CW / 8, RP = 64 / GP, NP = 16 / RP, PITCH = CW + 4;
+  static_assert(GP >= 4 && NP >= 1, "wave tile");
+  constexpr int PARTS = DUAL ? 2 : 1;
+  static_assert(NW * PARTS * 16 * PITCH * 4 <= 2 * SB, "scratch fits the stages");
+  __syncthreads();
+  float* scr = reinterpret_cast<float*>(lds) + wave * (PARTS * 16 * PITCH);
+  const int cg = lane % GP, r0 = lane / GP;
+  const int n = n0 + wn * CW + cg * 8, mw = m0 + wm * WTM + r0;
+  const bool in_n = n < (EPI == E_GATED_BWD ? a.npad : a.N);
+  const bool vec = a.vec != 0;
   const uint64_t off = EPI == E_OUT && a.drop ? drop_offset(a.d) : 0;
+  float cs0[8], cs1[8], bias[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const int c = min(n + e, a.N - 1);
+    if constexpr (DT == G_I8) {
+      cs0[e] = a.col_scale[c];
+      cs1[e] = DUAL ? a.col_scale1[c] : 0.f;
+    }
+    if constexpr (EPI == E_OUT) bias[e] = a.bias ? a.bias[c] : 0.f;
+  }
+  // what a row brings along, loaded one fragment row ahead
+  const T* side = EPI == E_GATED_BWD ? (const T*)a.dh : EPI == E_OUT ? (const T*)a.res : nullptr;
+  Raw8<T> sv[NP];
+  float rs[NP];
+  auto ahead = [&](int i) __attribute__((always_inline)) {
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int m = min(mw + i * 16 + p * RP, a.M - 1);
+      if constexpr (DT == G_I8) rs[p] = a.row_scale[m];
+      if constexpr (EPI == E_GATED_BWD || EPI == E_OUT) {
+        if (side && vec && n < a.N) sv[p] = load_raw8<T>(side + (long)m * a.N + n);
+      }
+    }
+  };
+  ahead(0);
 #pragma unroll
   for (int i = 0; i < FM; ++i) {
-    const int m = m0 + wm * WTM + i * 16 + lr;
-    if (m >= a.M) continue;
-    float rs = 1.f;
-    if constexpr (DT == G_I8) rs = a.row_scale[m];
-    if constexpr (DUAL) {
 #pragma unroll
-      for (int j = 0; j < FN / 2; ++j) {
-        const int n = n0 + wn * (WTN / 2) + j * 16 + lg * 4;
-        float g[4], u[4];
+    for (int j = 0; j < FN; ++j) {
+      const int part = DUAL ? j / (FN / 2) : 0, jc = DUAL ? j % (FN / 2) : j;
+      *reinterpret_cast<typename GT<DT>::acc*>(scr + (part * 16 + lr) * PITCH + jc * 16 + lg * 4) = acc[j][i];
+    }
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's own rows: no barrier
+    float f[NP][8], u[NP][8], q[NP][8];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          g[e] = (float)acc[j][i][e];
-          u[e] = (float)acc[j + FN / 2][i][e];
-          if constexpr (DT == G_I8) {
-            const int nn = min(n + e, a.N - 1);
-            g[e] = g[e] * rs * a.col_scale[nn];
-            u[e] = u[e] * rs * a.col_scale1[nn];
-          }
-        }
-        if constexpr (EPI == E_GATED) {
-          if (n >= a.N) continue;
+    for (int p = 0; p < NP; ++p) {
 #pragma unroll
-          for (int e = 0; e < 4; ++e) g[e] = act_f<FAST>(a.act, g[e]) * u[e];
-          store4<T>((T*)a.out + (long)m * a.ldo, n, a.N, a.vec, g);
-        } else {
-          if (n >= a.npad) continue;  // dg / du rows are npad long: always vectors
-          float d[4], dg[4], du[4];
-          load4<T>((const T*)a.dh + (long)m * a.N, n, a.N, a.vec, d);
+      for (int h = 0; h < 2; ++h) {
+        const auto v = *reinterpret_cast<const typename GT<DT>::acc*>(scr + (r0 + p * RP) * PITCH + cg * 8 + 4 * h);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            float av, sv;
-            act_slope<FAST>(a.act, g[e], av, sv);
-            dg[e] = n + e < a.N ? d[e] * u[e] * sv : 0.f;
-            du[e] = n + e < a.N ? d[e] * av : 0.f;
-          }
-          store4<T>((T*)a.out + (long)m * a.npad, n, a.npad, true, dg);
-          store4<T>((T*)a.out1 + (long)m * a.npad, n, a.npad, true, du);
+        for (int e = 0; e < 4; ++e) f[p][4 * h + e] = (float)v[e];
+        if constexpr (DUAL) {
+          const auto w = *reinterpret_cast<const typename GT<DT>::acc*>(scr + (16 + r0 + p * RP) * PITCH + cg * 8 + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) u[p][4 * h + e] = (float)w[e];
         }
       }
-    } else {
+      if constexpr (DT == G_I8) {
 #pragma unroll
-      for (int j = 0; j < FN; ++j) {
-        const int n = n0 + wn * WTN + j * 16 + lg * 4;
-        if (n >= a.N) continue;
-        float f[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[e] = (float)acc[j][i][e];
-        if constexpr (EPI == E_SLAB) {
-          float* s = a.slab + (((long)split * a.batch + bat) * a.M + m) * a.N;
-          store4<float>(s, n, a.N, (a.N & 3) == 0, f);
-        } else {
-          if constexpr (DT == G_I8) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) f[e] = f[e] * rs * a.col_scale[min(n + e, a.N - 1)];
-          }
-          finish4<T>(a, bat ? a.out1 : a.out, m, n, f, off);
+        for (int e = 0; e < 8; ++e) {
+          f[p][e] = f[p][e] * rs[p] * cs0[e];
+          if constexpr (DUAL) u[p][e] = u[p][e] * rs[p] * cs1[e];
         }
+      }
+      if constexpr (EPI == E_GATED_BWD || EPI == E_OUT) {
+        if (side) {
+          if (vec) unpack_raw8<T>(sv[p], q[p]);
+          else if (n < a.N) load8<T>(side + (long)min(mw + i * 16 + p * RP, a.M - 1) * a.N, n, a.N, false, q[p]);
+        }
+      }
+    }
+    if (i + 1 < FM) ahead(i + 1);
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next rows overwrite
+#pragma unroll
+    for (int p = 0; p < NP; ++p) {
+      const int m = mw + i * 16 + p * RP;
+      if (m >= a.M || !in_n) continue;
+      if constexpr (EPI == E_GATED) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[p][e] = act_f<FAST>(a.act, f[p][e]) * u[p][e];
+        store8<T>((T*)a.out + (long)m * a.N, n, a.N, vec, f[p]);
+      } else if constexpr (EPI == E_GATED_BWD) {
+        float dg[8], du[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          float av, sl;
+          act_slope<FAST>(a.act, f[p][e], av, sl);
+          dg[e] = n + e < a.N ? q[p][e] * u[p][e] * sl : 0.f;
+          du[e] = n + e < a.N ? q[p][e] * av : 0.f;
+        }
+        store8<T>((T*)a.out + (long)m * a.npad, n, a.npad, true, dg);
+        store8<T>((T*)a.out1 + (long)m * a.npad, n, a.npad, true, du);
+      } else if constexpr (EPI == E_SLAB) {
+        store8<float>(a.slab + (((long)split * a.batch + bat) * a.M + m) * a.N, n, a.N, vec, f[p]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[p][e] = fmaf(f[p][e], a.alpha, bias[e]);
+        if (a.drop) drop8(a, m, n, f[p], off);
+        if (side) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[p][e] += q[p][e];
+        }
+        store8<T>((T*)(bat ? a.out1 : a.out) + (long)m * a.N, n, a.N, vec, f[p]);
       }
     }
   }
@@ -519,34 +562,54 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
         f[p][e] = f[p][e] * a.row_scale[m] * (p ? a.col_scale1 : a.col_scale)[min(n + e, a.N - 1)];
     }
   }
-  if constexpr (DUAL) {
+  const uint32_t keep = !DUAL && a.drop ? drop_mask8((uint64_t)m * ((a.N + 7) >> 3) + (n >> 3), drop_offset(a.d),
+                                                     a.d.seed, a.d.thr) >> (n & 4) : 0;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[0][e] = act_f<sizeof(T) == 2>(a.act, f[0][e]) * f[P - 1][e];
-    store4<T>((T*)a.out + (long)m * a.ldo, n, a.N, a.vec, f[0]);
-  } else {
-    finish4<T>(a, a.out, m, n, f[0], a.drop ? drop_offset(a.d) : 0);
+  for (int e = 0; e < 4; ++e) {
+    if (n + e >= a.N) break;
+    const long at = (long)m * a.N + n + e;
+    float v = f[0][e];
+    if constexpr (DUAL) {
+      v = act_f<sizeof(T) == 2>(a.act, v) * f[P - 1][e];
+    } else {
+      if (a.bias) v += a.bias[n + e];
+      if (a.drop) v = (keep >> e) & 1u ? v * a.d.scale : 0.f;
+      if (a.res) v += to_f(((const T*)a.res)[at]);
+    }
+    ((T*)a.out)[at] = from_f<T>(v);
   }
 }
 
 // sum of the k ranges' partial sums in their order, then the epilogue of E_OUT
 template <typename T>
 __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
-  const int n4 = (a.N + 3) >> 2;
+  const int n8 = (a.N + 7) >> 3;
   const long t = (long)blockIdx.x * 256 + threadIdx.x;
-  if (t >= (long)a.batch * a.M * n4) return;
-  const int n = (int)(t % n4) * 4;
-  const long bm = t / n4;  // batch * M + m
+  if (t >= (long)a.batch * a.M * n8) return;
+  const int n = (int)(t % n8) * 8;
+  const long bm = t / n8;  // batch * M + m
   const int bat = (int)(bm / a.M), m = (int)(bm - (long)bat * a.M);
   const long pitch = (long)a.batch * a.M * a.N;
   const float* s = a.slab + bm * a.N;
-  float f[4] = {0.f, 0.f, 0.f, 0.f};
+  const bool vec = a.vec != 0;
+  float f[8] = {};
+#pragma unroll 4
   for (int k = 0; k < a.splits; ++k) {
-    float q[4];
-    load4<float>(s + k * pitch, n, a.N, (a.N & 3) == 0, q);
+    float q[8];
+    load8<float>(s + k * pitch, n, a.N, vec, q);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) f[e] += q[e];
+    for (int e = 0; e < 8; ++e) f[e] += q[e];
   }
-  finish4<T>(a, bat ? a.out1 : a.out, m, n, f, a.drop ? drop_offset(a.d) : 0);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] = f[e] * a.alpha + (a.bias && n + e < a.N ? a.bias[n + e] : 0.f);
+  if (a.drop) drop8(a, m, n, f, drop_offset(a.d));
+  if (a.res) {
+    float q[8];
+    load8<T>((const T*)a.res + (long)m * a.N, n, a.N, vec, q);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) f[e] += q[e];
+  }
+  store8<T>((T*)(bat ? a.out1 : a.out) + (long)m * a.N, n, a.N, vec, f);
 }
 
 // rows of K elements -> rows of Kp (16-byte multiple), the rest zero. E: unsigned type of es bytes
@@ -581,6 +644,29 @@ static inline void launch_pad(hipStream_t st, const void* src, void* dst, long r
   const long n = rows * (Kp * (long)sizeof(E) / 16);
   hipLaunchKernelGGL((pad_rows_kernel<E>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st,
                      (const E*)src, (E*)dst, rows, K, Kp);
+}
+
+// ---- tile size and split of a product ----
+struct GemmPlan {
+  bool big;  // 256-row / column tiles
+  int tiles_m, tiles_n, splits;
+  long slab;  // bytes
+};
+// per: a gated tile holds 2 x tile / 2 columns. wide: the type has 256-wide tiles
+static inline GemmPlan plan_gemm(bool wide, long M, long N, int per, int steps, int batch, bool can_split) {
+  GemmPlan p;
+  const long big = ((M + 255) / 256) * ((N + 256 / per - 1) / (256 / per)) * batch;
+  const long asked = route(HGK_ROUTE_FFN_TILE);
+  p.big = wide && (asked ? asked == 256 : big >= 256);
+  const int b = p.big ? 256 : 128;
+  p.tiles_m = (int)((M + b - 1) / b);
+  p.tiles_n = (int)((N + b / per - 1) / (b / per));
+  const long tiles = (long)p.tiles_m * p.tiles_n * batch;
+  p.splits = 1;
+  if (can_split && tiles * 2 <= (p.big ? 256 : kFillGroups))
+    p.splits = (int)std::max(1l, std::min<long>((p.big ? 256 : kFillGroups) / tiles, steps / 4));
+  p.slab = p.splits > 1 ? (long)p.splits * batch * M * N * 4 : 0;
+  return p;
 }
 
 // what a launch needs before its kernel is chosen

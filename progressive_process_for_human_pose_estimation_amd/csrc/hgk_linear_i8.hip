@@ -152,14 +152,13 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
   a.km = a.kn = w.Kp;
   a.spseg = (w.Kp + 127) / 128;
   a.out = y;
-  a.ldo = N;
   a.row_scale = (const float*)(ws + w.s);
   a.col_scale = s0;
   a.col_scale1 = s1;
   a.bias = bias;
   a.res = res;
   a.act = act;
-  a.vec = N % 4 == 0;
+  a.vec = N % 8 == 0;
   constexpr int EPI = GATED ? E_GATED : E_OUT, per = GATED ? 2 : 1;
   if (M <= 64) {
     const dim3 grid((unsigned)((N + 15) / 16));
@@ -167,12 +166,11 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
     else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<G_I8, T, 2, GATED>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((skinny_kernel<G_I8, T, 4, GATED>), grid, dim3(512), 0, st, a);
   } else {
-    const bool big = ((M + 255) / 256) * ((N + 256 / per - 1) / (256 / per)) >= 256;
-    const int b = big ? 256 : 128;
-    a.tiles_m = (int)((M + b - 1) / b);
-    a.tiles_n = (N + b / per - 1) / (b / per);
+    const GemmPlan g = plan_gemm(true, M, N, per, a.spseg, 1, false);
+    a.tiles_m = g.tiles_m;
+    a.tiles_n = g.tiles_n;
     const dim3 grid((unsigned)((long)a.tiles_m * a.tiles_n));
-    if (big) hipLaunchKernelGGL((gemm_kernel<G_I8, T, L_ROW, L_ROW, 256, 256, 2, 4, EPI, 2>), grid, dim3(512), 0, st, a);
+    if (g.big) hipLaunchKernelGGL((gemm_kernel<G_I8, T, L_ROW, L_ROW, 256, 256, 4, 2, EPI, 2>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((gemm_kernel<G_I8, T, L_ROW, L_ROW, 128, 128, 2, 2, EPI, 2>), grid, dim3(256), 0, st, a);
   }
   HGK_LAUNCH_CHECK();
