@@ -16,31 +16,17 @@
 
 namespace hgk {
 
-template <int DT, typename T, int LM, int LN, int EPI>
-static void run_tiles(hipStream_t st, const GemmArgs& a, bool big) {
-  const dim3 grid((unsigned)((long)a.tiles_m * a.tiles_n * a.batch * a.splits));
-  if constexpr (DT == G_BF16) {
-    if (big) {
-      hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 256, 256, 4, 2, EPI, 2>), grid, dim3(512), 0, st, a);
-      return;
-    }
-  }
-  hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 128, 2, 2, EPI, 2>), grid, dim3(256), 0, st, a);
-}
-
 template <int DT, typename T, int LM, int LN>
 static int run_product(hipStream_t st, GemmArgs& a, const GemmPlan& p, char* slab) {
-  a.tiles_m = p.tiles_m;
-  a.tiles_n = p.tiles_n;
   a.splits = p.splits;
   a.slab = (float*)slab;
   if (p.splits > 1) {
-    run_tiles<DT, T, LM, LN, E_SLAB>(st, a, p.big);
+    run_tiles<DT, T, LM, LN, E_SLAB>(st, a, p);
     HGK_LAUNCH_CHECK();
     const long n = (long)a.batch * a.M * ((a.N + 7) / 8);
     hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
   } else {
-    run_tiles<DT, T, LM, LN, E_OUT>(st, a, p.big);
+    run_tiles<DT, T, LM, LN, E_OUT>(st, a, p);
   }
   HGK_LAUNCH_CHECK();
   return HGK_OK;
@@ -88,7 +74,7 @@ struct GatedWs {
 };
 static GatedWs gated_ws(int dtype, long M, int C, int F, bool bwd) {
   GatedWs w;
-  const int es = es_of(dtype), q = 16 / es, ks = 128 / es;
+  const int es = es_of(dtype), q = 16 / es, ks = 64 / es;
   w.Cp = (int)up_to(C, q);
   w.Fp = (int)up_to(F, 8);
   w.pad = w.Cp != C;
@@ -113,8 +99,8 @@ static GatedWs gated_ws(int dtype, long M, int C, int F, bool bwd) {
 static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
 #define HGK_CHECK_ROWS(what, M, A, B)                                                              \
-  HGK_CHECK_ARG((M) >= 0 && (M) <= (1l << 30) && (A) >= 1 && (A) <= (1 << 24) && (B) >= 1 &&       \
-                    (B) <= (1 << 24),                                                              \
+  HGK_CHECK_ARG((M) >= 0 && (M) <= (1l << 30) && (A) >= 1 && (A) <= (1 << 21) && (B) >= 1 &&       \
+                    (B) <= (1 << 21),                                                              \
                 what ": bad sizes (%ld rows, %d, %d)", (long)(M), (int)(A), (int)(B))
 
 template <typename T>
@@ -133,7 +119,7 @@ static void gated_operands(hipStream_t st, GemmArgs& a, const GatedWs& w, char* 
   a.M = (int)M;
   a.N = F;
   a.km = a.kn = w.Cp;
-  a.spseg = (int)up_to((long)w.Cp * sizeof(T), 128) / 128;
+  a.spseg = (int)up_to((long)w.Cp * sizeof(T), 64) / 64;
 }
 
 template <typename T>
@@ -150,9 +136,7 @@ static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* 
     run_skinny<DT, T, true>(st, a);
   } else {
     const GemmPlan p = plan_gemm(dtype == HGK_BF16, M, F, 2, a.spseg, 1, false);
-    a.tiles_m = p.tiles_m;
-    a.tiles_n = p.tiles_n;
-    run_tiles<DT, T, L_ROW, L_ROW, E_GATED>(st, a, p.big);
+    run_tiles<DT, T, L_ROW, L_ROW, E_GATED>(st, a, p);
   }
   HGK_LAUNCH_CHECK();
   return HGK_OK;
@@ -163,7 +147,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
                      void* dx, void* dwg, void* dwu, long M, int C, int F, int act, char* ws,
                      int dtype) {
   constexpr int DT = TypeOf<T>::dt;
-  constexpr int es = sizeof(T), ks = 128 / es;
+  constexpr int es = sizeof(T), ks = 64 / es;
   const GatedWs w = gated_ws(dtype, M, C, F, true);
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
@@ -175,9 +159,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
   a.act = act;
   a.vec = F % 8 == 0;
   const GemmPlan p = plan_gemm(dtype == HGK_BF16, M, F, 2, a.spseg, 1, false);
-  a.tiles_m = p.tiles_m;
-  a.tiles_n = p.tiles_n;
-  run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p.big);
+  run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p);
   HGK_LAUNCH_CHECK();
   if (dx) {
     GemmArgs b = gemm_args();
@@ -226,7 +208,7 @@ struct LinearWs {
 };
 static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) {
   LinearWs w;
-  const int es = es_of(dtype), q = 16 / es, ks = 128 / es;
+  const int es = es_of(dtype), q = 16 / es, ks = 64 / es;
   w.Kp = (int)up_to(K, q);
   w.Np = (int)up_to(N, q);
   w.pad_k = w.Kp != K;
@@ -268,7 +250,7 @@ static int linear_fwd(hipStream_t st, const void* x, const void* wt, const void*
   a.M = (int)M;
   a.N = N;
   a.km = a.kn = w.Kp;
-  a.spseg = (int)up_to((long)w.Kp * sizeof(T), 128) / 128;
+  a.spseg = (int)up_to((long)w.Kp * sizeof(T), 64) / 64;
   a.out = y;
   a.res = res;
   a.vec = N % 8 == 0;
@@ -286,7 +268,7 @@ template <typename T>
 static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void* dy, void* dx, void* dw,
                       long M, int K, int N, const DropArgs& d, char* ws, int dtype) {
   constexpr int DT = TypeOf<T>::dt;
-  constexpr int es = sizeof(T), ks = 128 / es;
+  constexpr int es = sizeof(T), ks = 64 / es;
   typedef typename TypeOf<T>::raw raw;
   const bool drop = d.thr != 0;
   const LinearWs w = linear_ws(dtype, M, K, N, drop, true);

@@ -4,18 +4,23 @@
 //   D[m][n] = sum_k A(m, k) B(n, k)
 //
 // Byte geometry. Everything is counted in 16-byte chunks, so one address plan serves 8-bit
-// integers, bf16 and fp32: a K-step is 128 bytes of a row, a fragment is one chunk a lane
-// (16 bytes = 16 int8 / 8 bf16 / 4 fp32 values of k), a 64-byte half K-step is one
+// integers, bf16 and fp32: a K-step is 64 bytes of a row, a fragment is one chunk a lane
+// (16 bytes = 16 int8 / 8 bf16 / 4 fp32 values of k), and a step's fragment pair is one
 // mfma_i32_16x16x64_i8, one mfma_f32_16x16x32_bf16 or four mfma_f32_16x16x4_f32.
 //
 // Operand layouts.
-//   ROW: k runs along memory. LDS tile [rows][128 B]; chunk c of row r sits at chunk slot
-//        c ^ (r & 7), so the 8 rows that a b128 read takes at a time touch all 32 banks once.
+//   ROW: k runs along memory. LDS tile [rows][64 B]; chunk c of row r sits at slot
+//        c ^ ((r >> 1) & 3), so the 8 rows that a b128 read takes at a time touch all banks once.
 //   COL: k is the row index (weights of an input gradient, both operands of a weight gradient).
 //        LDS tile [KS rows][tile columns], read as transposed fragments
 //        (ds_read_b64_tr_b16; fp32: four b32 reads), slots swizzled by swz_col() below.
 // Global -> LDS by LDS-DMA (16 bytes a lane, no registers); the swizzle is in the source address
 // a lane picks, the LDS side is written in order.
+//
+// Pipeline. A ring of S K-steps in LDS, one barrier a step: at step t the barrier says that step
+// t + 1 has landed and that every wave holds step t's fragments in registers, so the DMA of step
+// t + S may go into t's slot, and the fragments of t + 1 are read while the matrix instructions of
+// t run. S - 1 steps are on their way at any time.
 //
 // The matrix instruction's A operand is the N side and its B operand the M side: a lane then holds
 // 4 consecutive n of one row m.
@@ -24,6 +29,7 @@
 // past the end reads a page of zeros on BOTH sides (a NaN times zero would not vanish).
 #pragma once
 #include <algorithm>
+#include <type_traits>
 
 #include "hgk_conv.h"
 #include "hgk_philox.h"
@@ -103,6 +109,14 @@ struct GemmArgs {
 
 static __device__ __attribute__((aligned(64))) char g_zero_page[64];
 
+// dma16 (hgk_conv.h) from a wave-uniform base and a 32-bit offset a lane
+__device__ __forceinline__ void dma16s(const char* base, uint32_t off, char* lds_wave_base) {
+  const uint32_t l = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char*)lds_wave_base;
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
+               ::"s"(__builtin_amdgcn_readfirstlane(l)), "v"(off), "s"(base)
+               : "memory", "m0");
+}
+
 // ---- activations: value and slope. `FAST`: bf16 results (hardware exponential and reciprocal,
 // 1 ulp of fp32, against a half step of 2^-9); fp32 results take the full-precision functions ----
 template <bool FAST>
@@ -110,26 +124,26 @@ __device__ __forceinline__ float sigmoid_f(float g) {
   if (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f));
   return 1.f / (1.f + expf(-g));
 }
-template <bool FAST>
-__device__ __forceinline__ float act_f(int act, float g) {
-  if (act == kActSilu) return g * sigmoid_f<FAST>(g);
-  if (act == kActGelu) return 0.5f * g * erfcf(g * -0.70710678f);
-  if (act == kActRelu) return g > 0.f || g != g ? g : 0.f;
+template <int ACT, bool FAST>
+__device__ __forceinline__ float act_f(float g) {
+  if (ACT == kActSilu) return g * sigmoid_f<FAST>(g);
+  if (ACT == kActGelu) return 0.5f * g * erfcf(g * -0.70710678f);
+  if (ACT == kActRelu) return g > 0.f || g != g ? g : 0.f;
   return sigmoid_f<FAST>(g);
 }
 // a(g) and a'(g)
-template <bool FAST>
-__device__ __forceinline__ void act_slope(int act, float g, float& a, float& s) {
-  if (act == kActSilu) {
+template <int ACT, bool FAST>
+__device__ __forceinline__ void act_slope(float g, float& a, float& s) {
+  if (ACT == kActSilu) {
     const float q = sigmoid_f<FAST>(g);
     a = g * q;
     s = q + a * (1.f - q);
-  } else if (act == kActGelu) {
+  } else if (ACT == kActGelu) {
     const float h = 0.5f * erfcf(g * -0.70710678f);
     const float e = FAST ? __builtin_amdgcn_exp2f(g * g * -0.72134752f) : expf(-0.5f * g * g);
     a = g * h;
     s = h + g * 0.39894228f * e;
-  } else if (act == kActRelu) {
+  } else if (ACT == kActRelu) {
     a = g > 0.f || g != g ? g : 0.f;
     s = g > 0.f ? 1.f : 0.f;
   } else {
@@ -137,6 +151,14 @@ __device__ __forceinline__ void act_slope(int act, float g, float& a, float& s) 
     a = q;
     s = q * (1.f - q);
   }
+}
+// f(constant) for the activation that `act` names: one branch, not one an element
+template <typename F>
+__device__ __forceinline__ void with_act(int act, F&& f) {
+  if (act == kActSilu) f(std::integral_constant<int, kActSilu>());
+  else if (act == kActGelu) f(std::integral_constant<int, kActGelu>());
+  else if (act == kActRelu) f(std::integral_constant<int, kActRelu>());
+  else f(std::integral_constant<int, kActSigmoid>());
 }
 
 // 8 consecutive elements of a row as they lie in memory (16 bytes of bf16, 32 of fp32)
@@ -193,32 +215,35 @@ __device__ __forceinline__ void drop8(const GemmArgs& a, int m, int n, float* f,
   for (int e = 0; e < 8; ++e) f[e] = (k >> e) & 1u ? f[e] * a.d.scale : 0.f;
 }
 
-// COL tiles: the rows that one half-wave reads together (8 lg + 0 .. 3 of two lane groups) land on
-// distinct 32-byte positions; fp32 reads 4 lg + i of two lane groups, 64 bytes apart
-template <int DT>
+// COL tiles of CH chunks a row. bf16: the 8 rows that a half-wave reads together (8 lg + 0 .. 3 of
+// two lane groups, 32 bytes of each) land on distinct 32-byte positions of the 256 that a read
+// covers; fp32: rows 4 lg + i of two lane groups, 64 bytes of each
+template <int DT, int CH>
 __device__ __forceinline__ int swz_col(int p) {
-  if constexpr (DT == G_BF16) return ((p & 3) | (((p >> 3) & 1) << 2)) << 1;
+  if constexpr (DT == G_BF16) {
+    if constexpr (CH >= 16) return ((p & 3) | (((p >> 3) & 1) << 2)) << 1;
+    return (((p >> 1) & 1) | (((p >> 3) & 1) << 1)) << 1;  // 128-byte rows: two fill the window
+  }
   return ((p >> 2) & 1) << 2;
 }
 
 // T: type of outputs, residual and dh
-template <int DT, typename T, int LM, int LN, int BM, int BN, int WM, int WN, int EPI, int MINW>
-__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(MINW)))
+template <int DT, typename T, int LM, int LN, int BM, int BN, int WM, int WN, int S, int EPI>
+__global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void gemm_kernel(GemmArgs a) {
   constexpr int NW = WM * WN, es = GT<DT>::es;
-  constexpr int KS = 128 / es;               // k per step
+  constexpr int KS = 64 / es;                // k per step
   constexpr bool DUAL = EPI == E_GATED || EPI == E_GATED_BWD;
-  constexpr int PM = BM * 128, PN = BN * 128, SB = PM + PN;  // LDS bytes of a stage
-  constexpr int DM = BM / 8 / NW, DN = BN / 8 / NW;          // 1-KB DMAs of a wave per stage
-  static_assert(BM % (8 * NW) == 0 && BN % (8 * NW) == 0, "whole DMAs per wave");
-  static_assert(LM == L_ROW || BM * es >= 256, "COL swizzle needs 16 chunks a row");
-  static_assert(LN == L_ROW || BN * es >= 256, "COL swizzle needs 16 chunks a row");
+  constexpr int PM = BM * 64, PN = BN * 64, SB = PM + PN;    // LDS bytes of a step
+  constexpr int DM = BM / 16 / NW, DN = BN / 16 / NW, D = DM + DN;  // 1-KB DMAs of a wave per step
+  static_assert(BM % (16 * NW) == 0 && BN % (16 * NW) == 0, "whole DMAs per wave");
+  static_assert(BM * es >= 128 || LM == L_ROW, "COL swizzle needs 8 chunks a row");
   static_assert(DT != G_I8 || (LM == L_ROW && LN == L_ROW), "8-bit operands are ROW");
   constexpr int WTM = BM / WM, WTN = BN / WN, FM = WTM / 16, FN = WTN / 16;
   static_assert(!DUAL || FN % 2 == 0, "gate and up halves");
-  __shared__ __attribute__((aligned(16))) char lds[2 * SB];
+  __shared__ __attribute__((aligned(16))) char lds[S * SB];
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
   const int wm = wave / WN, wn = wave % WN;
 
@@ -239,100 +264,94 @@ void gemm_kernel(GemmArgs a) {
   const int steps = a.spseg * a.nseg;
   const int s0 = (int)((long)split * steps / a.splits), s1 = (int)((long)(split + 1) * steps / a.splits);
 
-  // ---- DMA sources ----
-  const char* pm[DM];
-  const char* pn[DN];
-  const int seg0 = s0 / a.spseg, kin0 = s0 - seg0 * a.spseg;
-  const char* bm = (a.batch > 1 ? bat : seg0) ? a.m1 : a.m0;
-  const char* bn = (!DUAL && a.nseg > 1 && seg0) ? a.n1 : a.n0;
-  const int rchunk = (lane & 7) ^ ((lane >> 3) & 7);  // ROW: chunk of every DMA of this lane
+  // ---- DMA sources: a base that moves with the steps and an offset a lane (host: 256 rows of an
+  // operand are less than 4 GB) ----
+  const int seg0 = s0 / a.spseg;
+  int kin = s0 - seg0 * a.spseg;
+  const long stepm = LM == L_ROW ? 64 : (long)KS * a.ldm, stepn = LN == L_ROW ? 64 : (long)KS * a.ldn;
+  const char* bm = ((a.batch > 1 ? bat : seg0) ? a.m1 : a.m0) + kin * stepm;
+  const char* bn = (!DUAL && a.nseg > 1 && seg0 ? a.n1 : a.n0) + kin * stepn;
+  long dual = 0;  // E_GATED*: up weights minus gate weights, in bytes
+  if (DUAL) dual = a.n1 - a.n0;
+  if (LM == L_ROW) bm += (long)m0 * a.ldm;
+  if (LN == L_ROW) bn += (long)n0 * a.ldn;
+  uint32_t om[DM], on[DN];
+  const int rchunk = (lane & 3) ^ ((lane >> 3) & 3);  // ROW: chunk of every DMA of this lane
   constexpr int CM = BM * es / 16, CN = BN * es / 16;  // COL: chunks per LDS row
   auto colrow = [&](int d, int C) { return ((d * NW + wave) * 64 + lane) / C; };
 #pragma unroll
   for (int d = 0; d < DM; ++d) {
     if (LM == L_ROW) {
-      const int r = min(m0 + (d * NW + wave) * 8 + (lane >> 3), a.M - 1);
-      pm[d] = bm + r * a.ldm + (long)kin0 * 128 + rchunk * 16;
+      const int r = min((d * NW + wave) * 16 + (lane >> 2), a.M - 1 - m0);
+      om[d] = (uint32_t)r * (uint32_t)a.ldm + rchunk * 16;
     } else {
       const int p = colrow(d, CM);
-      const int c = (((d * NW + wave) * 64 + lane) % CM) ^ swz_col<DT>(p);
-      const int col = min(m0 * es + c * 16, (a.M * es - 1) & ~15);
-      pm[d] = bm + ((long)kin0 * KS + p) * a.ldm + col;
+      const int c = (((d * NW + wave) * 64 + lane) % CM) ^ swz_col<DT, CM>(p);
+      om[d] = (uint32_t)p * (uint32_t)a.ldm + min(m0 * es + c * 16, (a.M * es - 1) & ~15);
     }
   }
 #pragma unroll
   for (int d = 0; d < DN; ++d) {
     if (LN == L_ROW) {
-      int r = (d * NW + wave) * 8 + (lane >> 3);
-      const char* b = bn;
-      if (DUAL) {
-        if (r >= BN / 2) {
-          b = a.n1;
-          r -= BN / 2;
-        }
-      }
-      r = min(n0 + r, a.N - 1);
-      pn[d] = b + r * a.ldn + (long)kin0 * 128 + rchunk * 16;
+      // gated: the first half of the tile's rows are gate rows, the second up rows
+      const int r = (d * NW + wave) * 16 % (DUAL ? BN / 2 : BN) + (lane >> 2);
+      on[d] = (uint32_t)min(r, a.N - 1 - n0) * (uint32_t)a.ldn + rchunk * 16;
     } else {
       const int p = colrow(d, CN);
-      const int c = (((d * NW + wave) * 64 + lane) % CN) ^ swz_col<DT>(p);
-      const int col = min(n0 * es + c * 16, (a.N * es - 1) & ~15);
-      pn[d] = bn + ((long)kin0 * KS + p) * a.ldn + col;
+      const int c = (((d * NW + wave) * 64 + lane) % CN) ^ swz_col<DT, CN>(p);
+      on[d] = (uint32_t)p * (uint32_t)a.ldn + min(n0 * es + c * 16, (a.N * es - 1) & ~15);
     }
   }
+  static_assert(!DUAL || BN % 32 == 0, "a DMA brings gate rows or up rows");
   const bool tail_m = a.km % KS != 0, tail_n = a.kn % KS != 0;
-  int kin = kin0;
-  auto issue = [&](int slot) __attribute__((always_inline)) {
-    char* sb = lds + slot * SB;
-    const bool last = kin + 1 == a.spseg;
-    if (last && (tail_m || tail_n)) {
-      // the zero page stands in for k past the end
-#pragma unroll
-      for (int d = 0; d < DM; ++d) {
-        const bool ok = LM == L_ROW ? kin * 128 + rchunk * 16 < a.km * es
-                                    : kin * KS + colrow(d, CM) < a.km;
-        dma16(ok ? pm[d] : g_zero_page, sb + (d * NW + wave) * 1024);
-      }
-#pragma unroll
-      for (int d = 0; d < DN; ++d) {
-        const bool ok = LN == L_ROW ? kin * 128 + rchunk * 16 < a.kn * es
-                                    : kin * KS + colrow(d, CN) < a.kn;
-        dma16(ok ? pn[d] : g_zero_page, sb + PM + (d * NW + wave) * 1024);
-      }
+  // DMA d of the step at (bm, bn, kin) into its slot; in a segment's last step the zero page stands
+  // in for k past the end
+  auto dma = [&](int d, int slot, bool tail) __attribute__((always_inline)) {
+    const bool mside = d < DM;
+    const int e = mside ? d : d - DM;
+    char* to = lds + slot * SB + (mside ? 0 : PM) + (e * NW + wave) * 1024;
+    const char* base = mside ? bm : bn + (DUAL && (e * NW + wave) * 16 >= BN / 2 ? dual : 0);
+    const uint32_t off = mside ? om[e % DM] : on[e % DN];
+    if (tail) {
+      const int lay = mside ? LM : LN, k = mside ? a.km : a.kn;
+      const bool ok = lay == L_ROW ? kin * 64 + rchunk * 16 < k * es
+                                   : kin * KS + colrow(e, mside ? CM : CN) < k;
+      dma16(ok ? base + off : g_zero_page, to);
     } else {
-#pragma unroll
-      for (int d = 0; d < DM; ++d) dma16(pm[d], sb + (d * NW + wave) * 1024);
-#pragma unroll
-      for (int d = 0; d < DN; ++d) dma16(pn[d], sb + PM + (d * NW + wave) * 1024);
+      dma16s(base, off, to);
     }
+  };
+  auto is_tail = [&]() { return (tail_m || tail_n) && kin + 1 == a.spseg; };
+  auto advance = [&]() __attribute__((always_inline)) {
+    const bool last = kin + 1 == a.spseg;
     ++kin;
-    long im = LM == L_ROW ? 128 : (long)KS * a.ldm, in = LN == L_ROW ? 128 : (long)KS * a.ldn;
+    bm += stepm;
+    bn += stepn;
     if (a.nseg > 1 && last) {  // on to the second segment
-      im += (a.m1 - a.m0) - (LM == L_ROW ? (long)a.spseg * 128 : (long)a.spseg * KS * a.ldm);
-      in += (a.n1 - a.n0) - (LN == L_ROW ? (long)a.spseg * 128 : (long)a.spseg * KS * a.ldn);
+      bm += (a.m1 - a.m0) - a.spseg * stepm;
+      bn += (a.n1 - a.n0) - a.spseg * stepn;
       kin = 0;
     }
+  };
+  auto issue = [&](int slot) __attribute__((always_inline)) {
+    const bool tail = is_tail();
 #pragma unroll
-    for (int d = 0; d < DM; ++d) pm[d] += im;
-#pragma unroll
-    for (int d = 0; d < DN; ++d) pn[d] += in;
+    for (int d = 0; d < D; ++d) dma(d, slot, tail);
+    advance();
   };
 
-  // ---- fragment offsets within a stage ----
-  // ROW: row + lr, chunk lg + 4 s at slot ^ (row & 7) (tile rows are multiples of 8 apart)
-  const int x0 = (lg ^ (lr & 7)) << 4, x1 = ((lg + 4) ^ (lr & 7)) << 4;
+  // ---- fragments of a step ----
+  const int xr = lr * 64 + ((lg ^ ((lr >> 1) & 3)) << 4);
   auto rown = [&](int f) {
     return DUAL ? (f < FN / 2 ? wn * (WTN / 2) + f * 16 : BN / 2 + wn * (WTN / 2) + (f - FN / 2) * 16)
                 : wn * WTN + f * 16;
   };
-  auto frag_row = [&](const char* t, int row, int s) __attribute__((always_inline)) {
-    return *reinterpret_cast<const i32x4*>(t + (row + lr) * 128 + (s ? x1 : x0));
-  };
   typedef short s16x8 __attribute__((ext_vector_type(8)));
-  auto frag_col = [&](const char* t, int pitch, int col, int s) __attribute__((always_inline)) -> i32x4 {
+  auto frag_col = [&](const char* t, auto chunks, int col) __attribute__((always_inline)) -> i32x4 {
+    constexpr int CH = decltype(chunks)::value, pitch = CH * 16;
     if constexpr (DT == G_BF16) {
-      const int p = 32 * s + 8 * lg + (lr >> 2), c = col + 4 * (lr & 3);
-      const char* q = t + p * pitch + (((c >> 3) ^ swz_col<DT>(p)) << 4) + (c & 7) * 2;
+      const int p = 8 * lg + (lr >> 2), c = col + 4 * (lr & 3);
+      const char* q = t + p * pitch + (((c >> 3) ^ swz_col<DT, CH>(p)) << 4) + (c & 7) * 2;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
           (__attribute__((address_space(3))) s16x4*)(q + 4 * pitch));
@@ -343,10 +362,26 @@ void gemm_kernel(GemmArgs a) {
       const int c = col + lr;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int p = 16 * s + 4 * lg + i;
-        v[i] = *reinterpret_cast<const int*>(t + p * pitch + (((c >> 2) ^ swz_col<DT>(p)) << 4) + (c & 3) * 4);
+        const int p = 4 * lg + i;
+        v[i] = *reinterpret_cast<const int*>(t + p * pitch + (((c >> 2) ^ swz_col<DT, CH>(p)) << 4) + (c & 3) * 4);
       }
       return v;
+    }
+  };
+  struct Frags {
+    i32x4 m[FM], n[FN];
+  };
+  // fragment r of a step: the N side's first
+  auto read1 = [&](int slot, Frags& f, int r) __attribute__((always_inline)) {
+    const char* tm = lds + slot * SB;
+    const char* tn = tm + PM;
+    if (r < FN) {
+      f.n[r % FN] = LN == L_ROW ? *reinterpret_cast<const i32x4*>(tn + rown(r) * 64 + xr)
+                                : frag_col(tn, std::integral_constant<int, CN>(), rown(r));
+    } else {
+      const int i = r - FN;
+      f.m[i % FM] = LM == L_ROW ? *reinterpret_cast<const i32x4*>(tm + (wm * WTM + i * 16) * 64 + xr)
+                                : frag_col(tm, std::integral_constant<int, CM>(), wm * WTM + i * 16);
     }
   };
 
@@ -356,32 +391,59 @@ void gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = typename GT<DT>::acc{0, 0, 0, 0};
 
-  if (s0 < s1) issue(0);
-#pragma unroll 1
-  for (int s = s0; s < s1; ++s) {
-    // this wave's DMAs of step s have landed, and after the barrier every wave's; the other slot's
-    // last reads were consumed by the matrix instructions before it
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+  // all but the last `ahead` steps issued have landed, here and (after the barrier) in every wave
+  auto wait = [&](int ahead) __attribute__((always_inline)) {
+    if (ahead >= S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * D) : "memory");
+    else if (S > 3 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(D) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int slot = (s - s0) & 1;
-    if (s + 1 < s1) issue(slot ^ 1);
-    const char* tm = lds + slot * SB;
-    const char* tn = tm + PM;
+  };
+  static_assert(S == 3 || S == 4, "wait() counts one or two steps beyond the one it waits for");
+  const int nt = s1 - s0;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      i32x4 fm[FM], fn[FN];
+  for (int t = 0; t < S; ++t)
+    if (t < nt) issue(t);
+  if (nt >= S) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * D) : "memory");  // step 0 has landed
+  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+  Frags fa, fb;
 #pragma unroll
-      for (int j = 0; j < FN; ++j)
-        fn[j] = LN == L_ROW ? frag_row(tn, rown(j), h) : frag_col(tn, BN * es, rown(j), h);
+  for (int r = 0; r < FN + FM; ++r) read1(0, fa, r);
+  // A step in FM parts: each takes its share of the next DMAs and fragment reads along with the
+  // products of one fragment row. All DMAs first, as written plainly, hold every wave behind the
+  // barrier until the address unit has taken them (16 clocks each): 8192 x 2048 x (2 x 2048) ran
+  // with the matrix cores 50 % busy.
+  int slot = 0;
+  auto step = [&](int t, const Frags& cur, Frags& next) __attribute__((always_inline)) {
+    wait(nt - 2 - t);
+    const bool more = t + S < nt, tail = is_tail();
+    const int ns = slot + 1 == S ? 0 : slot + 1;
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
-        fm[i] = LM == L_ROW ? frag_row(tm, wm * WTM + i * 16, h) : frag_col(tm, BM * es, wm * WTM + i * 16, h);
+    for (int i = 0; i < FM; ++i) {
 #pragma unroll
-      for (int i = 0; i < FM; ++i)
+      for (int r = (FN + FM) * i / FM; r < (FN + FM) * (i + 1) / FM; ++r)
+        read1(ns, next, r);  // past the last step: whatever the slot holds, unused
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[j][i] = mma<DT>(fn[j], fm[i], acc[j][i]);
+      for (int j = 0; j < FN; ++j) acc[j][i] = mma<DT>(cur.n[j], cur.m[i], acc[j][i]);
+      // the compiler may not carry these products past the next barrier
+#pragma unroll
+      for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[j][i]));
+      if (more) {
+#pragma unroll
+        for (int d = D * i / FM; d < D * (i + 1) / FM; ++d) dma(d, slot, tail);
+      }
     }
+    if (more) advance();
+    slot = ns;
+  };
+#pragma unroll 1
+  for (int t = 0;;) {
+    step(t, fa, fb);
+    if (++t == nt) break;
+    step(t, fb, fa);
+    if (++t == nt) break;
   }
 
   // ---- epilogue. The sums go through LDS 16 rows of a wave at a time, so that a lane gets 8
@@ -390,13 +452,15 @@ void gemm_kernel(GemmArgs a) {
   // instruction) the 256-wide tile of a [32768][1024] result took 45 us a tile. ----
   constexpr bool FAST = sizeof(T) == 2;
   constexpr int CW = DUAL ? WTN / 2 : WTN;          // output columns of a wave
-  constexpr int GP = CW / 8, RP = 64 / GP, NP = 16 / RP, PITCH = CW + 4;
-  static_assert(GP >= 4 && NP >= 1, "wave tile");
+  // (64 x 64 gated tiles: 16 columns a wave, half of its lanes have a row)
+  constexpr int GP = CW / 8, RP = 64 / GP < 16 ? 64 / GP : 16, NP = 16 / RP, PITCH = CW + 4;
+  static_assert(GP >= 2 && RP <= 32, "wave tile");
   constexpr int PARTS = DUAL ? 2 : 1;
-  static_assert(NW * PARTS * 16 * PITCH * 4 <= 2 * SB, "scratch fits the stages");
+  static_assert(NW * PARTS * 16 * PITCH * 4 <= S * SB, "scratch fits the stages");
   __syncthreads();
   float* scr = reinterpret_cast<float*>(lds) + wave * (PARTS * 16 * PITCH);
-  const int cg = lane % GP, r0 = lane / GP;
+  const int cg = lane % GP, r0 = (lane / GP) % RP;
+  const bool has_row = lane / GP < RP;
   const int n = n0 + wn * CW + cg * 8, mw = m0 + wm * WTM + r0;
   const bool in_n = n < (EPI == E_GATED_BWD ? a.npad : a.N);
   const bool vec = a.vec != 0;
@@ -467,19 +531,28 @@ void gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
       const int m = mw + i * 16 + p * RP;
-      if (m >= a.M || !in_n) continue;
+      if (m >= a.M || !in_n || !has_row) continue;
       if constexpr (EPI == E_GATED) {
+        with_act(a.act, [&](auto A) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[p][e] = act_f<FAST>(a.act, f[p][e]) * u[p][e];
+          for (int e = 0; e < 8; ++e) f[p][e] = act_f<decltype(A)::value, FAST>(f[p][e]) * u[p][e];
+        });
         store8<T>((T*)a.out + (long)m * a.N, n, a.N, vec, f[p]);
       } else if constexpr (EPI == E_GATED_BWD) {
         float dg[8], du[8];
+        with_act(a.act, [&](auto A) __attribute__((always_inline)) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float av, sl;
-          act_slope<FAST>(a.act, f[p][e], av, sl);
-          dg[e] = n + e < a.N ? q[p][e] * u[p][e] * sl : 0.f;
-          du[e] = n + e < a.N ? q[p][e] * av : 0.f;
+          for (int e = 0; e < 8; ++e) {
+            float av, sl;
+            act_slope<decltype(A)::value, FAST>(f[p][e], av, sl);
+            dg[e] = q[p][e] * u[p][e] * sl;
+            du[e] = q[p][e] * av;
+          }
+        });
+        if (!vec) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (n + e >= a.N) dg[e] = du[e] = 0.f;
         }
         store8<T>((T*)a.out + (long)m * a.npad, n, a.npad, true, dg);
         store8<T>((T*)a.out1 + (long)m * a.npad, n, a.npad, true, du);
@@ -521,9 +594,9 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
   for (int p = 0; p < P; ++p)
 #pragma unroll
     for (int i = 0; i < MT; ++i) acc[p][i] = acc_t{0, 0, 0, 0};
-  const int kb = a.km * es;
+  const int kb = a.km * es, steps = (kb + 127) / 128;
 #pragma unroll 2
-  for (int s = wave; s < a.spseg; s += NW) {
+  for (int s = wave; s < steps; s += NW) {
     i32x4 wv[2][P], xv[2][MT];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -562,6 +635,12 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
         f[p][e] = f[p][e] * a.row_scale[m] * (p ? a.col_scale1 : a.col_scale)[min(n + e, a.N - 1)];
     }
   }
+  if constexpr (DUAL) {
+    with_act(a.act, [&](auto A) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) f[0][e] = act_f<decltype(A)::value, sizeof(T) == 2>(f[0][e]) * f[P - 1][e];
+    });
+  }
   const uint32_t keep = !DUAL && a.drop ? drop_mask8((uint64_t)m * ((a.N + 7) >> 3) + (n >> 3), drop_offset(a.d),
                                                      a.d.seed, a.d.thr) >> (n & 4) : 0;
 #pragma unroll
@@ -569,9 +648,7 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
     if (n + e >= a.N) break;
     const long at = (long)m * a.N + n + e;
     float v = f[0][e];
-    if constexpr (DUAL) {
-      v = act_f<sizeof(T) == 2>(a.act, v) * f[P - 1][e];
-    } else {
+    if constexpr (!DUAL) {
       if (a.bias) v += a.bias[n + e];
       if (a.drop) v = (keep >> e) & 1u ? v * a.d.scale : 0.f;
       if (a.res) v += to_f(((const T*)a.res)[at]);
@@ -636,8 +713,6 @@ static __global__ __launch_bounds__(256) void zero_kernel(uint32_t* p, long word
 int dropout_mask(hipStream_t st, int dtype, const void* dy, void* dz, long rows, int C, const DropArgs& d);
 
 static inline long up_to(long n, long q) { return (n + q - 1) / q * q; }
-// workgroups a launch is split up to along k: two 4-wave workgroups a CU
-static constexpr int kFillGroups = 512;
 
 template <typename E>
 static inline void launch_pad(hipStream_t st, const void* src, void* dst, long rows, int K, int Kp) {
@@ -648,23 +723,25 @@ static inline void launch_pad(hipStream_t st, const void* src, void* dst, long r
 
 // ---- tile size and split of a product ----
 struct GemmPlan {
-  bool big;  // 256-row / column tiles
+  int tile;  // 64: 64 x 64, 128: 128 x 128, 192: 128 x 256, 256: 256 x 256
   int tiles_m, tiles_n, splits;
   long slab;  // bytes
 };
-// per: a gated tile holds 2 x tile / 2 columns. wide: the type has 256-wide tiles
+// per: a gated tile holds 2 x (columns / 2) columns. wide: the type has 128 x 256 and 256 x 256 tiles
 static inline GemmPlan plan_gemm(bool wide, long M, long N, int per, int steps, int batch, bool can_split) {
   GemmPlan p;
-  const long big = ((M + 255) / 256) * ((N + 256 / per - 1) / (256 / per)) * batch;
-  const long asked = route(HGK_ROUTE_FFN_TILE);
-  p.big = wide && (asked ? asked == 256 : big >= 256);
-  const int b = p.big ? 256 : 128;
-  p.tiles_m = (int)((M + b - 1) / b);
-  p.tiles_n = (int)((N + b / per - 1) / (b / per));
-  const long tiles = (long)p.tiles_m * p.tiles_n * batch;
+  auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn / per - 1) / (bn / per)) * batch; };
+  const int asked = (int)route(HGK_ROUTE_FFN_TILE);
+  if (asked == 64 || asked == 128 || (wide && (asked == 192 || asked == 256))) p.tile = asked;
+  else if (wide && tiles(256, 256) >= 256) p.tile = 256;
+  else if (tiles(128, 128) >= 256) p.tile = 128;
+  else p.tile = 64;
+  const int bm = p.tile == 192 ? 128 : p.tile, bn = (p.tile == 192 ? 256 : p.tile) / per;
+  p.tiles_m = (int)((M + bm - 1) / bm);
+  p.tiles_n = (int)((N + bn - 1) / bn);
+  const long n = (long)p.tiles_m * p.tiles_n * batch, fill = p.tile == 256 ? 256 : p.tile == 64 ? 1024 : 512;
   p.splits = 1;
-  if (can_split && tiles * 2 <= (p.big ? 256 : kFillGroups))
-    p.splits = (int)std::max(1l, std::min<long>((p.big ? 256 : kFillGroups) / tiles, steps / 4));
+  if (can_split && n * 2 <= fill) p.splits = (int)std::max(1l, std::min<long>(fill / n, steps / 8));
   p.slab = p.splits > 1 ? (long)p.splits * batch * M * N * 4 : 0;
   return p;
 }
@@ -676,6 +753,25 @@ static inline GemmArgs gemm_args() {
   a.alpha = 1.f;
   a.nseg = a.batch = a.splits = 1;
   return a;
+}
+
+template <int DT, typename T, int LM, int LN, int EPI>
+static void run_tiles(hipStream_t st, GemmArgs& a, const GemmPlan& p) {
+  a.tiles_m = p.tiles_m;
+  a.tiles_n = p.tiles_n;
+  const dim3 grid((unsigned)((long)a.tiles_m * a.tiles_n * a.batch * a.splits));
+  if constexpr (DT != G_F32) {
+    if (p.tile == 256) {
+      hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 256, 256, 4, 2, 4, EPI>), grid, dim3(512), 0, st, a);
+      return;
+    }
+    if (p.tile == 192) {
+      hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 256, 2, 2, 3, EPI>), grid, dim3(256), 0, st, a);
+      return;
+    }
+  }
+  if (p.tile == 128) hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 128, 2, 2, 4, EPI>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 64, 64, 2, 2, 4, EPI>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace hgk

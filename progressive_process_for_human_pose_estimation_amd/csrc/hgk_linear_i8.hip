@@ -150,7 +150,7 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
   a.M = (int)M;
   a.N = N;
   a.km = a.kn = w.Kp;
-  a.spseg = (w.Kp + 127) / 128;
+  a.spseg = (w.Kp + 63) / 64;
   a.out = y;
   a.row_scale = (const float*)(ws + w.s);
   a.col_scale = s0;
@@ -166,12 +166,7 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
     else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<G_I8, T, 2, GATED>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((skinny_kernel<G_I8, T, 4, GATED>), grid, dim3(512), 0, st, a);
   } else {
-    const GemmPlan g = plan_gemm(true, M, N, per, a.spseg, 1, false);
-    a.tiles_m = g.tiles_m;
-    a.tiles_n = g.tiles_n;
-    const dim3 grid((unsigned)((long)a.tiles_m * a.tiles_n));
-    if (g.big) hipLaunchKernelGGL((gemm_kernel<G_I8, T, L_ROW, L_ROW, 256, 256, 4, 2, EPI, 2>), grid, dim3(512), 0, st, a);
-    else hipLaunchKernelGGL((gemm_kernel<G_I8, T, L_ROW, L_ROW, 128, 128, 2, 2, EPI, 2>), grid, dim3(256), 0, st, a);
+    run_tiles<G_I8, T, L_ROW, L_ROW, EPI>(st, a, plan_gemm(true, M, N, per, a.spseg, 1, false));
   }
   HGK_LAUNCH_CHECK();
   return HGK_OK;

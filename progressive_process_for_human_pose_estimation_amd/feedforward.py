@@ -91,23 +91,16 @@ def _grads(*ts):
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
 
 
-class _on:
-    """The device of a tensor made current for a call, where it is not already."""
-
-    def __init__(self, t):
-        self.guard = None
-        if t.device.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(t.device)
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return torch.cuda.current_stream().cuda_stream
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
-        return False
+def _launch(x, fn, *args):
+    """fn(stream, *args) on x's device and that device's current stream"""
+    dev = x.get_device()
+    if dev == torch._C._cuda_getDevice():
+        rc = fn(torch._C._cuda_getCurrentRawStream(dev), *args)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(torch._C._cuda_getCurrentRawStream(dev), *args)
+    if rc:
+        H.check(rc)
 
 
 def _workspace(n, x):
@@ -122,11 +115,10 @@ def _workspace(n, x):
 def _gated_fwd(x, wg, wu, act):
     F, C = wg.shape
     M, dt, lib = x.numel() // C, _DTYPES[x.dtype], H.lib()
-    with _on(x) as st:
-        h = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
-        wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, 0), x)
-        H.check(lib.hgk_gated_fwd(st, dt, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), M, C,
-                                  F, act, wp, n))
+    h = x.new_empty((*x.shape[:-1], F))
+    wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, 0), x)
+    _launch(x, lib.hgk_gated_fwd, dt, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), h.data_ptr(), M, C, F,
+            act, wp, n)
     return h
 
 
@@ -144,14 +136,13 @@ class _Gated(torch.autograd.Function):
         x, wg, wu = ctx.saved_tensors
         F, C = wg.shape
         M, dt, lib = x.numel() // C, _DTYPES[x.dtype], H.lib()
-        with _on(x) as st:
-            dh = _dense(dh)
-            dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-            dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-            dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if dw else (None, None)
-            wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, 1), x)
-            H.check(lib.hgk_gated_bwd(st, dt, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), dh.data_ptr(),
-                                      H.ptr(dx), H.ptr(dwg), H.ptr(dwu), M, C, F, ctx.act, wp, n))
+        dh = _dense(dh)
+        dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+        dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
+        dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if dw else (None, None)
+        wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, 1), x)
+        _launch(x, lib.hgk_gated_bwd, dt, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), dh.data_ptr(),
+                H.ptr(dx), H.ptr(dwg), H.ptr(dwu), M, C, F, ctx.act, wp, n)
         return dx, dwg, dwu, None
 
 
@@ -173,11 +164,10 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
 def _linear_fwd(x, w, res, p, seed, offset, step):
     N, K = w.shape
     M, dt, lib = x.numel() // K, _DTYPES[x.dtype], H.lib()
-    with _on(x) as st:
-        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-        wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, p > 0, 0), x)
-        H.check(lib.hgk_linear_fwd(st, dt, x.data_ptr(), w.data_ptr(), H.ptr(res), y.data_ptr(), M, K, N,
-                                   p, seed, offset, H.ptr(step), wp, n))
+    y = x.new_empty((*x.shape[:-1], N))
+    wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, p > 0, 0), x)
+    _launch(x, lib.hgk_linear_fwd, dt, x.data_ptr(), w.data_ptr(), H.ptr(res), y.data_ptr(), M, K, N, p,
+            seed, offset, H.ptr(step), wp, n)
     return y
 
 
@@ -198,13 +188,12 @@ class _Linear(torch.autograd.Function):
         M, dt, lib = x.numel() // K, _DTYPES[x.dtype], H.lib()
         dx = dw = None
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
-            with _on(x) as st:
-                g = _dense(dy)
-                dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-                dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
-                wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, p > 0, 1), x)
-                H.check(lib.hgk_linear_bwd(st, dt, x.data_ptr(), w.data_ptr(), g.data_ptr(), H.ptr(dx),
-                                           H.ptr(dw), M, K, N, p, seed, offset, H.ptr(step), wp, n))
+            g = _dense(dy)
+            dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+            dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
+            wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, p > 0, 1), x)
+            _launch(x, lib.hgk_linear_bwd, dt, x.data_ptr(), w.data_ptr(), g.data_ptr(), H.ptr(dx),
+                    H.ptr(dw), M, K, N, p, seed, offset, H.ptr(step), wp, n)
         return dx, dw, dy if ctx.needs_input_grad[2] else None, None, None, None, None
 
 
@@ -227,27 +216,29 @@ def linear_dropout_add(x, w, residual=None, p=0.0, seed=0, offset=0, step=None):
 # ---- dropout ----
 def _dropout(x, res, rows_per_mask, p, seed, offset, step):
     C = x.shape[-1]
-    with _on(x) as st:
-        y = torch.empty_like(x)
-        if x.numel():
-            H.check(H.lib().hgk_dropout_add(st, _DTYPES[x.dtype], x.data_ptr(), H.ptr(res), y.data_ptr(),
-                                            x.numel() // C, C, rows_per_mask, p, seed, offset,
-                                            H.ptr(step)))
+    y = torch.empty_like(x)
+    n = x.numel()
+    if n:
+        _launch(x, H.lib().hgk_dropout_add, _DTYPES[x.dtype], x.data_ptr(), H.ptr(res), y.data_ptr(), n // C,
+                C, rows_per_mask, p, seed, offset, H.ptr(step))
     return y
 
 
 class _DropoutAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, res, rows_per_mask, p, seed, offset, step):
-        ctx.save_for_backward(step)
+        if step is not None:
+            ctx.save_for_backward(step)
         ctx.args = (rows_per_mask, p, seed, offset)
         return _dropout(_dense(x), None if res is None else _dense(res), rows_per_mask, p, seed, offset, step)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        step, = ctx.saved_tensors
-        dx = _dropout(_dense(dy), None, *ctx.args, step) if ctx.needs_input_grad[0] else None
+        saved = ctx.saved_tensors
+        dx = None
+        if ctx.needs_input_grad[0]:
+            dx = _dropout(_dense(dy), None, *ctx.args, saved[0] if saved else None)
         return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
 
 
@@ -272,7 +263,6 @@ def dropout_add(x, residual=None, p=0.5, seed=0, offset=0, step=None, rows_per_m
 
 
 # ---- 8-bit integers ----
-@torch.no_grad()
 def quantize_rows(x):
     """(q int8 [..., K], scale fp32 [...]): scale = max |row| / 127, q = rint(row / scale). A row of
     zeros has scale 0; a row that holds an infinity or a NaN has scale NaN."""
@@ -282,11 +272,10 @@ def quantize_rows(x):
         raise H.HgkError("quantize_rows: expected [..., K]")
     _gpu("quantize_rows", x)
     x = _dense(x)
-    with _on(x) as st:
-        q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
-        s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-        H.check(H.lib().hgk_quantize_rows_i8(st, dt, x.data_ptr(), q.data_ptr(), s.data_ptr(), s.numel(),
-                                             x.shape[-1]))
+    q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
+    s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
+    _launch(x, H.lib().hgk_quantize_rows_i8, dt, x.data_ptr(), q.data_ptr(), s.data_ptr(), s.numel(),
+            x.shape[-1])
     return q, s
 
 
@@ -296,7 +285,6 @@ def _scale(what, s, n):
     return None if s is None else _dense(s)
 
 
-@torch.no_grad()
 def linear_i8(x, w, w_scale, bias=None, residual=None):
     """x w^T (+ bias + residual) in 8-bit integers: x [..., K] fp32 / bf16 is quantised row by row
     (quantize_rows), w is int8 [N, K] with w_scale fp32 [N] (quantize_rows of the weights), bias fp32
@@ -315,15 +303,13 @@ def linear_i8(x, w, w_scale, bias=None, residual=None):
     x, w = _dense(x), _dense(w)
     residual = None if residual is None else _dense(residual)
     M, lib = x.numel() // K, H.lib()
-    with _on(x) as st:
-        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-        wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, K, N, 0), x)
-        H.check(lib.hgk_linear_i8(st, dt, x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), H.ptr(bias),
-                                  H.ptr(residual), y.data_ptr(), M, K, N, wp, n))
+    y = x.new_empty((*x.shape[:-1], N))
+    wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, K, N, 0), x)
+    _launch(x, lib.hgk_linear_i8, dt, x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), H.ptr(bias),
+            H.ptr(residual), y.data_ptr(), M, K, N, wp, n)
     return y
 
 
-@torch.no_grad()
 def gated_linear_i8(x, w_gate, gate_scale, w_up, up_scale, activation="silu"):
     """gated_linear with both products in 8-bit integers (see linear_i8): w_gate and w_up int8 [F, C]
     with a scale for each row. No gradient."""
@@ -337,11 +323,10 @@ def gated_linear_i8(x, w_gate, gate_scale, w_up, up_scale, activation="silu"):
     _gpu("gated_linear_i8", x)
     x, wg, wu = _dense(x), _dense(w_gate), _dense(w_up)
     M, lib = x.numel() // C, H.lib()
-    with _on(x) as st:
-        h = torch.empty(*x.shape[:-1], F, dtype=x.dtype, device=x.device)
-        wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, C, F, 1), x)
-        H.check(lib.hgk_gated_i8(st, dt, x.data_ptr(), wg.data_ptr(), sg.data_ptr(), wu.data_ptr(),
-                                 su.data_ptr(), h.data_ptr(), M, C, F, act, wp, n))
+    h = x.new_empty((*x.shape[:-1], F))
+    wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, C, F, 1), x)
+    _launch(x, lib.hgk_gated_i8, dt, x.data_ptr(), wg.data_ptr(), sg.data_ptr(), wu.data_ptr(),
+            su.data_ptr(), h.data_ptr(), M, C, F, act, wp, n)
     return h
 
 

@@ -66,6 +66,31 @@ def test_gated_wide_tiles(M, C, Fh):
         R.worst(g, w, what)
 
 
+# every tile size on sizes that do not fill it, one step of k and several, k past the ring's depth
+@pytest.mark.parametrize("tile", [64, 128, 192, 256])
+@pytest.mark.parametrize("M,C,Fh", [(65, 8, 9), (300, 72, 40), (129, 33, 257), (700, 264, 300), (1000, 520, 129)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_every_tile(tile, M, C, Fh, dtype, routes):
+    routes(ffn_tile=tile)
+    got, (x, wg, wu, dh) = gated_case(M, C, Fh, dtype, "silu", seed=tile)
+    want = R.gated(*(v.detach().double() for v in (x, wg, wu)), "silu", dtype, dh.double())
+    for g, w, what in zip(got, want, ("h", "dx", "dw_gate", "dw_up")):
+        R.worst(g, w, what)
+    h, w, res, dy = (t.detach().requires_grad_() for t in (got[0], rnd(5, C, Fh, dtype=dtype), rnd(6, M, C, dtype=dtype),
+                                                           rnd(7, M, C, dtype=dtype)))
+    y = F.linear_dropout_add(h, w, res, 0.3, seed=1, offset=2)
+    want = R.linear(h.detach().double(), w.detach().double(), res.detach().double(), R.kept(M, C, 0.3, 1, 2).to(DEV), 0.3,
+                    dtype, dy.detach().double())
+    for g, v, what in zip((y.detach(), *torch.autograd.grad(y, (h, w), dy.detach())), want, ("y", "dh", "dw")):
+        R.worst(g, v, what)
+    (qg, sg), (q, s) = F.quantize_rows(wg), R.quantize(x.detach())
+    v, e = (t.to(DEV) for t in R.product_i8(q, s, qg.cpu(), sg.cpu()))
+    R.worst(F.linear_i8(x.detach(), qg, sg), (v, e + R.U[dtype] * (v.abs() + e)))
+    a, ea = R.act("relu", v), e
+    R.worst(F.gated_linear_i8(x.detach(), qg, sg, qg, sg, "relu"),
+            (a * v, ea * (v.abs() + e) + a * e + 2 ** -23 * (a * v).abs() + R.U[dtype] * (a * v).abs() * 1.001 + R.TINY))
+
+
 @pytest.mark.parametrize("M", [1, 16, 40, 64])
 @pytest.mark.parametrize("dtype", TYPES)
 def test_gated_few_rows_long(M, dtype):
