@@ -90,9 +90,9 @@ const char* hgk_last_error(void);
  *                           total, go to ONE halo launch whose splits run over the concatenated
  *                           tiles (each slab read-modified-written once per launch, not per use;
  *                           the other uses take the implicit GEMM multi launch); default 128; 0 = off
- *   HGK_ROUTE_FFN_TILE      feed-forward products (hgk_gated_*, hgk_linear_*, *_i8) on tiles of
- *                           64 x 64 (64), 128 x 128 (128), 128 x 256 (192; not fp32) or 256 x 256
- *                           (256; not fp32) wherever the tiled kernel runs; 0 (default): by the sizes
+ *   HGK_ROUTE_FFN_TILE      feed-forward products (hgk_gated_*, hgk_linear_*, *_i8) on tiles of 64,
+ *                           128 or 256 (not fp32) rows and columns wherever the tiled kernel runs;
+ *                           0 (default): by the sizes
  * hgk_set_route returns the previous value (HGK_ERR_ARG for an unknown knob); a negative value
  * restores the default. */
 enum {

@@ -74,7 +74,7 @@ struct GatedWs {
 };
 static GatedWs gated_ws(int dtype, long M, int C, int F, bool bwd) {
   GatedWs w;
-  const int es = es_of(dtype), q = 16 / es, ks = 64 / es;
+  const int es = es_of(dtype), q = 16 / es, ks = 128 / es;
   w.Cp = (int)up_to(C, q);
   w.Fp = (int)up_to(F, 8);
   w.pad = w.Cp != C;
@@ -119,7 +119,7 @@ static void gated_operands(hipStream_t st, GemmArgs& a, const GatedWs& w, char* 
   a.M = (int)M;
   a.N = F;
   a.km = a.kn = w.Cp;
-  a.spseg = (int)up_to((long)w.Cp * sizeof(T), 64) / 64;
+  a.spseg = (int)up_to((long)w.Cp * sizeof(T), 128) / 128;
 }
 
 template <typename T>
@@ -147,7 +147,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
                      void* dx, void* dwg, void* dwu, long M, int C, int F, int act, char* ws,
                      int dtype) {
   constexpr int DT = TypeOf<T>::dt;
-  constexpr int es = sizeof(T), ks = 64 / es;
+  constexpr int es = sizeof(T), ks = 128 / es;
   const GatedWs w = gated_ws(dtype, M, C, F, true);
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
@@ -208,7 +208,7 @@ struct LinearWs {
 };
 static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) {
   LinearWs w;
-  const int es = es_of(dtype), q = 16 / es, ks = 64 / es;
+  const int es = es_of(dtype), q = 16 / es, ks = 128 / es;
   w.Kp = (int)up_to(K, q);
   w.Np = (int)up_to(N, q);
   w.pad_k = w.Kp != K;
@@ -250,7 +250,7 @@ static int linear_fwd(hipStream_t st, const void* x, const void* wt, const void*
   a.M = (int)M;
   a.N = N;
   a.km = a.kn = w.Kp;
-  a.spseg = (int)up_to((long)w.Kp * sizeof(T), 64) / 64;
+  a.spseg = (int)up_to((long)w.Kp * sizeof(T), 128) / 128;
   a.out = y;
   a.res = res;
   a.vec = N % 8 == 0;
@@ -268,7 +268,7 @@ template <typename T>
 static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void* dy, void* dx, void* dw,
                       long M, int K, int N, const DropArgs& d, char* ws, int dtype) {
   constexpr int DT = TypeOf<T>::dt;
-  constexpr int es = sizeof(T), ks = 64 / es;
+  constexpr int es = sizeof(T), ks = 128 / es;
   typedef typename TypeOf<T>::raw raw;
   const bool drop = d.thr != 0;
   const LinearWs w = linear_ws(dtype, M, K, N, drop, true);

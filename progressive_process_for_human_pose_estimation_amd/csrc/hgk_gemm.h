@@ -4,23 +4,27 @@
 //   D[m][n] = sum_k A(m, k) B(n, k)
 //
 // Byte geometry. Everything is counted in 16-byte chunks, so one address plan serves 8-bit
-// integers, bf16 and fp32: a K-step is 64 bytes of a row, a fragment is one chunk a lane
-// (16 bytes = 16 int8 / 8 bf16 / 4 fp32 values of k), and a step's fragment pair is one
-// mfma_i32_16x16x64_i8, one mfma_f32_16x16x32_bf16 or four mfma_f32_16x16x4_f32.
+// integers, bf16 and fp32: a K-step is 128 bytes of a row (a whole cache line), a fragment is one
+// chunk a lane (16 bytes = 16 int8 / 8 bf16 / 4 fp32 values of k), and a half step's fragment pair
+// is one mfma_i32_16x16x64_i8, one mfma_f32_16x16x32_bf16 or four mfma_f32_16x16x4_f32.
 //
 // Operand layouts.
-//   ROW: k runs along memory. LDS tile [rows][64 B]; chunk c of row r sits at slot
-//        c ^ ((r >> 1) & 3), so the 8 rows that a b128 read takes at a time touch all banks once.
+//   ROW: k runs along memory. LDS tile [rows][128 B]; chunk c of row r sits at slot c ^ (r & 7),
+//        so the 8 rows that a b128 read takes at a time touch all banks once.
 //   COL: k is the row index (weights of an input gradient, both operands of a weight gradient).
 //        LDS tile [KS rows][tile columns], read as transposed fragments
 //        (ds_read_b64_tr_b16; fp32: four b32 reads), slots swizzled by swz_col() below.
 // Global -> LDS by LDS-DMA (16 bytes a lane, no registers); the swizzle is in the source address
 // a lane picks, the LDS side is written in order.
 //
-// Pipeline. A ring of S K-steps in LDS, one barrier a step: at step t the barrier says that step
-// t + 1 has landed and that every wave holds step t's fragments in registers, so the DMA of step
-// t + S may go into t's slot, and the fragments of t + 1 are read while the matrix instructions of
-// t run. S - 1 steps are on their way at any time.
+// Pipeline. The tiles of the two sides of each K-step are units M0 N0 M1 N1 .. in a ring of five
+// LDS slots. In the first half of step P the unit M(P + 2) is sent for, the second half's fragments
+// are read and the first half's products run; then one barrier says that step P + 1 has landed and
+// step P is in registers; in the second half N(P + 2) is sent for (into M(P)'s slot), the next
+// step's first fragments are read and the second half's products run. Each unit is on its way
+// for two to three half steps. Lines are asked for whole: with 64-byte K-steps, four slots of both
+// sides and a barrier each, the address units took twice as many requests and an
+// 8192 x 4096 x 8192 product ran at 1227 TFLOP/s (1651 with the DMAs left out).
 //
 // The matrix instruction's A operand is the N side and its B operand the M side: a lane then holds
 // 4 consecutive n of one row m.
@@ -228,20 +232,19 @@ __device__ __forceinline__ int swz_col(int p) {
 }
 
 // T: type of outputs, residual and dh
-template <int DT, typename T, int LM, int LN, int BM, int BN, int WM, int WN, int S, int EPI>
+template <int DT, typename T, int LM, int LN, int BT, int WM, int WN, int EPI>
 __global__ __launch_bounds__(WM * WN * 64) __attribute__((amdgpu_waves_per_eu(2)))
 void gemm_kernel(GemmArgs a) {
-  constexpr int NW = WM * WN, es = GT<DT>::es;
-  constexpr int KS = 64 / es;                // k per step
+  constexpr int NW = WM * WN, es = GT<DT>::es, BM = BT, BN = BT;
+  constexpr int KS = 128 / es;               // k per step
   constexpr bool DUAL = EPI == E_GATED || EPI == E_GATED_BWD;
-  constexpr int PM = BM * 64, PN = BN * 64, SB = PM + PN;    // LDS bytes of a step
-  constexpr int DM = BM / 16 / NW, DN = BN / 16 / NW, D = DM + DN;  // 1-KB DMAs of a wave per step
-  static_assert(BM % (16 * NW) == 0 && BN % (16 * NW) == 0, "whole DMAs per wave");
-  static_assert(BM * es >= 128 || LM == L_ROW, "COL swizzle needs 8 chunks a row");
+  constexpr int UB = BT * 128;               // LDS bytes of a unit
+  constexpr int D = BT / 8 / NW;             // 1-KB DMAs of a wave per unit
+  static_assert(BT % (8 * NW) == 0, "whole DMAs per wave");
   static_assert(DT != G_I8 || (LM == L_ROW && LN == L_ROW), "8-bit operands are ROW");
   constexpr int WTM = BM / WM, WTN = BN / WN, FM = WTM / 16, FN = WTN / 16;
   static_assert(!DUAL || FN % 2 == 0, "gate and up halves");
-  __shared__ __attribute__((aligned(16))) char lds[S * SB];
+  __shared__ __attribute__((aligned(16))) char lds[5 * UB];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
@@ -267,90 +270,88 @@ void gemm_kernel(GemmArgs a) {
   // ---- DMA sources: a base that moves with the steps and an offset a lane (host: 256 rows of an
   // operand are less than 4 GB) ----
   const int seg0 = s0 / a.spseg;
-  int kin = s0 - seg0 * a.spseg;
-  const long stepm = LM == L_ROW ? 64 : (long)KS * a.ldm, stepn = LN == L_ROW ? 64 : (long)KS * a.ldn;
-  const char* bm = ((a.batch > 1 ? bat : seg0) ? a.m1 : a.m0) + kin * stepm;
-  const char* bn = (!DUAL && a.nseg > 1 && seg0 ? a.n1 : a.n0) + kin * stepn;
-  long dual = 0;  // E_GATED*: up weights minus gate weights, in bytes
-  if (DUAL) dual = a.n1 - a.n0;
+  const long stepm = LM == L_ROW ? 128 : (long)KS * a.ldm, stepn = LN == L_ROW ? 128 : (long)KS * a.ldn;
+  int kinm = s0 - seg0 * a.spseg, kinn = kinm;
+  const char* bm = ((a.batch > 1 ? bat : seg0) ? a.m1 : a.m0) + kinm * stepm;
+  const char* bn = (!DUAL && a.nseg > 1 && seg0 ? a.n1 : a.n0) + kinn * stepn;
   if (LM == L_ROW) bm += (long)m0 * a.ldm;
   if (LN == L_ROW) bn += (long)n0 * a.ldn;
-  uint32_t om[DM], on[DN];
-  const int rchunk = (lane & 3) ^ ((lane >> 3) & 3);  // ROW: chunk of every DMA of this lane
-  constexpr int CM = BM * es / 16, CN = BN * es / 16;  // COL: chunks per LDS row
-  auto colrow = [&](int d, int C) { return ((d * NW + wave) * 64 + lane) / C; };
+  const char* bu = bn;  // E_GATED*: the up weights
+  if (DUAL) bu += a.n1 - a.n0;
+  const long jumpm = (a.m1 - a.m0) - a.spseg * stepm, jumpn = (a.n1 - a.n0) - a.spseg * stepn;
+  uint32_t om[D], on[D];
+  const int rchunk = (lane & 7) ^ ((lane >> 3) & 7);  // ROW: chunk of every DMA of this lane
+  constexpr int CH = BT * es / 16;                    // COL: chunks per LDS row
+  auto colrow = [&](int d) { return ((d * NW + wave) * 64 + lane) / CH; };
 #pragma unroll
-  for (int d = 0; d < DM; ++d) {
-    if (LM == L_ROW) {
-      const int r = min((d * NW + wave) * 16 + (lane >> 2), a.M - 1 - m0);
-      om[d] = (uint32_t)r * (uint32_t)a.ldm + rchunk * 16;
-    } else {
-      const int p = colrow(d, CM);
-      const int c = (((d * NW + wave) * 64 + lane) % CM) ^ swz_col<DT, CM>(p);
-      om[d] = (uint32_t)p * (uint32_t)a.ldm + min(m0 * es + c * 16, (a.M * es - 1) & ~15);
-    }
+  for (int d = 0; d < D; ++d) {
+    const int row = (d * NW + wave) * 8 + (lane >> 3), p = colrow(d);
+    const int c = (((d * NW + wave) * 64 + lane) % CH) ^ swz_col<DT, CH>(p);
+    if (LM == L_ROW) om[d] = (uint32_t)min(row, a.M - 1 - m0) * (uint32_t)a.ldm + rchunk * 16;
+    else om[d] = (uint32_t)p * (uint32_t)a.ldm + min(m0 * es + c * 16, (a.M * es - 1) & ~15);
+    // gated: the first half of the tile's rows are gate rows, the second up rows
+    if (LN == L_ROW) on[d] = (uint32_t)min(DUAL ? row % (BN / 2) : row, a.N - 1 - n0) * (uint32_t)a.ldn + rchunk * 16;
+    else on[d] = (uint32_t)p * (uint32_t)a.ldn + min(n0 * es + c * 16, (a.N * es - 1) & ~15);
   }
-#pragma unroll
-  for (int d = 0; d < DN; ++d) {
-    if (LN == L_ROW) {
-      // gated: the first half of the tile's rows are gate rows, the second up rows
-      const int r = (d * NW + wave) * 16 % (DUAL ? BN / 2 : BN) + (lane >> 2);
-      on[d] = (uint32_t)min(r, a.N - 1 - n0) * (uint32_t)a.ldn + rchunk * 16;
-    } else {
-      const int p = colrow(d, CN);
-      const int c = (((d * NW + wave) * 64 + lane) % CN) ^ swz_col<DT, CN>(p);
-      on[d] = (uint32_t)p * (uint32_t)a.ldn + min(n0 * es + c * 16, (a.N * es - 1) & ~15);
-    }
-  }
-  static_assert(!DUAL || BN % 32 == 0, "a DMA brings gate rows or up rows");
+  static_assert(!DUAL || BN / 2 % (8 * NW) == 0, "DMA d of every wave brings gate rows or up rows");
   const bool tail_m = a.km % KS != 0, tail_n = a.kn % KS != 0;
-  // DMA d of the step at (bm, bn, kin) into its slot; in a segment's last step the zero page stands
-  // in for k past the end
-  auto dma = [&](int d, int slot, bool tail) __attribute__((always_inline)) {
-    const bool mside = d < DM;
-    const int e = mside ? d : d - DM;
-    char* to = lds + slot * SB + (mside ? 0 : PM) + (e * NW + wave) * 1024;
-    const char* base = mside ? bm : bn + (DUAL && (e * NW + wave) * 16 >= BN / 2 ? dual : 0);
-    const uint32_t off = mside ? om[e % DM] : on[e % DN];
-    if (tail) {
-      const int lay = mside ? LM : LN, k = mside ? a.km : a.kn;
-      const bool ok = lay == L_ROW ? kin * 64 + rchunk * 16 < k * es
-                                   : kin * KS + colrow(e, mside ? CM : CN) < k;
+  // DMA d of the M (N) side's next unit into a slot. TAIL: a segment's last step, where the zero page
+  // stands in for k past the end
+  auto dma = [&](auto nside, auto tail, int d, int slot) __attribute__((always_inline)) {
+    constexpr bool NS = decltype(nside)::value, TAIL = decltype(tail)::value;
+    char* to = lds + slot * UB + (d * NW + wave) * 1024;
+    const char* base = NS ? (DUAL && d * NW * 8 >= BN / 2 ? bu : bn) : bm;
+    const uint32_t off = NS ? on[d] : om[d];
+    if constexpr (TAIL) {
+      const int k = NS ? a.kn : a.km, kin = NS ? kinn : kinm;
+      const bool ok = (NS ? LN : LM) == L_ROW ? kin * 128 + rchunk * 16 < k * es : kin * KS + colrow(d) < k;
       dma16(ok ? base + off : g_zero_page, to);
     } else {
       dma16s(base, off, to);
     }
   };
-  auto is_tail = [&]() { return (tail_m || tail_n) && kin + 1 == a.spseg; };
-  auto advance = [&]() __attribute__((always_inline)) {
-    const bool last = kin + 1 == a.spseg;
-    ++kin;
-    bm += stepm;
-    bn += stepn;
-    if (a.nseg > 1 && last) {  // on to the second segment
-      bm += (a.m1 - a.m0) - a.spseg * stepm;
-      bn += (a.n1 - a.n0) - a.spseg * stepn;
-      kin = 0;
-    }
+  auto is_tail = [&](auto nside) {
+    constexpr bool NS = decltype(nside)::value;
+    return (NS ? tail_n : tail_m) && (NS ? kinn : kinm) + 1 == a.spseg;
   };
-  auto issue = [&](int slot) __attribute__((always_inline)) {
-    const bool tail = is_tail();
+  auto advance = [&](auto nside) __attribute__((always_inline)) {
+    constexpr bool NS = decltype(nside)::value;
+    int& kin = NS ? kinn : kinm;
+    long by = NS ? stepn : stepm;
+    if (!DUAL) {  // past a segment's end: on to the second one
+      const bool over = kin + 1 == a.spseg && a.nseg > 1;
+      by += over ? (NS ? jumpn : jumpm) : 0;
+      kin = over ? 0 : kin + 1;
+    } else {
+      ++kin;
+    }
+    (NS ? bn : bm) += by;
+    if (DUAL && NS) bu += by;
+  };
+  const std::false_type side_m;
+  const std::true_type side_n;
+  auto send = [&](auto nside, int slot) __attribute__((always_inline)) {
+    if (is_tail(nside)) {
 #pragma unroll
-    for (int d = 0; d < D; ++d) dma(d, slot, tail);
-    advance();
+      for (int d = 0; d < D; ++d) dma(nside, std::true_type(), d, slot);
+    } else {
+#pragma unroll
+      for (int d = 0; d < D; ++d) dma(nside, std::false_type(), d, slot);
+    }
+    advance(nside);
   };
 
   // ---- fragments of a step ----
-  const int xr = lr * 64 + ((lg ^ ((lr >> 1) & 3)) << 4);
+  const int x0 = lr * 128 + ((lg ^ (lr & 7)) << 4), x1 = lr * 128 + (((lg + 4) ^ (lr & 7)) << 4);
   auto rown = [&](int f) {
     return DUAL ? (f < FN / 2 ? wn * (WTN / 2) + f * 16 : BN / 2 + wn * (WTN / 2) + (f - FN / 2) * 16)
                 : wn * WTN + f * 16;
   };
   typedef short s16x8 __attribute__((ext_vector_type(8)));
-  auto frag_col = [&](const char* t, auto chunks, int col) __attribute__((always_inline)) -> i32x4 {
-    constexpr int CH = decltype(chunks)::value, pitch = CH * 16;
+  auto frag_col = [&](const char* t, int col, int h) __attribute__((always_inline)) -> i32x4 {
+    constexpr int pitch = CH * 16;
     if constexpr (DT == G_BF16) {
-      const int p = 8 * lg + (lr >> 2), c = col + 4 * (lr & 3);
+      const int p = 32 * h + 8 * lg + (lr >> 2), c = col + 4 * (lr & 3);
       const char* q = t + p * pitch + (((c >> 3) ^ swz_col<DT, CH>(p)) << 4) + (c & 7) * 2;
       const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
@@ -362,7 +363,7 @@ void gemm_kernel(GemmArgs a) {
       const int c = col + lr;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int p = 4 * lg + i;
+        const int p = 16 * h + 4 * lg + i;
         v[i] = *reinterpret_cast<const int*>(t + p * pitch + (((c >> 2) ^ swz_col<DT, CH>(p)) << 4) + (c & 3) * 4);
       }
       return v;
@@ -371,17 +372,17 @@ void gemm_kernel(GemmArgs a) {
   struct Frags {
     i32x4 m[FM], n[FN];
   };
-  // fragment r of a step: the N side's first
-  auto read1 = [&](int slot, Frags& f, int r) __attribute__((always_inline)) {
-    const char* tm = lds + slot * SB;
-    const char* tn = tm + PM;
+  // fragment r of half h of a step: the N side's first
+  auto read1 = [&](int um, int un, int h, Frags& f, int r) __attribute__((always_inline)) {
+    const char* tm = lds + um * UB;
+    const char* tn = lds + un * UB;
     if (r < FN) {
-      f.n[r % FN] = LN == L_ROW ? *reinterpret_cast<const i32x4*>(tn + rown(r) * 64 + xr)
-                                : frag_col(tn, std::integral_constant<int, CN>(), rown(r));
+      f.n[r % FN] = LN == L_ROW ? *reinterpret_cast<const i32x4*>(tn + rown(r) * 128 + (h ? x1 : x0))
+                                : frag_col(tn, rown(r), h);
     } else {
       const int i = r - FN;
-      f.m[i % FM] = LM == L_ROW ? *reinterpret_cast<const i32x4*>(tm + (wm * WTM + i * 16) * 64 + xr)
-                                : frag_col(tm, std::integral_constant<int, CM>(), wm * WTM + i * 16);
+      f.m[i % FM] = LM == L_ROW ? *reinterpret_cast<const i32x4*>(tm + (wm * WTM + i * 16) * 128 + (h ? x1 : x0))
+                                : frag_col(tm, wm * WTM + i * 16, h);
     }
   };
 
@@ -391,59 +392,75 @@ void gemm_kernel(GemmArgs a) {
 #pragma unroll
     for (int j = 0; j < FM; ++j) acc[i][j] = typename GT<DT>::acc{0, 0, 0, 0};
 
-  // all but the last `ahead` steps issued have landed, here and (after the barrier) in every wave
-  auto wait = [&](int ahead) __attribute__((always_inline)) {
-    if (ahead >= S - 2) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((S - 2) * D) : "memory");
-    else if (S > 3 && ahead == 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(D) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-  static_assert(S == 3 || S == 4, "wait() counts one or two steps beyond the one it waits for");
-  const int nt = s1 - s0;
-#pragma unroll
-  for (int t = 0; t < S; ++t)
-    if (t < nt) issue(t);
-  if (nt >= S) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((S - 1) * D) : "memory");  // step 0 has landed
-  else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  const int np = s1 - s0;
+  send(side_m, 0);
+  send(side_n, 1);
+  if (np > 1) {
+    send(side_m, 2);
+    send(side_n, 3);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * D) : "memory");  // step 0 has landed
+  } else {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  }
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
   Frags fa, fb;
 #pragma unroll
-  for (int r = 0; r < FN + FM; ++r) read1(0, fa, r);
-  // A step in FM parts: each takes its share of the next DMAs and fragment reads along with the
-  // products of one fragment row. All DMAs first, as written plainly, hold every wave behind the
-  // barrier until the address unit has taken them (16 clocks each): 8192 x 2048 x (2 x 2048) ran
-  // with the matrix cores 50 % busy.
-  int slot = 0;
-  auto step = [&](int t, const Frags& cur, Frags& next) __attribute__((always_inline)) {
-    wait(nt - 2 - t);
-    const bool more = t + S < nt, tail = is_tail();
-    const int ns = slot + 1 == S ? 0 : slot + 1;
+  for (int r = 0; r < FN + FM; ++r) read1(0, 1, 0, fa, r);
+  auto wrap = [](int slot) { return slot >= 5 ? slot - 5 : slot; };
+  // half a step in FM parts: each takes its share of the DMAs and of the next half's fragment reads
+  // along with the products of one fragment row. All DMAs first hold every wave behind the barrier
+  // until the address unit has taken them; a branch around each DMA takes longer than the other
+  // wave's share of matrix instructions lasts.
+  // PLAIN: the DMAs are neither missing nor a segment's last
+  auto half = [&](auto is_plain, auto nside, bool more, int to, int um, int un, int h, const Frags& cur,
+                  Frags& nxt) __attribute__((always_inline)) {
+    constexpr bool PLAIN = decltype(is_plain)::value;
+    const bool last = !PLAIN && is_tail(nside);
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
 #pragma unroll
-      for (int r = (FN + FM) * i / FM; r < (FN + FM) * (i + 1) / FM; ++r)
-        read1(ns, next, r);  // past the last step: whatever the slot holds, unused
+      for (int r = (FN + FM) * i / FM; r < (FN + FM) * (i + 1) / FM; ++r) read1(um, un, h, nxt, r);
 #pragma unroll
       for (int j = 0; j < FN; ++j) acc[j][i] = mma<DT>(cur.n[j], cur.m[i], acc[j][i]);
-      // the compiler may not carry these products past the next barrier
+      // the parts stay as they are written, and no product is carried past the next barrier
 #pragma unroll
       for (int j = 0; j < FN; ++j) asm volatile("" : "+v"(acc[j][i]));
-      if (more) {
 #pragma unroll
-        for (int d = D * i / FM; d < D * (i + 1) / FM; ++d) dma(d, slot, tail);
+      for (int d = D * i / FM; d < D * (i + 1) / FM; ++d) {
+        if (PLAIN) {
+          dma(nside, std::false_type(), d, to);
+        } else if (more) {
+          if (last) dma(nside, std::true_type(), d, to);
+          else dma(nside, std::false_type(), d, to);
+        }
       }
+      __builtin_amdgcn_sched_barrier(0);
     }
-    if (more) advance();
-    slot = ns;
+    if (PLAIN || more) advance(nside);
   };
+  int s = 0;  // slot of M(P)
+  auto step = [&](auto is_plain, bool more) __attribute__((always_inline)) {
+    half(is_plain, side_m, more, wrap(s + 4), s, wrap(s + 1), 1, fa, fb);
+    // step P + 1 has landed (M(P + 2) may be on its way), step P is in registers: of every wave
+    // after the barrier
+    if (decltype(is_plain)::value || more) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(D) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // past the last step the fragments are whatever the slots hold, and unused
+    half(is_plain, side_n, more, s, wrap(s + 2), wrap(s + 3), 0, fb, fa);
+    s = wrap(s + 2);
+  };
+  const bool tails = tail_m || tail_n;
 #pragma unroll 1
-  for (int t = 0;;) {
-    step(t, fa, fb);
-    if (++t == nt) break;
-    step(t, fb, fa);
-    if (++t == nt) break;
+  for (int P = 0; P < np; ++P) {
+    // a run of steps without a branch, up to one that sends a segment's last step or nothing
+    int lim = np - 2;
+    if (tails) lim = min(lim, P + a.spseg - 1 - kinm);
+#pragma unroll 1
+    for (; P < lim; ++P) step(std::true_type(), true);
+    step(std::false_type(), P + 2 < np);
   }
 
   // ---- epilogue. The sums go through LDS 16 rows of a wave at a time, so that a lane gets 8
@@ -456,7 +473,7 @@ void gemm_kernel(GemmArgs a) {
   constexpr int GP = CW / 8, RP = 64 / GP < 16 ? 64 / GP : 16, NP = 16 / RP, PITCH = CW + 4;
   static_assert(GP >= 2 && RP <= 32, "wave tile");
   constexpr int PARTS = DUAL ? 2 : 1;
-  static_assert(NW * PARTS * 16 * PITCH * 4 <= S * SB, "scratch fits the stages");
+  static_assert(NW * PARTS * 16 * PITCH * 4 <= 5 * UB, "scratch fits the slots");
   __syncthreads();
   float* scr = reinterpret_cast<float*>(lds) + wave * (PARTS * 16 * PITCH);
   const int cg = lane % GP, r0 = (lane / GP) % RP;
@@ -723,25 +740,24 @@ static inline void launch_pad(hipStream_t st, const void* src, void* dst, long r
 
 // ---- tile size and split of a product ----
 struct GemmPlan {
-  int tile;  // 64: 64 x 64, 128: 128 x 128, 192: 128 x 256, 256: 256 x 256
+  int tile;  // rows and columns
   int tiles_m, tiles_n, splits;
   long slab;  // bytes
 };
-// per: a gated tile holds 2 x (columns / 2) columns. wide: the type has 128 x 256 and 256 x 256 tiles
+// per: a gated tile holds 2 x (columns / 2) columns. wide: the type has tiles of 256
 static inline GemmPlan plan_gemm(bool wide, long M, long N, int per, int steps, int batch, bool can_split) {
   GemmPlan p;
-  auto tiles = [&](int bm, int bn) { return ((M + bm - 1) / bm) * ((N + bn / per - 1) / (bn / per)) * batch; };
+  auto tiles = [&](int b) { return ((M + b - 1) / b) * ((N + b / per - 1) / (b / per)) * batch; };
   const int asked = (int)route(HGK_ROUTE_FFN_TILE);
-  if (asked == 64 || asked == 128 || (wide && (asked == 192 || asked == 256))) p.tile = asked;
-  else if (wide && tiles(256, 256) >= 256) p.tile = 256;
-  else if (tiles(128, 128) >= 256) p.tile = 128;
+  if (asked == 64 || asked == 128 || (wide && asked == 256)) p.tile = asked;
+  else if (wide && tiles(256) >= 256) p.tile = 256;
+  else if (tiles(128) >= 256) p.tile = 128;
   else p.tile = 64;
-  const int bm = p.tile == 192 ? 128 : p.tile, bn = (p.tile == 192 ? 256 : p.tile) / per;
-  p.tiles_m = (int)((M + bm - 1) / bm);
-  p.tiles_n = (int)((N + bn - 1) / bn);
-  const long n = (long)p.tiles_m * p.tiles_n * batch, fill = p.tile == 256 ? 256 : p.tile == 64 ? 1024 : 512;
+  p.tiles_m = (int)((M + p.tile - 1) / p.tile);
+  p.tiles_n = (int)((N + p.tile / per - 1) / (p.tile / per));
+  const long n = tiles(p.tile), fill = p.tile == 256 ? 256 : p.tile == 64 ? 1024 : 512;
   p.splits = 1;
-  if (can_split && n * 2 <= fill) p.splits = (int)std::max(1l, std::min<long>(fill / n, steps / 8));
+  if (can_split && n * 2 <= fill) p.splits = (int)std::max(1l, std::min<long>(fill / n, steps / 4));
   p.slab = p.splits > 1 ? (long)p.splits * batch * M * N * 4 : 0;
   return p;
 }
@@ -762,16 +778,12 @@ static void run_tiles(hipStream_t st, GemmArgs& a, const GemmPlan& p) {
   const dim3 grid((unsigned)((long)a.tiles_m * a.tiles_n * a.batch * a.splits));
   if constexpr (DT != G_F32) {
     if (p.tile == 256) {
-      hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 256, 256, 4, 2, 4, EPI>), grid, dim3(512), 0, st, a);
-      return;
-    }
-    if (p.tile == 192) {
-      hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 256, 2, 2, 3, EPI>), grid, dim3(256), 0, st, a);
+      hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 256, 4, 2, EPI>), grid, dim3(512), 0, st, a);
       return;
     }
   }
-  if (p.tile == 128) hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 128, 2, 2, 4, EPI>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 64, 64, 2, 2, 4, EPI>), grid, dim3(256), 0, st, a);
+  if (p.tile == 128) hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 2, 2, EPI>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 64, 2, 2, EPI>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace hgk

@@ -150,7 +150,7 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
   a.M = (int)M;
   a.N = N;
   a.km = a.kn = w.Kp;
-  a.spseg = (w.Kp + 63) / 64;
+  a.spseg = (w.Kp + 127) / 128;
   a.out = y;
   a.row_scale = (const float*)(ws + w.s);
   a.col_scale = s0;
