@@ -88,8 +88,8 @@ static GatedWs gated_ws(int dtype, long M, int C, int F, bool bwd) {
   if (bwd) {
     w.dg = c.take(M * w.Fp * es);
     w.du = c.take(M * w.Fp * es);
-    w.dx = plan_gemm(dtype == HGK_BF16, M, C, 1, 2 * (int)((F + ks - 1) / ks), 1, true);
-    w.dw = plan_gemm(dtype == HGK_BF16, F, C, 1, (int)((M + ks - 1) / ks), 2, true);
+    w.dx = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, C, 1, 2 * (int)((F + ks - 1) / ks), 1, true);
+    w.dw = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, F, C, 1, (int)((M + ks - 1) / ks), 2, true);
     w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
   }
   w.total = c.at;
@@ -135,7 +135,7 @@ static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* 
   if (M <= kSkinnyRows) {
     run_skinny<DT, T, true>(st, a);
   } else {
-    const GemmPlan p = plan_gemm(dtype == HGK_BF16, M, F, 2, a.spseg, 1, false);
+    const GemmPlan p = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, F, 2, a.spseg, 1, false);
     run_tiles<DT, T, L_ROW, L_ROW, E_GATED>(st, a, p);
   }
   HGK_LAUNCH_CHECK();
@@ -158,7 +158,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
   a.npad = w.Fp;
   a.act = act;
   a.vec = F % 8 == 0;
-  const GemmPlan p = plan_gemm(dtype == HGK_BF16, M, F, 2, a.spseg, 1, false);
+  const GemmPlan p = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, F, 2, a.spseg, 1, false);
   run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p);
   HGK_LAUNCH_CHECK();
   if (dx) {
@@ -219,12 +219,12 @@ static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) 
     w.x = c.take(M * w.Kp * es);
     w.w = c.take((long)N * w.Kp * es);
   }
-  w.fwd = plan_gemm(dtype == HGK_BF16, M, N, 1, (int)((w.Kp + ks - 1) / ks), 1, true);
+  w.fwd = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, N, 1, (int)((w.Kp + ks - 1) / ks), 1, true);
   if (bwd) {
     if (drop) w.dz = c.take(M * N * es);
     if (w.pad_n) w.dzp = c.take(M * w.Np * es);
-    w.dx = plan_gemm(dtype == HGK_BF16, M, K, 1, (N + ks - 1) / ks, 1, true);
-    w.dw = plan_gemm(dtype == HGK_BF16, N, K, 1, (int)((M + ks - 1) / ks), 1, true);
+    w.dx = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, K, 1, (N + ks - 1) / ks, 1, true);
+    w.dw = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, N, K, 1, (int)((M + ks - 1) / ks), 1, true);
     w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
   } else {
     w.slab = c.take(w.fwd.slab);

@@ -9,8 +9,9 @@
 // is one mfma_i32_16x16x64_i8, one mfma_f32_16x16x32_bf16 or four mfma_f32_16x16x4_f32.
 //
 // Operand layouts.
-//   ROW: k runs along memory. LDS tile [rows][128 B]; chunk c of row r sits at slot c ^ (r & 7),
-//        so the 8 rows that a b128 read takes at a time touch all banks once.
+//   ROW: k runs along memory. LDS tile [rows][128 B]; chunk c of row r sits at slot c ^ s(r), s(r) = r & 7
+//        on the M side and (r & 3) | (r >> 3 & 1) << 2 on the N side (below), so the 8 rows that a
+//        b128 read takes at a time touch all banks once.
 //   COL: k is the row index (weights of an input gradient, both operands of a weight gradient).
 //        LDS tile [KS rows][tile columns], read as transposed fragments
 //        (ds_read_b64_tr_b16; fp32: four b32 reads), slots swizzled by swz_col() below.
@@ -26,8 +27,12 @@
 // sides and a barrier each, the address units took twice as many requests and an
 // 8192 x 4096 x 8192 product ran at 1227 TFLOP/s (1651 with the DMAs left out).
 //
-// The matrix instruction's A operand is the N side and its B operand the M side: a lane then holds
-// 4 consecutive n of one row m.
+// The matrix instruction's A operand is the N side and its B operand the M side: a lane then holds 4
+// consecutive rows of the N side for one row m. The N side's rows are dealt to the fragments so that
+// a pair of them gives a lane 8 CONSECUTIVE columns of row m: row i of fragment 2 G + o is column
+// 32 G + 8 (i / 4) + 4 o + i % 4. 8 columns are a dropout group and 16 bytes of bf16; four lanes fill
+// 64 bytes of a row, and the epilogue works from registers. (Through LDS, in whole lines, the
+// epilogue of a [32768][2048] result from K = 256 took 13 us of 60.)
 //
 // Ends: rows / columns past the last are clamped to the last (their results are not stored); k
 // past the end reads a page of zeros on BOTH sides (a NaN times zero would not vanish).
@@ -219,16 +224,24 @@ __device__ __forceinline__ void drop8(const GemmArgs& a, int m, int n, float* f,
   for (int e = 0; e < 8; ++e) f[e] = (k >> e) & 1u ? f[e] * a.d.scale : 0.f;
 }
 
-// COL tiles of CH chunks a row. bf16: the 8 rows that a half-wave reads together (8 lg + 0 .. 3 of
-// two lane groups, 32 bytes of each) land on distinct 32-byte positions of the 256 that a read
-// covers; fp32: rows 4 lg + i of two lane groups, 64 bytes of each
-template <int DT, int CH>
+// COL tiles of CH chunks a row. A half-wave's transposed read takes 8 bytes of each of 8 rows (8 lg +
+// 0 .. 3 of two lane groups) and 4 places; its 32 pieces should cover a 256-byte window of the banks.
+//   M side: the 4 places are 32 bytes of a row: the rows differ in chunk bits 1 .. 3.
+//   N side: place q is column 8 q + 4 (o ^ q & 1), half a chunk, the halves alternating with q: two
+//   places share a half and differ in chunk bit 1, the rows in bits 0, 2 and 3. (Odd lane groups
+//   then hold their 8 columns' halves the other way round; the epilogue swaps them.)
+// Rows of 8 chunks: two fill the window, one bit less. fp32 reads single values: rows 4 lg + i of two
+// lane groups, 64 contiguous bytes of each (M) or four chunks two apart (N).
+template <int DT, int CH, bool NSIDE>
 __device__ __forceinline__ int swz_col(int p) {
-  if constexpr (DT == G_BF16) {
+  if constexpr (DT == G_BF16 && !NSIDE) {
     if constexpr (CH >= 16) return ((p & 3) | (((p >> 3) & 1) << 2)) << 1;
-    return (((p >> 1) & 1) | (((p >> 3) & 1) << 1)) << 1;  // 128-byte rows: two fill the window
+    return (((p >> 1) & 1) | (((p >> 3) & 1) << 1)) << 1;
+  } else if constexpr (DT == G_BF16) {
+    if constexpr (CH >= 16) return (p & 1) | (((p >> 1) & 1) << 2) | (((p >> 3) & 1) << 3);
+    return ((p >> 1) & 1) | (((p >> 3) & 1) << 2);
   }
-  return ((p >> 2) & 1) << 2;
+  return ((p >> 2) & 1) << (NSIDE ? 0 : 2);
 }
 
 // T: type of outputs, residual and dh
@@ -243,7 +256,7 @@ void gemm_kernel(GemmArgs a) {
   static_assert(BT % (8 * NW) == 0, "whole DMAs per wave");
   static_assert(DT != G_I8 || (LM == L_ROW && LN == L_ROW), "8-bit operands are ROW");
   constexpr int WTM = BM / WM, WTN = BN / WN, FM = WTM / 16, FN = WTN / 16;
-  static_assert(!DUAL || FN % 2 == 0, "gate and up halves");
+  static_assert(FN % (DUAL ? 4 : 2) == 0 && NW % 2 == 0, "pairs of N fragments, of gate and of up columns");
   __shared__ __attribute__((aligned(16))) char lds[5 * UB];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -280,18 +293,21 @@ void gemm_kernel(GemmArgs a) {
   if (DUAL) bu += a.n1 - a.n0;
   const long jumpm = (a.m1 - a.m0) - a.spseg * stepm, jumpn = (a.n1 - a.n0) - a.spseg * stepn;
   uint32_t om[D], on[D];
-  const int rchunk = (lane & 7) ^ ((lane >> 3) & 7);  // ROW: chunk of every DMA of this lane
+  // ROW: chunk of every DMA of this lane (a DMA's 8 rows start at a multiple of 8, N: at odd or even
+  // multiples with the wave)
+  const int rchm = (lane & 7) ^ ((lane >> 3) & 7), rchn = (lane & 7) ^ (((lane >> 3) & 3) | ((wave & 1) << 2));
   constexpr int CH = BT * es / 16;                    // COL: chunks per LDS row
   auto colrow = [&](int d) { return ((d * NW + wave) * 64 + lane) / CH; };
 #pragma unroll
   for (int d = 0; d < D; ++d) {
     const int row = (d * NW + wave) * 8 + (lane >> 3), p = colrow(d);
-    const int c = (((d * NW + wave) * 64 + lane) % CH) ^ swz_col<DT, CH>(p);
-    if (LM == L_ROW) om[d] = (uint32_t)min(row, a.M - 1 - m0) * (uint32_t)a.ldm + rchunk * 16;
-    else om[d] = (uint32_t)p * (uint32_t)a.ldm + min(m0 * es + c * 16, (a.M * es - 1) & ~15);
+    const int c = ((d * NW + wave) * 64 + lane) % CH;
+    const int cm = c ^ swz_col<DT, CH, false>(p), cn = c ^ swz_col<DT, CH, true>(p);
+    if (LM == L_ROW) om[d] = (uint32_t)min(row, a.M - 1 - m0) * (uint32_t)a.ldm + rchm * 16;
+    else om[d] = (uint32_t)p * (uint32_t)a.ldm + min(m0 * es + cm * 16, (a.M * es - 1) & ~15);
     // gated: the first half of the tile's rows are gate rows, the second up rows
-    if (LN == L_ROW) on[d] = (uint32_t)min(DUAL ? row % (BN / 2) : row, a.N - 1 - n0) * (uint32_t)a.ldn + rchunk * 16;
-    else on[d] = (uint32_t)p * (uint32_t)a.ldn + min(n0 * es + c * 16, (a.N * es - 1) & ~15);
+    if (LN == L_ROW) on[d] = (uint32_t)min(DUAL ? row % (BN / 2) : row, a.N - 1 - n0) * (uint32_t)a.ldn + rchn * 16;
+    else on[d] = (uint32_t)p * (uint32_t)a.ldn + min(n0 * es + cn * 16, (a.N * es - 1) & ~15);
   }
   static_assert(!DUAL || BN / 2 % (8 * NW) == 0, "DMA d of every wave brings gate rows or up rows");
   const bool tail_m = a.km % KS != 0, tail_n = a.kn % KS != 0;
@@ -304,7 +320,7 @@ void gemm_kernel(GemmArgs a) {
     const uint32_t off = NS ? on[d] : om[d];
     if constexpr (TAIL) {
       const int k = NS ? a.kn : a.km, kin = NS ? kinn : kinm;
-      const bool ok = (NS ? LN : LM) == L_ROW ? kin * 128 + rchunk * 16 < k * es : kin * KS + colrow(d) < k;
+      const bool ok = (NS ? LN : LM) == L_ROW ? kin * 128 + (NS ? rchn : rchm) * 16 < k * es : kin * KS + colrow(d) < k;
       dma16(ok ? base + off : g_zero_page, to);
     } else {
       dma16s(base, off, to);
@@ -342,29 +358,34 @@ void gemm_kernel(GemmArgs a) {
   };
 
   // ---- fragments of a step ----
-  const int x0 = lr * 128 + ((lg ^ (lr & 7)) << 4), x1 = lr * 128 + (((lg + 4) ^ (lr & 7)) << 4);
-  auto rown = [&](int f) {
-    return DUAL ? (f < FN / 2 ? wn * (WTN / 2) + f * 16 : BN / 2 + wn * (WTN / 2) + (f - FN / 2) * 16)
-                : wn * WTN + f * 16;
+  const int x0 = (lg ^ (lr & 7)) << 4, x1 = ((lg + 4) ^ (lr & 7)) << 4;  // ROW: s(row) is lr & 7 on both sides
+  const int rm = (wm * WTM + lr) * 128, rn = (8 * (lr >> 2) + (lr & 3)) * 128;
+  // first column of N fragment f's group of 32
+  auto coln = [&](int f) {
+    return DUAL ? (f < FN / 2 ? wn * (WTN / 2) + f / 2 * 32 : BN / 2 + wn * (WTN / 2) + (f - FN / 2) / 2 * 32)
+                : wn * WTN + f / 2 * 32;
   };
   typedef short s16x8 __attribute__((ext_vector_type(8)));
-  auto frag_col = [&](const char* t, int col, int h) __attribute__((always_inline)) -> i32x4 {
+  // 4 k values (fp32: one) of the fragment's 16 columns; N side: group `col`, half `o`
+  auto frag_col = [&](auto nside, const char* t, int col, int o, int h) __attribute__((always_inline)) -> i32x4 {
+    constexpr bool NS = decltype(nside)::value;
     constexpr int pitch = CH * 16;
     if constexpr (DT == G_BF16) {
-      const int p = 32 * h + 8 * lg + (lr >> 2), c = col + 4 * (lr & 3);
-      const char* q = t + p * pitch + (((c >> 3) ^ swz_col<DT, CH>(p)) << 4) + (c & 7) * 2;
-      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(q));
+      const int p = 32 * h + 8 * lg + (lr >> 2), q = lr & 3;
+      const int c = col + (NS ? 8 * q + 4 * (o ^ (q & 1)) : 4 * q);
+      const char* at = t + p * pitch + (((c >> 3) ^ swz_col<DT, CH, NS>(p)) << 4) + (c & 7) * 2;
+      const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at));
       const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-          (__attribute__((address_space(3))) s16x4*)(q + 4 * pitch));
+          (__attribute__((address_space(3))) s16x4*)(at + 4 * pitch));
       const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       return __builtin_bit_cast(i32x4, v);
     } else {
       i32x4 v;
-      const int c = col + lr;
+      const int c = col + (NS ? 8 * (lr >> 2) + 4 * o + (lr & 3) : lr);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int p = 16 * h + 4 * lg + i;
-        v[i] = *reinterpret_cast<const int*>(t + p * pitch + (((c >> 2) ^ swz_col<DT, CH>(p)) << 4) + (c & 3) * 4);
+        v[i] = *reinterpret_cast<const int*>(t + p * pitch + (((c >> 2) ^ swz_col<DT, CH, NS>(p)) << 4) + (c & 3) * 4);
       }
       return v;
     }
@@ -377,12 +398,12 @@ void gemm_kernel(GemmArgs a) {
     const char* tm = lds + um * UB;
     const char* tn = lds + un * UB;
     if (r < FN) {
-      f.n[r % FN] = LN == L_ROW ? *reinterpret_cast<const i32x4*>(tn + rown(r) * 128 + (h ? x1 : x0))
-                                : frag_col(tn, rown(r), h);
+      f.n[r % FN] = LN == L_ROW ? *reinterpret_cast<const i32x4*>(tn + (coln(r) + 4 * (r & 1)) * 128 + rn + (h ? x1 : x0))
+                                : frag_col(side_n, tn, coln(r), r & 1, h);
     } else {
       const int i = r - FN;
-      f.m[i % FM] = LM == L_ROW ? *reinterpret_cast<const i32x4*>(tm + (wm * WTM + i * 16) * 128 + (h ? x1 : x0))
-                                : frag_col(tm, wm * WTM + i * 16, h);
+      f.m[i % FM] = LM == L_ROW ? *reinterpret_cast<const i32x4*>(tm + i * 16 * 128 + rm + (h ? x1 : x0))
+                                : frag_col(side_m, tm, wm * WTM + i * 16, 0, h);
     }
   };
 
@@ -463,127 +484,119 @@ void gemm_kernel(GemmArgs a) {
     step(std::false_type(), P + 2 < np);
   }
 
-  // ---- epilogue. The sums go through LDS 16 rows of a wave at a time, so that a lane gets 8
-  // consecutive columns of one row (a dropout group, a 16-byte vector of bf16): rows are then
-  // read and written in whole lines. Stored from the fragment layout (8 bytes a lane, 16 rows an
-  // instruction) the 256-wide tile of a [32768][1024] result took 45 us a tile. ----
+  // ---- epilogue: a lane holds groups of 8 columns of row m, a pair of fragments each ----
   constexpr bool FAST = sizeof(T) == 2;
-  constexpr int CW = DUAL ? WTN / 2 : WTN;          // output columns of a wave
-  // (64 x 64 gated tiles: 16 columns a wave, half of its lanes have a row)
-  constexpr int GP = CW / 8, RP = 64 / GP < 16 ? 64 / GP : 16, NP = 16 / RP, PITCH = CW + 4;
-  static_assert(GP >= 2 && RP <= 32, "wave tile");
-  constexpr int PARTS = DUAL ? 2 : 1;
-  static_assert(NW * PARTS * 16 * PITCH * 4 <= 5 * UB, "scratch fits the slots");
-  __syncthreads();
-  float* scr = reinterpret_cast<float*>(lds) + wave * (PARTS * 16 * PITCH);
-  const int cg = lane % GP, r0 = (lane / GP) % RP;
-  const bool has_row = lane / GP < RP;
-  const int n = n0 + wn * CW + cg * 8, mw = m0 + wm * WTM + r0;
-  const bool in_n = n < (EPI == E_GATED_BWD ? a.npad : a.N);
+  constexpr int NG = DUAL ? FN / 4 : FN / 2;  // groups of a row
   const bool vec = a.vec != 0;
   const uint64_t off = EPI == E_OUT && a.drop ? drop_offset(a.d) : 0;
-  float cs0[8], cs1[8], bias[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    const int c = min(n + e, a.N - 1);
-    if constexpr (DT == G_I8) {
-      cs0[e] = a.col_scale[c];
-      cs1[e] = DUAL ? a.col_scale1[c] : 0.f;
-    }
-    if constexpr (EPI == E_OUT) bias[e] = a.bias ? a.bias[c] : 0.f;
-  }
-  // what a row brings along, loaded one fragment row ahead
+  const int nw = n0 + wn * (DUAL ? WTN / 2 : WTN) + 8 * lg, mw = m0 + wm * WTM + lr;
   const T* side = EPI == E_GATED_BWD ? (const T*)a.dh : EPI == E_OUT ? (const T*)a.res : nullptr;
-  Raw8<T> sv[NP];
-  float rs[NP];
-  auto ahead = [&](int i) __attribute__((always_inline)) {
+  const bool swapped = LN == L_COL && DT == G_BF16 && (lg & 1);
+  auto group = [&](int g, int i, float* f) __attribute__((always_inline)) {
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int m = min(mw + i * 16 + p * RP, a.M - 1);
-      if constexpr (DT == G_I8) rs[p] = a.row_scale[m];
-      if constexpr (EPI == E_GATED_BWD || EPI == E_OUT) {
-        if (side && vec && n < a.N) sv[p] = load_raw8<T>(side + (long)m * a.N + n);
-      }
+    for (int e = 0; e < 4; ++e) {
+      const auto x = acc[2 * g][i][e], y = acc[2 * g + 1][i][e];
+      f[e] = (float)(swapped ? y : x);
+      f[4 + e] = (float)(swapped ? x : y);
     }
   };
-  ahead(0);
+  // two groups at a time, one line of bf16: its halves are stored one after the other
+  constexpr int GS = NG > 1 ? 2 : 1;
 #pragma unroll
-  for (int i = 0; i < FM; ++i) {
+  for (int g0 = 0; g0 < NG; g0 += GS) {
+    float cs0[GS][8], cs1[GS][8], bias[GS][8];
 #pragma unroll
-    for (int j = 0; j < FN; ++j) {
-      const int part = DUAL ? j / (FN / 2) : 0, jc = DUAL ? j % (FN / 2) : j;
-      *reinterpret_cast<typename GT<DT>::acc*>(scr + (part * 16 + lr) * PITCH + jc * 16 + lg * 4) = acc[j][i];
-    }
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // this wave's own rows: no barrier
-    float f[NP][8], u[NP][8], q[NP][8];
+    for (int k = 0; k < GS; ++k)
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const auto v = *reinterpret_cast<const typename GT<DT>::acc*>(scr + (r0 + p * RP) * PITCH + cg * 8 + 4 * h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f[p][4 * h + e] = (float)v[e];
-        if constexpr (DUAL) {
-          const auto w = *reinterpret_cast<const typename GT<DT>::acc*>(scr + (16 + r0 + p * RP) * PITCH + cg * 8 + 4 * h);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) u[p][4 * h + e] = (float)w[e];
+      for (int e = 0; e < 8; ++e) {
+        const int c = min(nw + 32 * (g0 + k) + e, a.N - 1);
+        if constexpr (DT == G_I8) {
+          cs0[k][e] = a.col_scale[c];
+          cs1[k][e] = DUAL ? a.col_scale1[c] : 0.f;
         }
+        if constexpr (EPI == E_OUT) bias[k][e] = a.bias ? a.bias[c] : 0.f;
       }
-      if constexpr (DT == G_I8) {
+    // what the rows bring along
+    Raw8<T> sv[FM][GS];
+    float rs[FM];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          f[p][e] = f[p][e] * rs[p] * cs0[e];
-          if constexpr (DUAL) u[p][e] = u[p][e] * rs[p] * cs1[e];
-        }
-      }
+    for (int i = 0; i < FM; ++i) {
+      const int m = min(mw + i * 16, a.M - 1);
+      if constexpr (DT == G_I8) rs[i] = a.row_scale[m];
       if constexpr (EPI == E_GATED_BWD || EPI == E_OUT) {
-        if (side) {
-          if (vec) unpack_raw8<T>(sv[p], q[p]);
-          else if (n < a.N) load8<T>(side + (long)min(mw + i * 16 + p * RP, a.M - 1) * a.N, n, a.N, false, q[p]);
+#pragma unroll
+        for (int k = 0; k < GS; ++k) {
+          const int n = nw + 32 * (g0 + k);
+          if (side && vec && n < a.N) sv[i][k] = load_raw8<T>(side + (long)m * a.N + n);
         }
       }
     }
-    if (i + 1 < FM) ahead(i + 1);
-    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read before the next rows overwrite
 #pragma unroll
-    for (int p = 0; p < NP; ++p) {
-      const int m = mw + i * 16 + p * RP;
-      if (m >= a.M || !in_n || !has_row) continue;
-      if constexpr (EPI == E_GATED) {
-        with_act(a.act, [&](auto A) __attribute__((always_inline)) {
+    for (int i = 0; i < FM; ++i) {
+      const int m = mw + i * 16;
+      if (m >= a.M) continue;
+      float dg[GS][8], du[GS][8];  // E_GATED_BWD
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[p][e] = act_f<decltype(A)::value, FAST>(f[p][e]) * u[p][e];
-        });
-        store8<T>((T*)a.out + (long)m * a.N, n, a.N, vec, f[p]);
-      } else if constexpr (EPI == E_GATED_BWD) {
-        float dg[8], du[8];
-        with_act(a.act, [&](auto A) __attribute__((always_inline)) {
+      for (int k = 0; k < GS; ++k) {
+        const int n = nw + 32 * (g0 + k);
+        if (n >= (EPI == E_GATED_BWD ? a.npad : a.N)) continue;
+        float f[8], u[8], q[8];
+        group(g0 + k, i, f);
+        if constexpr (DUAL) group(NG + g0 + k, i, u);
+        if constexpr (DT == G_I8) {
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
-            float av, sl;
-            act_slope<decltype(A)::value, FAST>(f[p][e], av, sl);
-            dg[e] = q[p][e] * u[p][e] * sl;
-            du[e] = q[p][e] * av;
+            f[e] = f[e] * rs[i] * cs0[k][e];
+            if constexpr (DUAL) u[e] = u[e] * rs[i] * cs1[k][e];
           }
-        });
-        if (!vec) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            if (n + e >= a.N) dg[e] = du[e] = 0.f;
         }
-        store8<T>((T*)a.out + (long)m * a.npad, n, a.npad, true, dg);
-        store8<T>((T*)a.out1 + (long)m * a.npad, n, a.npad, true, du);
-      } else if constexpr (EPI == E_SLAB) {
-        store8<float>(a.slab + (((long)split * a.batch + bat) * a.M + m) * a.N, n, a.N, vec, f[p]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) f[p][e] = fmaf(f[p][e], a.alpha, bias[e]);
-        if (a.drop) drop8(a, m, n, f[p], off);
-        if (side) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) f[p][e] += q[p][e];
+        if constexpr (EPI == E_GATED_BWD || EPI == E_OUT) {
+          if (side) {
+            if (vec) unpack_raw8<T>(sv[i][k], q);
+            else load8<T>(side + (long)m * a.N, n, a.N, false, q);
+          }
         }
-        store8<T>((T*)(bat ? a.out1 : a.out) + (long)m * a.N, n, a.N, vec, f[p]);
+        if constexpr (EPI == E_GATED) {
+          with_act(a.act, [&](auto A) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] = act_f<decltype(A)::value, FAST>(f[e]) * u[e];
+          });
+          store8<T>((T*)a.out + (long)m * a.N, n, a.N, vec, f);
+        } else if constexpr (EPI == E_GATED_BWD) {
+          with_act(a.act, [&](auto A) __attribute__((always_inline)) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              float av, sl;
+              act_slope<decltype(A)::value, FAST>(f[e], av, sl);
+              dg[k][e] = q[e] * u[e] * sl;
+              du[k][e] = q[e] * av;
+            }
+          });
+          if (!vec) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e >= a.N) dg[k][e] = du[k][e] = 0.f;
+          }
+        } else if constexpr (EPI == E_SLAB) {
+          store8<float>(a.slab + (((long)split * a.batch + bat) * a.M + m) * a.N, n, a.N, vec, f);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] = fmaf(f[e], a.alpha, bias[k][e]);
+          if (a.drop) drop8(a, m, n, f, off);
+          if (side) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) f[e] += q[e];
+          }
+          store8<T>((T*)(bat ? a.out1 : a.out) + (long)m * a.N, n, a.N, vec, f);
+        }
+      }
+      if constexpr (EPI == E_GATED_BWD) {
+#pragma unroll
+        for (int k = 0; k < 2 * GS; ++k) {
+          const int n = nw + 32 * (g0 + k % GS);
+          if (n < a.npad)
+            store8<T>((T*)(k < GS ? a.out : a.out1) + (long)m * a.npad, n, a.npad, true, k < GS ? dg[k % GS] : du[k % GS]);
+        }
       }
     }
   }
@@ -744,22 +757,43 @@ struct GemmPlan {
   int tiles_m, tiles_n, splits;
   long slab;  // bytes
 };
-// per: a gated tile holds 2 x (columns / 2) columns. wide: the type has tiles of 256
-static inline GemmPlan plan_gemm(bool wide, long M, long N, int per, int steps, int batch, bool can_split) {
-  GemmPlan p;
-  auto tiles = [&](int b) { return ((M + b - 1) / b) * ((N + b / per - 1) / (b / per)) * batch; };
-  const int asked = (int)route(HGK_ROUTE_FFN_TILE);
-  if (asked == 64 || asked == 128 || (wide && asked == 256)) p.tile = asked;
-  else if (wide && tiles(256) >= 256) p.tile = 256;
-  else if (tiles(128) >= 256) p.tile = 128;
-  else p.tile = 64;
-  p.tiles_m = (int)((M + p.tile - 1) / p.tile);
-  p.tiles_n = (int)((N + p.tile / per - 1) / (p.tile / per));
-  const long n = tiles(p.tile), fill = p.tile == 256 ? 256 : p.tile == 64 ? 1024 : 512;
-  p.splits = 1;
-  if (can_split && n * 2 <= fill) p.splits = (int)std::max(1l, std::min<long>(fill / n, steps / 4));
-  p.slab = p.splits > 1 ? (long)p.splits * batch * M * N * 4 : 0;
-  return p;
+// per: a gated tile holds 2 x (columns / 2) columns. dt: GemmType. steps: K-steps of 128 bytes.
+//
+// The tile and the split are those of the least estimated time. A K-step of a 256-wide tile takes
+// 1.5 us of a CU in bf16 (1467 TFLOP/s over the chip at 8192 x 4096 x 8192); per unit of work a
+// 128-wide tile takes 1.3 times that (1147), a 64-wide one 2 to 3 times (502 .. 704): its waves read
+// twice to four times the fragments per product. fp32's matrix instructions are 16 times slower and
+// hide all of that. A CU that holds too few waves waits instead: 0.5 us a step at least. Against the
+// tile stand the rounds: tiles are dealt to 256 CUs whole. Splitting k costs the partial sums' way to
+// memory and back (4.5 TB/s) and a second launch (5 us).
+static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int batch, bool can_split) {
+  GemmPlan best;
+  double least = 1e30;
+  const long asked = route(HGK_ROUTE_FFN_TILE);
+  for (int b = dt == G_F32 ? 128 : 256; b >= 64; b /= 2) {
+    if ((asked == 64 || asked == 128 || (asked == 256 && dt != G_F32)) && asked != b) continue;
+    GemmPlan p;
+    p.tile = b;
+    p.tiles_m = (int)((M + b - 1) / b);
+    p.tiles_n = (int)((N + b / per - 1) / (b / per));
+    const long n = (long)p.tiles_m * p.tiles_n * batch;
+    const double slow = dt == G_F32 ? (b == 128 ? 1.0 : 1.1) : b == 256 ? 1.0 : b == 128 ? 1.3 : 2.4;
+    const double step = (dt == G_F32 ? 12.0 : dt == G_I8 ? 1.1 : 1.5) * b * b / 65536 * slow;
+    const long slots = 256l * (b == 256 ? 1 : b == 128 ? 2 : 4);
+    for (int split = 1; split <= 64; split *= 2) {
+      if (split > 1 && (!can_split || n * split > slots || steps / split < 4)) break;
+      const double rounds = (double)((n * split + 255) / 256), each = (double)((steps + split - 1) / split);
+      double t = std::max(rounds * step, 0.5) * each;
+      if (split > 1) t += 5 + 8.0 * split * batch * M * N / 4.5e6;
+      if (t < least) {
+        least = t;
+        best = p;
+        best.splits = split;
+      }
+    }
+  }
+  best.slab = best.splits > 1 ? (long)best.splits * batch * M * N * 4 : 0;
+  return best;
 }
 
 // what a launch needs before its kernel is chosen
@@ -783,7 +817,7 @@ static void run_tiles(hipStream_t st, GemmArgs& a, const GemmPlan& p) {
     }
   }
   if (p.tile == 128) hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 2, 2, EPI>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 64, 2, 2, EPI>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 64, 2, 1, EPI>), grid, dim3(128), 0, st, a);
 }
 
 }  // namespace hgk

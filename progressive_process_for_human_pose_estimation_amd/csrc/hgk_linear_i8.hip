@@ -10,14 +10,15 @@ namespace hgk {
 
 static constexpr int kI8MaxK = 1 << 17;
 
-// One wave a row. NCH > 0: the row stays in registers (NCH 16-B chunks a lane), read once;
-// NCH == 0: two passes, the second from the cache. VEC false: rows not on 16-B borders.
-template <typename T, int NCH, bool VEC>
+// L lanes a row (64 / L rows a wave, so that short rows fill the wave), NCH 16-byte chunks a lane held in
+// registers: the row is read once. NCH == 0: two passes, the second from the cache. VEC false: rows not on
+// 16-byte borders, single elements. Bound by memory: 2 bytes in and 1 out an element of bf16.
+template <typename T, int L, int NCH, bool VEC>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
                                                          float* __restrict__ s, long rows, int K, int Kp) {
   constexpr int V = VEC ? Vec16<T>::N : 1;
-  const int lane = threadIdx.x & 63;
-  const long r = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  const int lane = threadIdx.x % L;
+  const long r = ((long)blockIdx.x * 256 + threadIdx.x) / L;
   if (r >= rows) return;
   const T* row = x + r * K;
   int8_t* qrow = q + r * Kp;
@@ -39,30 +40,44 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
   if constexpr (NCH > 0) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
-      const int c = lane + i * 64;
+      const int c = lane + i * L;
       if (c < nc) load(c, f[i]);
       else
         for (int e = 0; e < V; ++e) f[i][e] = 0.f;
-      scan(f[i]);
     }
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) scan(f[i]);
   } else {
-    for (int c = lane; c < nc; c += 64) {
+    for (int c = lane; c < nc; c += L) {
       load(c, f[0]);
       scan(f[0]);
     }
   }
+  int any = odd;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor(m, o, 64));
-  odd = __any(odd);
+  for (int o = L / 2; o > 0; o >>= 1) {
+    m = fmaxf(m, __shfl_xor(m, o, L));
+    any |= __shfl_xor(any, o, L);
+  }
   const float sc = m / 127.f;
-  const bool none = odd || sc == 0.f;
-  if (lane == 0) s[r] = odd ? __int_as_float(0x7fc00000) : sc;
+  const bool none = any || sc == 0.f;
+  if (lane == 0) s[r] = any ? __int_as_float(0x7fc00000) : sc;
+  // v / sc correctly rounded, the quotient of two fp32 values that the definition rounds to a whole step: from
+  // the correctly rounded reciprocal, one fused step makes the product faithful (within a unit in the last
+  // place) and the next one exact (Markstein, 1990). Where sc or its reciprocal leaves the normal numbers: the
+  // division itself.
+  const float inv = 1.f / sc;
+  const bool plain = sc >= 1e-30f && sc <= 1e30f;
   auto put = [&](int c, const float* v) __attribute__((always_inline)) {
     int8_t b[V];
 #pragma unroll
-    for (int e = 0; e < V; ++e)  // the quotient of two fp32 values, not a product with 1 / s: the
-      // same whole step as the definition's in every case
-      b[e] = none ? 0 : (int8_t)(int)fminf(fmaxf(rintf(v[e] / sc), -127.f), 127.f);
+    for (int e = 0; e < V; ++e) {
+      float t = v[e] * inv;
+      t = fmaf(fmaf(-t, sc, v[e]), inv, t);
+      t = fmaf(fmaf(-t, sc, v[e]), inv, t);
+      if (!plain) t = v[e] / sc;
+      b[e] = none ? 0 : (int8_t)(int)fminf(fmaxf(rintf(t), -127.f), 127.f);
+    }
     if constexpr (VEC && V == 8) {
       uint2 w;
       memcpy(&w, b, 8);
@@ -78,33 +93,42 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
   if constexpr (NCH > 0) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i)
-      if (lane + i * 64 < nc) put(lane + i * 64, f[i]);
+      if (lane + i * L < nc) put(lane + i * L, f[i]);
   } else {
-    for (int c = lane; c < nc; c += 64) {
+    for (int c = lane; c < nc; c += L) {
       load(c, f[0]);
       put(c, f[0]);
     }
   }
-  for (int c = K + lane; c < Kp; c += 64) qrow[c] = 0;
+  for (int c = K + lane; c < Kp; c += L) qrow[c] = 0;
+}
+
+template <typename T, bool VEC>
+static void launch_quant_as(hipStream_t st, const T* x, int8_t* q, float* s, long rows, int K, int Kp) {
+  const int nc = VEC ? K / Vec16<T>::N : K;
+  const dim3 blk(256);
+  auto grid = [&](int L) { return dim3((unsigned)((rows * L + 255) / 256)); };
+#define HGK_QUANT(L, NCH) \
+  hipLaunchKernelGGL((quant_rows_kernel<T, L, NCH, VEC>), grid(L), blk, 0, st, x, q, s, rows, K, Kp)
+  if (nc <= 8) HGK_QUANT(8, 1);
+  else if (nc <= 16) HGK_QUANT(16, 1);
+  else if (nc <= 32) HGK_QUANT(16, 2);
+  else if (nc <= 64) HGK_QUANT(32, 2);
+  else if (nc <= 128) HGK_QUANT(64, 2);
+  else if (nc <= 256) HGK_QUANT(64, 4);
+  else if (nc <= 512) HGK_QUANT(64, 8);
+  else HGK_QUANT(64, 0);
+#undef HGK_QUANT
 }
 
 template <typename T>
 static void launch_quant(hipStream_t st, const void* x, int8_t* q, float* s, long rows, int K, int Kp) {
   constexpr int V = Vec16<T>::N;
-  const dim3 grid((unsigned)((rows + 3) / 4)), blk(256);
-  const T* p = (const T*)x;
-  // the quantised rows are written in words of V: q and its pitch have to allow them
-  if (K % V == 0 && Kp % V == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)q & 7) == 0) {
-    const int per = (K / V + 63) / 64;
-    if (per <= 1) hipLaunchKernelGGL((quant_rows_kernel<T, 1, true>), grid, blk, 0, st, p, q, s, rows, K, Kp);
-    else if (per <= 2) hipLaunchKernelGGL((quant_rows_kernel<T, 2, true>), grid, blk, 0, st, p, q, s, rows, K, Kp);
-    else if (per <= 8) hipLaunchKernelGGL((quant_rows_kernel<T, 8, true>), grid, blk, 0, st, p, q, s, rows, K, Kp);
-    else hipLaunchKernelGGL((quant_rows_kernel<T, 0, true>), grid, blk, 0, st, p, q, s, rows, K, Kp);
-  } else {
-    const int per = (K + 63) / 64;
-    if (per <= 16) hipLaunchKernelGGL((quant_rows_kernel<T, 16, false>), grid, blk, 0, st, p, q, s, rows, K, Kp);
-    else hipLaunchKernelGGL((quant_rows_kernel<T, 0, false>), grid, blk, 0, st, p, q, s, rows, K, Kp);
-  }
+  // quantised rows are written in words of V: q and its pitch have to allow them
+  if (K % V == 0 && Kp % V == 0 && ((uintptr_t)x & 15) == 0 && ((uintptr_t)q & 7) == 0)
+    launch_quant_as<T, true>(st, (const T*)x, q, s, rows, K, Kp);
+  else
+    launch_quant_as<T, false>(st, (const T*)x, q, s, rows, K, Kp);
 }
 
 struct I8Ws {
@@ -166,7 +190,7 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
     else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<G_I8, T, 2, GATED>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((skinny_kernel<G_I8, T, 4, GATED>), grid, dim3(512), 0, st, a);
   } else {
-    run_tiles<G_I8, T, L_ROW, L_ROW, EPI>(st, a, plan_gemm(true, M, N, per, a.spseg, 1, false));
+    run_tiles<G_I8, T, L_ROW, L_ROW, EPI>(st, a, plan_gemm(G_I8, M, N, per, a.spseg, 1, false));
   }
   HGK_LAUNCH_CHECK();
   return HGK_OK;
