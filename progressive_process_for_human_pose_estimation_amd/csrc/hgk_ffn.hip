@@ -108,9 +108,11 @@ static void gated_operands(hipStream_t st, GemmArgs& a, const GatedWs& w, char* 
                            const void* wg, const void* wu, long M, int C, int F) {
   typedef typename TypeOf<T>::raw raw;
   if (w.pad) {
-    launch_pad<raw>(st, x, ws + w.x, M, C, w.Cp);
-    launch_pad<raw>(st, wg, ws + w.wg, F, C, w.Cp);
-    launch_pad<raw>(st, wu, ws + w.wu, F, C, w.Cp);
+    Pads p;
+    p.add(x, ws + w.x, M, C, w.Cp, sizeof(T));
+    p.add(wg, ws + w.wg, F, C, w.Cp, sizeof(T));
+    p.add(wu, ws + w.wu, F, C, w.Cp, sizeof(T));
+    p.launch<raw>(st);
   }
   a.m0 = a.m1 = w.pad ? ws + w.x : (const char*)x;
   a.n0 = w.pad ? ws + w.wg : (const char*)wg;
@@ -201,7 +203,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
 
 // ---- linear with dropout and residual ----
 struct LinearWs {
-  long x, w, dz, dzp, slab, total;
+  long x, w, dz, slab, total;
   int Kp, Np;
   bool pad_k, pad_n;
   GemmPlan fwd, dx, dw;
@@ -214,15 +216,14 @@ static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) 
   w.pad_k = w.Kp != K;
   w.pad_n = w.Np != N;
   Carve c;
-  w.x = w.w = w.dz = w.dzp = w.slab = 0;
+  w.x = w.w = w.dz = w.slab = 0;
   if (w.pad_k) {
     w.x = c.take(M * w.Kp * es);
     w.w = c.take((long)N * w.Kp * es);
   }
   w.fwd = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, N, 1, (int)((w.Kp + ks - 1) / ks), 1, true);
   if (bwd) {
-    if (drop) w.dz = c.take(M * N * es);
-    if (w.pad_n) w.dzp = c.take(M * w.Np * es);
+    if (drop || w.pad_n) w.dz = c.take(M * w.Np * es);
     w.dx = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, K, 1, (N + ks - 1) / ks, 1, true);
     w.dw = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, N, K, 1, (int)((M + ks - 1) / ks), 1, true);
     w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
@@ -240,8 +241,10 @@ static int linear_fwd(hipStream_t st, const void* x, const void* wt, const void*
   typedef typename TypeOf<T>::raw raw;
   const LinearWs w = linear_ws(dtype, M, K, N, d.thr != 0, false);
   if (w.pad_k) {
-    launch_pad<raw>(st, x, ws + w.x, M, K, w.Kp);
-    launch_pad<raw>(st, wt, ws + w.w, N, K, w.Kp);
+    Pads p;
+    p.add(x, ws + w.x, M, K, w.Kp, sizeof(T));
+    p.add(wt, ws + w.w, N, K, w.Kp, sizeof(T));
+    p.launch<raw>(st);
   }
   GemmArgs a = gemm_args();
   a.m0 = w.pad_k ? ws + w.x : (const char*)x;
@@ -272,22 +275,22 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
   typedef typename TypeOf<T>::raw raw;
   const bool drop = d.thr != 0;
   const LinearWs w = linear_ws(dtype, M, K, N, drop, true);
-  const char* dz = (const char*)dy;
-  if (drop) {
+  const char *dz = (const char*)dy, *xp = (const char*)x, *wp = (const char*)wt;
+  Pads p;
+  if (w.pad_n) {
+    p.add(dy, ws + w.dz, M, N, w.Np, es, drop ? &d : nullptr);
+    dz = ws + w.dz;
+  } else if (drop) {
     if (int rc = dropout_mask(st, dtype, dy, ws + w.dz, M, N, d)) return rc;
     dz = ws + w.dz;
   }
-  if (w.pad_n) {
-    launch_pad<raw>(st, dz, ws + w.dzp, M, N, w.Np);
-    dz = ws + w.dzp;
-  }
-  const char *xp = (const char*)x, *wp = (const char*)wt;
   if (w.pad_k) {
-    if (dw) launch_pad<raw>(st, x, ws + w.x, M, K, w.Kp);
-    if (dx) launch_pad<raw>(st, wt, ws + w.w, N, K, w.Kp);
+    if (dw) p.add(x, ws + w.x, M, K, w.Kp, es);
+    if (dx) p.add(wt, ws + w.w, N, K, w.Kp, es);
     xp = ws + w.x;
     wp = ws + w.w;
   }
+  p.launch<raw>(st);
   HGK_LAUNCH_CHECK();
   const float alpha = drop ? d.scale : 1.f;
   if (dx) {

@@ -719,20 +719,57 @@ __global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
   store8<T>((T*)(bat ? a.out1 : a.out) + (long)m * a.N, n, a.N, vec, f);
 }
 
-// rows of K elements -> rows of Kp (16-byte multiple), the rest zero. E: unsigned type of es bytes
+// Up to three tensors at once: rows of K elements -> rows of Kp (whole 16-byte chunks), the rest zero; the
+// one with `drop` set also through a dropout mask (unscaled). E: unsigned type of an element. Rows are
+// read in words of `unit` bytes, the largest that both their pitch and their start allow.
+struct PadJob {
+  const char* src;
+  char* dst;
+  long rows, first;  // first: chunks of the jobs before
+  int K, Kp, unit, drop;
+};
+struct PadArgs {
+  PadJob j[3];
+  int n;
+  long chunks;
+  DropArgs d;
+};
 template <typename E>
-__global__ __launch_bounds__(256) void pad_rows_kernel(const E* __restrict__ src, E* __restrict__ dst,
-                                                       long rows, int K, int Kp) {
+__global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
   constexpr int V = 16 / sizeof(E);
   const long t = (long)blockIdx.x * 256 + threadIdx.x;
-  const int cp = Kp / V;
-  const long r = t / cp;
-  if (r >= rows) return;
-  const int c0 = (int)(t - r * cp) * V;
-  E v[V];
+  if (t >= a.chunks) return;
+  const int k = a.n > 2 && t >= a.j[2].first ? 2 : a.n > 1 && t >= a.j[1].first ? 1 : 0;
+  const PadJob& j = a.j[k];
+  const uint32_t cp = j.Kp / V;
+  const uint32_t l = (uint32_t)(t - j.first);  // host: a job's chunks are less than 2^32
+  const uint32_t r = l / cp;
+  const int c0 = (int)(l - r * cp) * V;
+  const char* src = j.src + ((long)r * j.K + c0) * (long)sizeof(E);
+  const int left = (j.K - c0) * (int)sizeof(E);  // bytes of the row from here on
+  uint4 v = make_uint4(0, 0, 0, 0);
+  auto take = [&](auto word) __attribute__((always_inline)) {
+    typedef decltype(word) W;
+    W w[16 / sizeof(W)];
 #pragma unroll
-  for (int e = 0; e < V; ++e) v[e] = c0 + e < K ? src[r * K + c0 + e] : E(0);
-  *reinterpret_cast<uint4*>(dst + r * Kp + c0) = *reinterpret_cast<const uint4*>(v);
+    for (int e = 0; e < (int)(16 / sizeof(W)); ++e)
+      w[e] = (e + 1) * (int)sizeof(W) <= left ? reinterpret_cast<const W*>(src)[e] : W(0);
+    memcpy(&v, w, 16);
+  };
+  if (j.unit >= 8) take(uint64_t());
+  else if (j.unit == 4) take(uint32_t());
+  else if (sizeof(E) == 2 || j.unit == 2) take(uint16_t());
+  else take(uint8_t());
+  if (j.drop) {
+    E e[V];
+    memcpy(e, &v, 16);
+    const uint32_t m = drop_mask8((uint64_t)r * ((j.K + 7) >> 3) + (c0 >> 3), drop_offset(a.d), a.d.seed, a.d.thr) >> (c0 & 7);
+#pragma unroll
+    for (int i = 0; i < V; ++i)
+      if (!((m >> i) & 1u)) e[i] = 0;
+    memcpy(&v, e, 16);
+  }
+  reinterpret_cast<uint4*>(j.dst)[l] = v;
 }
 static __global__ __launch_bounds__(256) void zero_kernel(uint32_t* p, long words) {
   for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < words; i += (long)gridDim.x * 256) p[i] = 0;
@@ -744,12 +781,34 @@ int dropout_mask(hipStream_t st, int dtype, const void* dy, void* dz, long rows,
 
 static inline long up_to(long n, long q) { return (n + q - 1) / q * q; }
 
-template <typename E>
-static inline void launch_pad(hipStream_t st, const void* src, void* dst, long rows, int K, int Kp) {
-  const long n = rows * (Kp * (long)sizeof(E) / 16);
-  hipLaunchKernelGGL((pad_rows_kernel<E>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st,
-                     (const E*)src, (E*)dst, rows, K, Kp);
-}
+// collects the rows to pad, then one launch
+struct Pads {
+  PadArgs a;
+  Pads() {
+    a.n = 0;
+    a.chunks = 0;
+    a.d = DropArgs();
+  }
+  void add(const void* src, void* dst, long rows, int K, int Kp, int es, const DropArgs* drop = nullptr) {
+    PadJob& j = a.j[a.n++];
+    j.src = (const char*)src;
+    j.dst = (char*)dst;
+    j.rows = rows;
+    j.K = K;
+    j.Kp = Kp;
+    j.first = a.chunks;
+    const long bits = (long)K * es | (long)(uintptr_t)src;
+    j.unit = bits % 8 == 0 ? 8 : bits % 4 == 0 ? 4 : bits % 2 == 0 ? 2 : 1;
+    j.drop = drop != nullptr;
+    if (drop) a.d = *drop;
+    a.chunks += rows * ((long)Kp * es / 16);
+  }
+  template <typename E>
+  void launch(hipStream_t st) {
+    if (a.n)
+      hipLaunchKernelGGL((pad_rows_kernel<E>), dim3((unsigned)((a.chunks + 255) / 256)), dim3(256), 0, st, a);
+  }
+};
 
 // ---- tile size and split of a product ----
 struct GemmPlan {
@@ -763,7 +822,8 @@ struct GemmPlan {
 // 1.5 us of a CU in bf16 (1467 TFLOP/s over the chip at 8192 x 4096 x 8192); per unit of work a
 // 128-wide tile takes 1.3 times that (1147), a 64-wide one 2 to 3 times (502 .. 704): its waves read
 // twice to four times the fragments per product. fp32's matrix instructions are 16 times slower and
-// hide all of that. A CU that holds too few waves waits instead: 0.5 us a step at least. Against the
+// hide all of that. A CU with one or two workgroups waits for memory instead: 1.2 us
+// a step at least. Against the
 // tile stand the rounds: tiles are dealt to 256 CUs whole. Splitting k costs the partial sums' way to
 // memory and back (4.5 TB/s) and a second launch (5 us).
 static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int batch, bool can_split) {
@@ -783,7 +843,7 @@ static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int
     for (int split = 1; split <= 64; split *= 2) {
       if (split > 1 && (!can_split || n * split > slots || steps / split < 4)) break;
       const double rounds = (double)((n * split + 255) / 256), each = (double)((steps + split - 1) / split);
-      double t = std::max(rounds * step, 0.5) * each;
+      double t = std::max(rounds * step, 1.2) * each;
       if (split > 1) t += 5 + 8.0 * split * batch * M * N / 4.5e6;
       if (t < least) {
         least = t;
@@ -817,7 +877,7 @@ static void run_tiles(hipStream_t st, GemmArgs& a, const GemmPlan& p) {
     }
   }
   if (p.tile == 128) hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 2, 2, EPI>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 64, 2, 1, EPI>), grid, dim3(128), 0, st, a);
+  else hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 64, 4, 1, EPI>), grid, dim3(256), 0, st, a);
 }
 
 }  // namespace hgk

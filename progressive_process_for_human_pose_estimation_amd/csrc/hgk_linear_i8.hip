@@ -28,14 +28,11 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
     else v[0] = to_f(row[c]);
   };
   const int nc = K / V;  // VEC: K % V == 0
-  float m = 0.f;
-  bool odd = false;  // an infinity or a NaN
+  // magnitudes compare like their bits, infinities and NaN above all numbers
+  uint32_t m = 0;
   auto scan = [&](const float* v) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      odd |= !(fabsf(v[e]) <= 3.402823466e38f);
-      m = fmaxf(m, fabsf(v[e]));
-    }
+    for (int e = 0; e < V; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
   };
   if constexpr (NCH > 0) {
 #pragma unroll
@@ -53,41 +50,42 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
       scan(f[0]);
     }
   }
-  int any = odd;
 #pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    m = fmaxf(m, __shfl_xor(m, o, L));
-    any |= __shfl_xor(any, o, L);
-  }
-  const float sc = m / 127.f;
-  const bool none = any || sc == 0.f;
-  if (lane == 0) s[r] = any ? __int_as_float(0x7fc00000) : sc;
+  for (int o = L / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, L));
+  const bool odd = m >= 0x7f800000u;  // an infinity or a NaN
+  const float sc = __uint_as_float(m) / 127.f;
+  const bool none = odd || sc == 0.f;
+  if (lane == 0) s[r] = odd ? __int_as_float(0x7fc00000) : sc;
   // v / sc correctly rounded, the quotient of two fp32 values that the definition rounds to a whole step: from
   // the correctly rounded reciprocal, one fused step makes the product faithful (within a unit in the last
   // place) and the next one exact (Markstein, 1990). Where sc or its reciprocal leaves the normal numbers: the
-  // division itself.
+  // division itself. Adding 1.5 2^23 rounds to a whole number, whose low byte is the result.
   const float inv = 1.f / sc;
   const bool plain = sc >= 1e-30f && sc <= 1e30f;
   auto put = [&](int c, const float* v) __attribute__((always_inline)) {
-    int8_t b[V];
+    uint32_t b[V];
+    if (plain) {
 #pragma unroll
-    for (int e = 0; e < V; ++e) {
-      float t = v[e] * inv;
-      t = fmaf(fmaf(-t, sc, v[e]), inv, t);
-      t = fmaf(fmaf(-t, sc, v[e]), inv, t);
-      if (!plain) t = v[e] / sc;
-      b[e] = none ? 0 : (int8_t)(int)fminf(fmaxf(rintf(t), -127.f), 127.f);
-    }
-    if constexpr (VEC && V == 8) {
-      uint2 w;
-      memcpy(&w, b, 8);
-      *reinterpret_cast<uint2*>(qrow + c * 8) = w;
-    } else if constexpr (VEC) {
-      uint32_t w;
-      memcpy(&w, b, 4);
-      *reinterpret_cast<uint32_t*>(qrow + c * 4) = w;
+      for (int e = 0; e < V; ++e) {
+        float t = v[e] * inv;
+        t = fmaf(fmaf(-t, sc, v[e]), inv, t);
+        t = fmaf(fmaf(-t, sc, v[e]), inv, t);
+        b[e] = __float_as_uint(t + 12582912.f);
+      }
     } else {
-      qrow[c] = b[0];
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        b[e] = none ? 0 : (uint32_t)(int)fminf(fmaxf(rintf(v[e] / sc), -127.f), 127.f);
+    }
+    if constexpr (VEC) {
+      uint32_t w[V / 4];
+#pragma unroll
+      for (int e = 0; e < V; e += 4)
+        w[e / 4] = (b[e] & 0xffu) | (b[e + 1] & 0xffu) << 8 | (b[e + 2] & 0xffu) << 16 | b[e + 3] << 24;
+      if constexpr (V == 8) *reinterpret_cast<uint2*>(qrow + c * 8) = make_uint2(w[0], w[1]);
+      else *reinterpret_cast<uint32_t*>(qrow + c * 4) = w[0];
+    } else {
+      qrow[c] = (int8_t)b[0];
     }
   };
   if constexpr (NCH > 0) {
@@ -162,8 +160,10 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
   launch_quant<T>(st, x, (int8_t*)(ws + w.q), (float*)(ws + w.s), M, K, w.Kp);
   HGK_LAUNCH_CHECK();
   if (w.pad) {
-    launch_pad<uint8_t>(st, w0, ws + w.w0, N, K, w.Kp);
-    if (GATED) launch_pad<uint8_t>(st, w1, ws + w.w1, N, K, w.Kp);
+    Pads p;
+    p.add(w0, ws + w.w0, N, K, w.Kp, 1);
+    if (GATED) p.add(w1, ws + w.w1, N, K, w.Kp, 1);
+    p.launch<uint8_t>(st);
     HGK_LAUNCH_CHECK();
   }
   GemmArgs a = gemm_args();

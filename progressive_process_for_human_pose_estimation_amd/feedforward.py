@@ -111,6 +111,15 @@ def _workspace(n, x):
     return ws.data_ptr(), n, ws
 
 
+def _once(backward):
+    """once_differentiable, whose bookkeeping is spared where no second derivative can be asked for"""
+    checked = torch.autograd.function.once_differentiable(backward)
+
+    def call(ctx, grad):
+        return checked(ctx, grad) if torch.is_grad_enabled() else backward(ctx, grad)
+    return call
+
+
 # ---- the gated product ----
 def _gated_fwd(x, wg, wu, act):
     F, C = wg.shape
@@ -131,7 +140,7 @@ class _Gated(torch.autograd.Function):
         return _gated_fwd(x, wg, wu, act)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dh):
         x, wg, wu = ctx.saved_tensors
         F, C = wg.shape
@@ -180,7 +189,7 @@ class _Linear(torch.autograd.Function):
         return _linear_fwd(x, w, None if res is None else _dense(res), p, seed, offset, step)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         x, w, step = ctx.saved_tensors
         p, seed, offset = ctx.drop
@@ -233,7 +242,7 @@ class _DropoutAdd(torch.autograd.Function):
         return _dropout(_dense(x), None if res is None else _dense(res), rows_per_mask, p, seed, offset, step)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once
     def backward(ctx, dy):
         saved = ctx.saved_tensors
         dx = None
