@@ -133,10 +133,31 @@ __device__ __forceinline__ float sigmoid_f(float g) {
   if (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f));
   return 1.f / (1.f + expf(-g));
 }
+// Phi(g), the normal distribution's integral, and e = exp(-g^2 / 2). FAST: Abramowitz and Stegun 7.1.26
+// (|error| <= 1.5e-7 of erfc, on the scale of 1), a third of erfcf's instructions
+template <bool FAST>
+__device__ __forceinline__ float phi_f(float g, float& e) {
+  if (!FAST) {
+    e = expf(-0.5f * g * g);
+    return 0.5f * erfcf(g * -0.70710678f);
+  }
+  const float x = fabsf(g) * 0.70710678f;
+  const float t = __builtin_amdgcn_rcpf(fmaf(0.3275911f, x, 1.f));
+  e = __builtin_amdgcn_exp2f(x * x * -1.44269504f);
+  float p = fmaf(1.061405429f, t, -1.453152027f);
+  p = fmaf(p, t, 1.421413741f);
+  p = fmaf(p, t, -0.284496736f);
+  p = fmaf(p, t, 0.254829592f);
+  const float q = 0.5f * p * t * e;  // Phi(-|g|)
+  return g < 0.f ? q : 1.f - q;
+}
 template <int ACT, bool FAST>
 __device__ __forceinline__ float act_f(float g) {
   if (ACT == kActSilu) return g * sigmoid_f<FAST>(g);
-  if (ACT == kActGelu) return 0.5f * g * erfcf(g * -0.70710678f);
+  if (ACT == kActGelu) {
+    float e;
+    return g * phi_f<FAST>(g, e);
+  }
   if (ACT == kActRelu) return g > 0.f || g != g ? g : 0.f;
   return sigmoid_f<FAST>(g);
 }
@@ -148,8 +169,8 @@ __device__ __forceinline__ void act_slope(float g, float& a, float& s) {
     a = g * q;
     s = q + a * (1.f - q);
   } else if (ACT == kActGelu) {
-    const float h = 0.5f * erfcf(g * -0.70710678f);
-    const float e = FAST ? __builtin_amdgcn_exp2f(g * g * -0.72134752f) : expf(-0.5f * g * g);
+    float e;
+    const float h = phi_f<FAST>(g, e);
     a = g * h;
     s = h + g * 0.39894228f * e;
   } else if (ACT == kActRelu) {
@@ -602,15 +623,89 @@ void gemm_kernel(GemmArgs a) {
   }
 }
 
+// ---- quantising: s = max |v| / 127, q = rint(v / s) ----
+struct QuantScale {
+  float sc, inv;
+  bool none, plain;
+};
+// m: the largest magnitude's bits (magnitudes compare like their bits, infinities and NaN above all
+// numbers); returns the scale that is stored
+__device__ __forceinline__ float quant_scale(uint32_t m, QuantScale& z) {
+  const bool odd = m >= 0x7f800000u;  // an infinity or a NaN
+  z.sc = __uint_as_float(m) / 127.f;
+  z.none = odd || z.sc == 0.f;
+  z.inv = 1.f / z.sc;
+  z.plain = z.sc >= 1e-30f && z.sc <= 1e30f;
+  return odd ? __int_as_float(0x7fc00000) : z.sc;
+}
+// The low byte of b[e] is rint(v[e] / sc), v / sc correctly rounded as the definition's quotient of two fp32
+// values is: from the correctly rounded reciprocal, one fused step makes the product faithful (within a
+// unit in the last place) and the next one exact (Markstein, 1990). Where sc or its reciprocal leaves
+// the normal numbers: the division itself. Adding 1.5 2^23 rounds to a whole number.
+template <int V>
+__device__ __forceinline__ void quant_bytes(const float* v, const QuantScale& z, uint32_t* b) {
+  if (z.plain) {
+#pragma unroll
+    for (int e = 0; e < V; ++e) {
+      float t = v[e] * z.inv;
+      t = fmaf(fmaf(-t, z.sc, v[e]), z.inv, t);
+      t = fmaf(fmaf(-t, z.sc, v[e]), z.inv, t);
+      b[e] = __float_as_uint(t + 12582912.f);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e)
+      b[e] = z.none ? 0 : (uint32_t)(int)fminf(fmaxf(rintf(v[e] / z.sc), -127.f), 127.f);
+  }
+}
+__device__ __forceinline__ uint32_t pack_bytes(const uint32_t* b) {
+  return (b[0] & 0xffu) | (b[1] & 0xffu) << 8 | (b[2] & 0xffu) << 16 | b[3] << 24;
+}
+template <int V>
+__device__ __forceinline__ uint32_t max_bits(const float* v, uint32_t m) {
+#pragma unroll
+  for (int e = 0; e < V; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
+  return m;
+}
+// a wave quantises one row of K elements (K a multiple of 16 bytes of T) in two passes, the second from the cache
+template <typename T>
+__device__ __forceinline__ float quant_row(const T* row, int8_t* q, int K, int lane) {
+  constexpr int V = Vec16<T>::N;
+  uint32_t m = 0;
+  for (int c = lane; c < K / V; c += 64) {
+    float f[V];
+    unpack16<T>(load16(row + c * V), f);
+    m = max_bits<V>(f, m);
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
+  QuantScale z;
+  const float sc = quant_scale(m, z);
+  for (int c = lane; c < K / V; c += 64) {
+    float f[V];
+    uint32_t b[V];
+    unpack16<T>(load16(row + c * V), f);
+    quant_bytes<V>(f, z, b);
+#pragma unroll
+    for (int e = 0; e < V; e += 4) *reinterpret_cast<uint32_t*>(q + c * V + e) = pack_bytes(b + e);
+  }
+  return sc;
+}
+
 // ---- few rows (M <= 16 MT): the weights stream once from memory into fragments, no LDS tiles ----
 // A workgroup owns 16 output columns (gated: 16 gate and 16 up), its 8 waves take every 8th K-step
 // of 128 bytes, the partial sums meet in LDS in wave order. Bound by the weights' bytes: one
 // column group of 16 rows x 128 bytes per load pair, M rows of x from the caches.
-template <int DT, typename T, int MT, bool DUAL>
+// QUANT (8-bit integers, M <= kQuantRows, K <= kQuantK): x is T, and every workgroup quantises its few rows
+// into LDS itself, in place of a launch and a trip through memory.
+static constexpr int kQuantRows = 4, kQuantK = 8192;
+template <int DT, typename T, int MT, bool DUAL, bool QUANT = false>
 __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
   constexpr int es = GT<DT>::es, P = DUAL ? 2 : 1, NW = 8;
   typedef typename GT<DT>::acc acc_t;
   __shared__ acc_t red[NW][P * MT][64];
+  __shared__ __attribute__((aligned(16))) int8_t xq[QUANT ? kQuantRows * kQuantK : 16];
+  __shared__ float xs[QUANT ? kQuantRows : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
   const int n0 = blockIdx.x * 16;
   const char* w[P];
@@ -619,6 +714,13 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
   const char* x[MT];
 #pragma unroll
   for (int i = 0; i < MT; ++i) x[i] = a.m0 + (long)min(i * 16 + lr, a.M - 1) * a.ldm;
+  if constexpr (QUANT) {
+    if (wave < a.M) {
+      const float sc = quant_row<T>((const T*)a.m0 + (long)wave * a.km, xq + wave * a.km, a.km, lane);
+      if (lane == 0) xs[wave] = sc;
+    }
+    __syncthreads();
+  }
   acc_t acc[P][MT];
 #pragma unroll
   for (int p = 0; p < P; ++p)
@@ -635,7 +737,13 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
 #pragma unroll
       for (int p = 0; p < P; ++p) wv[h][p] = *reinterpret_cast<const i32x4*>(ok ? w[p] + k : g_zero_page);
 #pragma unroll
-      for (int i = 0; i < MT; ++i) xv[h][i] = *reinterpret_cast<const i32x4*>(ok ? x[i] + k : g_zero_page);
+      for (int i = 0; i < MT; ++i) {
+        if constexpr (QUANT) {
+          xv[h][i] = ok ? *reinterpret_cast<const i32x4*>(xq + min(lr, a.M - 1) * a.km + k) : i32x4{0, 0, 0, 0};
+        } else {
+          xv[h][i] = *reinterpret_cast<const i32x4*>(ok ? x[i] + k : g_zero_page);
+        }
+      }
     }
 #pragma unroll
     for (int h = 0; h < 2; ++h)
@@ -662,7 +770,7 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
     for (int e = 0; e < 4; ++e) {
       f[p][e] = (float)t[e];
       if constexpr (DT == G_I8)
-        f[p][e] = f[p][e] * a.row_scale[m] * (p ? a.col_scale1 : a.col_scale)[min(n + e, a.N - 1)];
+        f[p][e] = f[p][e] * (QUANT ? xs[QUANT ? m : 0] : a.row_scale[m]) * (p ? a.col_scale1 : a.col_scale)[min(n + e, a.N - 1)];
     }
   }
   if constexpr (DUAL) {
@@ -822,8 +930,8 @@ struct GemmPlan {
 // 1.5 us of a CU in bf16 (1467 TFLOP/s over the chip at 8192 x 4096 x 8192); per unit of work a
 // 128-wide tile takes 1.3 times that (1147), a 64-wide one 2 to 3 times (502 .. 704): its waves read
 // twice to four times the fragments per product. fp32's matrix instructions are 16 times slower and
-// hide all of that. A CU with one or two workgroups waits for memory instead: 1.2 us
-// a step at least. Against the
+// hide all of that. A CU with one or two workgroups waits for memory instead: 0.8 us
+// a step and its products. A round ends with its epilogue, 4 us of a 256-wide tile. Against the
 // tile stand the rounds: tiles are dealt to 256 CUs whole. Splitting k costs the partial sums' way to
 // memory and back (4.5 TB/s) and a second launch (5 us).
 static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int batch, bool can_split) {
@@ -843,7 +951,7 @@ static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int
     for (int split = 1; split <= 64; split *= 2) {
       if (split > 1 && (!can_split || n * split > slots || steps / split < 4)) break;
       const double rounds = (double)((n * split + 255) / 256), each = (double)((steps + split - 1) / split);
-      double t = std::max(rounds * step, 1.2) * each;
+      double t = std::max(rounds * step, 0.8 + step) * each + rounds * 4.0 * b * b / 65536;
       if (split > 1) t += 5 + 8.0 * split * batch * M * N / 4.5e6;
       if (t < least) {
         least = t;

@@ -28,12 +28,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
     else v[0] = to_f(row[c]);
   };
   const int nc = K / V;  // VEC: K % V == 0
-  // magnitudes compare like their bits, infinities and NaN above all numbers
   uint32_t m = 0;
-  auto scan = [&](const float* v) __attribute__((always_inline)) {
-#pragma unroll
-    for (int e = 0; e < V; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
-  };
+  auto scan = [&](const float* v) __attribute__((always_inline)) { m = max_bits<V>(v, m); };
   if constexpr (NCH > 0) {
 #pragma unroll
     for (int i = 0; i < NCH; ++i) {
@@ -52,41 +48,15 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
   }
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, L));
-  const bool odd = m >= 0x7f800000u;  // an infinity or a NaN
-  const float sc = __uint_as_float(m) / 127.f;
-  const bool none = odd || sc == 0.f;
-  if (lane == 0) s[r] = odd ? __int_as_float(0x7fc00000) : sc;
-  // v / sc correctly rounded, the quotient of two fp32 values that the definition rounds to a whole step: from
-  // the correctly rounded reciprocal, one fused step makes the product faithful (within a unit in the last
-  // place) and the next one exact (Markstein, 1990). Where sc or its reciprocal leaves the normal numbers: the
-  // division itself. Adding 1.5 2^23 rounds to a whole number, whose low byte is the result.
-  const float inv = 1.f / sc;
-  const bool plain = sc >= 1e-30f && sc <= 1e30f;
+  QuantScale z;
+  const float sc = quant_scale(m, z);
+  if (lane == 0) s[r] = sc;
   auto put = [&](int c, const float* v) __attribute__((always_inline)) {
     uint32_t b[V];
-    if (plain) {
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        float t = v[e] * inv;
-        t = fmaf(fmaf(-t, sc, v[e]), inv, t);
-        t = fmaf(fmaf(-t, sc, v[e]), inv, t);
-        b[e] = __float_as_uint(t + 12582912.f);
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < V; ++e)
-        b[e] = none ? 0 : (uint32_t)(int)fminf(fmaxf(rintf(v[e] / sc), -127.f), 127.f);
-    }
-    if constexpr (VEC) {
-      uint32_t w[V / 4];
-#pragma unroll
-      for (int e = 0; e < V; e += 4)
-        w[e / 4] = (b[e] & 0xffu) | (b[e + 1] & 0xffu) << 8 | (b[e + 2] & 0xffu) << 16 | b[e + 3] << 24;
-      if constexpr (V == 8) *reinterpret_cast<uint2*>(qrow + c * 8) = make_uint2(w[0], w[1]);
-      else *reinterpret_cast<uint32_t*>(qrow + c * 4) = w[0];
-    } else {
-      qrow[c] = (int8_t)b[0];
-    }
+    quant_bytes<V>(v, z, b);
+    if constexpr (VEC && V == 8) *reinterpret_cast<uint2*>(qrow + c * 8) = make_uint2(pack_bytes(b), pack_bytes(b + 4));
+    else if constexpr (VEC) *reinterpret_cast<uint32_t*>(qrow + c * 4) = pack_bytes(b);
+    else qrow[c] = (int8_t)b[0];
   };
   if constexpr (NCH > 0) {
 #pragma unroll
@@ -129,6 +99,141 @@ static void launch_quant(hipStream_t st, const void* x, int8_t* q, float* s, lon
     launch_quant_as<T, false>(st, (const T*)x, q, s, rows, K, Kp);
 }
 
+// ---- wide maps of few channels (K <= 256, N <= 256: the pointwise products of the pixel levels) ----
+// The weights stay in LDS and a workgroup walks 128-row tiles: a tile's rows are read once as T, quantised
+// in registers (4 lanes a row) and written to LDS as bytes, so the quantised rows never go through memory:
+// 4 bytes an element of x and y in all. The next tile is on its way from memory while this one's products
+// run. Bound by memory.
+static constexpr int kMapK = 256, kMapN = 256, kMapRows = 128;
+template <typename T>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
+void i8_map_kernel(GemmArgs a, int tiles) {
+  constexpr int V = Vec16<T>::N, NC = kMapK / V / 4;  // 16-byte chunks of a lane
+  __shared__ __attribute__((aligned(16))) char lw[kMapN * kMapK];
+  __shared__ __attribute__((aligned(16))) char lx[2][kMapRows * kMapK];
+  __shared__ float ls[2][kMapRows];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
+  const int wm = wave >> 2, wn = wave & 3;  // wave tile: 64 rows x 64 columns
+  const int K = a.km, halves = (K + 63) / 64;
+  // byte chunk c of row r sits at slot c ^ (r & 7) of its group of 8: the 8 rows of a b128 read differ
+  for (int i = tid; i < kMapN * (kMapK / 16); i += 512) {
+    const int r = i / (kMapK / 16), c = i % (kMapK / 16);
+    const int n = min(r, a.N - 1);
+    const uint4 v = c * 16 < K ? *reinterpret_cast<const uint4*>(a.n0 + (long)n * K + c * 16) : make_uint4(0, 0, 0, 0);
+    *reinterpret_cast<uint4*>(lw + r * kMapK + ((c ^ (r & 7)) << 4)) = v;
+  }
+  const int qr = tid >> 2, ql = tid & 3;
+  typename Vec16<T>::type xv[NC];
+  auto load = [&](int tile) __attribute__((always_inline)) {
+    const T* row = (const T*)a.m0 + min((long)tile * kMapRows + qr, (long)a.M - 1) * K;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int c = ql + 4 * j;
+      if (c * V < K) xv[j] = load16(row + c * V);
+    }
+  };
+  auto quantise = [&](int buf) __attribute__((always_inline)) {
+    uint32_t m = 0;
+    float f[V];
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      if ((ql + 4 * j) * V < K) {
+        unpack16<T>(xv[j], f);
+        m = max_bits<V>(f, m);
+      }
+    }
+    m = max(m, (uint32_t)__shfl_xor((int)m, 1, 4));
+    m = max(m, (uint32_t)__shfl_xor((int)m, 2, 4));
+    QuantScale z;
+    const float sc = quant_scale(m, z);
+    if (ql == 0) ls[buf][qr] = sc;
+#pragma unroll
+    for (int j = 0; j < NC; ++j) {
+      const int at = (ql + 4 * j) * V;  // byte in the row
+      uint32_t b[V];
+#pragma unroll
+      for (int e = 0; e < V; ++e) b[e] = 0;
+      if (at < K) {
+        unpack16<T>(xv[j], f);
+        quant_bytes<V>(f, z, b);
+      }
+      char* p = lx[buf] + qr * kMapK + ((((at >> 4) ^ (qr & 7))) << 4) + (at & 15);
+#pragma unroll
+      for (int e = 0; e < V; e += 4) *reinterpret_cast<uint32_t*>(p + e) = pack_bytes(b + e);
+    }
+  };
+  int tile = blockIdx.x, buf = 0;
+  if (tile < tiles) load(tile);
+  for (; tile < tiles; tile += gridDim.x, buf ^= 1) {  // the whole workgroup
+    quantise(buf);
+    __syncthreads();  // also: every wave is done with this buffer's last tile but one
+    if (tile + (int)gridDim.x < tiles) load(tile + gridDim.x);
+    i32x4 acc[4][4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
+    for (int h = 0; h < halves; ++h) {
+      i32x4 fm[4], fn[4];
+      const int c = h * 4 + lg;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // the order of the N rows as in gemm_kernel
+        const int r = wn * 64 + (j >> 1) * 32 + 8 * (lr >> 2) + 4 * (j & 1) + (lr & 3);
+        fn[j] = *reinterpret_cast<const i32x4*>(lw + r * kMapK + ((c ^ (r & 7)) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = wm * 64 + i * 16 + lr;
+        fm[i] = *reinterpret_cast<const i32x4*>(lx[buf] + r * kMapK + ((c ^ (r & 7)) << 4));
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j][i] = mma<G_I8>(fn[j], fm[i], acc[j][i]);
+    }
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      const int n = wn * 64 + 32 * g + 8 * lg;
+      if (n >= a.N) continue;
+      float cs[8], bias[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int c = min(n + e, a.N - 1);
+        cs[e] = a.col_scale[c];
+        bias[e] = a.bias ? a.bias[c] : 0.f;
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = wm * 64 + i * 16 + lr;
+        const long m = (long)tile * kMapRows + r;
+        if (m >= a.M) continue;
+        const float rs = ls[buf][r];
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) f[e] = (float)acc[2 * g + (e >> 2)][i][e & 3] * rs * cs[e] + bias[e];
+        if (a.res) {
+          float q[8];
+          load8<T>((const T*)a.res + m * a.N, n, a.N, a.vec, q);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) f[e] += q[e];
+        }
+        store8<T>((T*)a.out + m * a.N, n, a.N, a.vec, f);
+      }
+    }
+  }
+}
+
+// which kernel a call takes, and what it needs
+enum I8Way { W_FEW_FUSED, W_FEW, W_MAP, W_TILES };
+static I8Way i8_way(long M, int K, int N, bool gated) {
+  if (M <= kQuantRows && K <= kQuantK && K % 16 == 0) return W_FEW_FUSED;
+  if (M <= 64) return W_FEW;
+  // at least two row tiles a CU: 131072 x 256 x 256 takes 33 us against 51 of the quantiser and the tiled
+  // product; with fewer the CUs that stay empty cost more than the second launch
+  if (!gated && K <= kMapK && K % 16 == 0 && N <= kMapN && M >= 512 * kMapRows) return W_MAP;
+  return W_TILES;
+}
+
 struct I8Ws {
   long q, s, w0, w1, total;
   int Kp;
@@ -138,6 +243,9 @@ static I8Ws i8_ws(long M, int K, int N, bool gated) {
   I8Ws w;
   w.Kp = (int)up_to(K, 16);
   w.pad = w.Kp != K;
+  w.q = w.s = w.w0 = w.w1 = w.total = 0;
+  const I8Way way = i8_way(M, K, N, gated);
+  if (way == W_FEW_FUSED || way == W_MAP) return w;
   long at = 0;
   auto take = [&](long b) {
     const long o = at;
@@ -157,34 +265,50 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
                      const float* s1, const float* bias, const void* res, void* y, long M, int K, int N, int act,
                      char* ws) {
   const I8Ws w = i8_ws(M, K, N, GATED);
-  launch_quant<T>(st, x, (int8_t*)(ws + w.q), (float*)(ws + w.s), M, K, w.Kp);
-  HGK_LAUNCH_CHECK();
-  if (w.pad) {
-    Pads p;
-    p.add(w0, ws + w.w0, N, K, w.Kp, 1);
-    if (GATED) p.add(w1, ws + w.w1, N, K, w.Kp, 1);
-    p.launch<uint8_t>(st);
-    HGK_LAUNCH_CHECK();
-  }
+  const I8Way way = i8_way(M, K, N, GATED);
   GemmArgs a = gemm_args();
-  a.m0 = ws + w.q;
-  a.n0 = w.pad ? ws + w.w0 : (const char*)w0;
-  a.n1 = w.pad ? ws + w.w1 : (const char*)w1;
+  a.n0 = (const char*)w0;
+  a.n1 = (const char*)w1;
   a.ldm = a.ldn = w.Kp;
   a.M = (int)M;
   a.N = N;
   a.km = a.kn = w.Kp;
   a.spseg = (w.Kp + 127) / 128;
   a.out = y;
-  a.row_scale = (const float*)(ws + w.s);
   a.col_scale = s0;
   a.col_scale1 = s1;
   a.bias = bias;
   a.res = res;
   a.act = act;
   a.vec = N % 8 == 0;
+  if (way == W_FEW_FUSED || way == W_MAP) {
+    a.m0 = (const char*)x;
+    if (way == W_MAP) {
+      const int tiles = (int)((M + kMapRows - 1) / kMapRows);
+      hipLaunchKernelGGL((i8_map_kernel<T>), dim3(256), dim3(512), 0, st, a, tiles);
+    } else {
+      hipLaunchKernelGGL((skinny_kernel<G_I8, T, 1, GATED, true>), dim3((unsigned)((N + 15) / 16)), dim3(512), 0, st, a);
+    }
+    HGK_LAUNCH_CHECK();
+    return HGK_OK;
+  }
+  launch_quant<T>(st, x, (int8_t*)(ws + w.q), (float*)(ws + w.s), M, K, w.Kp);
+  HGK_LAUNCH_CHECK();
+  a.m0 = ws + w.q;
+  a.row_scale = (const float*)(ws + w.s);
+  if (w.pad) {
+    Pads p;
+    p.add(w0, ws + w.w0, N, K, w.Kp, 1);
+    a.n0 = ws + w.w0;
+    if (GATED) {
+      p.add(w1, ws + w.w1, N, K, w.Kp, 1);
+      a.n1 = ws + w.w1;
+    }
+    p.launch<uint8_t>(st);
+    HGK_LAUNCH_CHECK();
+  }
   constexpr int EPI = GATED ? E_GATED : E_OUT, per = GATED ? 2 : 1;
-  if (M <= 64) {
+  if (way == W_FEW) {
     const dim3 grid((unsigned)((N + 15) / 16));
     if (M <= 16) hipLaunchKernelGGL((skinny_kernel<G_I8, T, 1, GATED>), grid, dim3(512), 0, st, a);
     else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<G_I8, T, 2, GATED>), grid, dim3(512), 0, st, a);
@@ -226,9 +350,9 @@ int hgk_linear_i8(hgk_stream_t stream, int dtype, const void* x, const void* wq,
   HGK_CHECK_ARG(M >= 0 && M <= (1l << 30) && K >= 1 && K <= kI8MaxK && N >= 1 && N <= (1 << 24),
                 "linear_i8: bad sizes (%ld, %d, %d)", M, K, N);
   if (M == 0) return HGK_OK;
-  HGK_CHECK_ARG(x && wq && wscale && y && workspace, "linear_i8: null pointer");
+  HGK_CHECK_ARG(x && wq && wscale && y, "linear_i8: null pointer");
   HGK_CHECK_ARG(al16(x) && al16(wq) && al16(res) && al16(y) && al16(workspace), "linear_i8: pointers must be 16-byte aligned");
-  HGK_CHECK_ARG(ws_bytes >= hgk_linear_i8_workspace(M, K, N, 0), "linear_i8: workspace of %zu bytes is too small", ws_bytes);
+  HGK_CHECK_ARG(ws_bytes >= hgk_linear_i8_workspace(M, K, N, 0) && (workspace || !hgk_linear_i8_workspace(M, K, N, 0)), "linear_i8: workspace of %zu bytes is too small", ws_bytes);
   HGK_DISPATCH_DTYPE(dtype, T, return (linear_i8<T, false>((hipStream_t)stream, x, wq, wscale, nullptr, nullptr,
                                                            bias, res, y, M, K, N, 0, (char*)workspace)));
 }
@@ -240,9 +364,9 @@ int hgk_gated_i8(hgk_stream_t stream, int dtype, const void* x, const void* wqg,
                 "gated_i8: bad sizes (%ld, %d, %d)", M, C, F);
   HGK_CHECK_ARG(act >= 0 && act < HGK_ACT_COUNT, "gated_i8: unknown activation %d", act);
   if (M == 0) return HGK_OK;
-  HGK_CHECK_ARG(x && wqg && sg && wqu && su && h && workspace, "gated_i8: null pointer");
+  HGK_CHECK_ARG(x && wqg && sg && wqu && su && h, "gated_i8: null pointer");
   HGK_CHECK_ARG(al16(x) && al16(wqg) && al16(wqu) && al16(h) && al16(workspace), "gated_i8: pointers must be 16-byte aligned");
-  HGK_CHECK_ARG(ws_bytes >= hgk_linear_i8_workspace(M, C, F, 1), "gated_i8: workspace of %zu bytes is too small", ws_bytes);
+  HGK_CHECK_ARG(ws_bytes >= hgk_linear_i8_workspace(M, C, F, 1) && (workspace || !hgk_linear_i8_workspace(M, C, F, 1)), "gated_i8: workspace of %zu bytes is too small", ws_bytes);
   HGK_DISPATCH_DTYPE(dtype, T, return (linear_i8<T, true>((hipStream_t)stream, x, wqg, sg, wqu, su, nullptr, nullptr, h,
                                                           M, C, F, act, (char*)workspace)));
 }

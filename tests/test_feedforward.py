@@ -75,7 +75,7 @@ def test_abi_refusals():
     refused(L.hgk_quantize_rows_i8(None, 0, A, A, A, 4, (1 << 17) + 1), "bad sizes")
     refused(L.hgk_quantize_rows_i8(None, 0, A, None, A, 4, 8), "null")
     refused(L.hgk_linear_i8(None, 0, A, A, A, None, None, A, 4, (1 << 17) + 1, 8, A, big), "bad sizes")
-    refused(L.hgk_linear_i8(None, 0, A, A, A, None, None, A, 4, 8, 8, A, 8), "too small")
+    refused(L.hgk_linear_i8(None, 0, A, A, A, None, None, A, 40, 8, 8, A, 8), "too small")
     refused(L.hgk_linear_i8(None, 0, A, A, None, None, None, A, 4, 8, 8, A, big), "null")
     refused(L.hgk_gated_i8(None, 0, A, A, A, A, A, A, 4, 8, 8, 9, A, big), "activation")
     refused(L.hgk_gated_i8(None, 0, A, A + 8, A, A, A, A, 4, 8, 8, 0, A, big), "16-byte")

@@ -225,7 +225,9 @@ def test_expanded_input_gradient():
 
 # ---- 8-bit integers ----
 I8 = [(1, 8, 8), (1, 1, 1), (2, 17, 5), (16, 1000, 40), (17, 64, 129), (64, 130, 16), (65, 128, 128), (200, 257, 66),
-      (333, 96, 515), (8192 + 5, 48, 2064), (20, 5000, 24), (4, 20000, 8)]
+      (333, 96, 515), (8192 + 5, 48, 2064), (20, 5000, 24), (4, 20000, 8),
+      (1, 8192, 33), (4, 16, 7), (3, 4096, 100), (4, 8208, 20),              # rows quantised by each workgroup
+      (65536 + 3, 256, 256), (65535, 64, 40), (65536 + 200, 48, 129), (70000, 16, 1), (65536, 240, 255)]  # wide maps
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -262,16 +264,42 @@ def test_gated_i8(M, C, Fh, name, dtype):
     R.worst(F.gated_linear_i8(x, wg, sg, wu, su, name), (h, e + R.U[dtype] * (h.abs() + e) + R.TINY))
 
 
-def test_i8_rows_of_infinities_and_zeros():
-    x = rnd(0, 70, 48)
+@pytest.mark.parametrize("M", [70, 65536 + 70])
+def test_i8_rows_of_infinities_and_zeros(M):
+    x = rnd(0, M, 48)
     x[5, 3], x[6, 0], x[7] = float("inf"), float("nan"), 0
     wq, ws = F.quantize_rows(rnd(1, 20, 48))
     y = F.linear_i8(x, wq, ws)
     assert bool(y[5:7].isnan().all()) and torch.equal(y[7], torch.zeros_like(y[7]))
-    rest = [i for i in range(70) if i not in (5, 6)]
+    rest = torch.tensor([i for i in range(M) if i not in (5, 6)], device=DEV)
     clean = x.clone()
     clean[5:7] = 0
     assert torch.equal(y[rest], F.linear_i8(clean, wq, ws)[rest])
+
+
+@pytest.mark.parametrize("M,K", [(1, 64), (100, 64), (65536, 64), (300, 1000)])
+def test_quantised_steps_at_the_borders(M, K):
+    """Values at and next to half steps of the grid, tiny and huge scales: the quotient of two fp32 values
+    rounded to a whole step, as the CPU's division has it."""
+    g = torch.Generator().manual_seed(M + K)
+    amax = torch.ldexp(1 + torch.rand(M, generator=g), torch.randint(-120, 120, (M,), generator=g))
+    s = amax / 127
+    k = torch.randint(-127, 127, (M, K), generator=g)
+    x = (k + 0.5) * s[:, None]
+    x = torch.where(torch.rand(M, K, generator=g) < 0.5, torch.nextafter(x, torch.full_like(x, 3e38)), x).clamp(-amax[:, None], amax[:, None])
+    x[:, 0] = amax
+    if M > 3:
+        x[1] = torch.randint(-300, 300, (K,), generator=g) * 1e-45  # below the normal numbers
+        x[1, 0] = 9e-44
+    q, sc = F.quantize_rows(x.to(DEV))
+    q0, s0 = R.quantize(x)
+    if M > 3:  # a scale of a few units may be rounded to below a 127th: clamped to the grid
+        q0[1] = torch.round(x[1] / s0[1]).clamp(-127, 127).to(torch.int8)
+    assert torch.equal(sc.cpu(), s0) and torch.equal(q.cpu(), q0)
+    wq = torch.eye(K, dtype=torch.int8, device=DEV)[:min(K, 200)]
+    one = torch.ones(len(wq), device=DEV)
+    y = F.linear_i8(x.to(DEV), wq, one).cpu()
+    assert torch.equal(y, q0[:, :len(wq)].float() * s0[:, None])
 
 
 def test_i8_largest_sums_are_exact():
