@@ -24,7 +24,7 @@ static int run_product(hipStream_t st, GemmArgs& a, const GemmPlan& p, char* sla
     run_tiles<DT, T, LM, LN, E_SLAB>(st, a, p);
     HGK_LAUNCH_CHECK();
     const long n = (long)a.batch * a.M * ((a.N + 7) / 8);
-    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((n + 63) / 64)), dim3(64), 0, st, a);
   } else {
     run_tiles<DT, T, LM, LN, E_OUT>(st, a, p);
   }

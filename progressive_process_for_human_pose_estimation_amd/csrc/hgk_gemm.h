@@ -48,7 +48,7 @@ namespace hgk {
 enum GemmType { G_F32 = 0, G_BF16 = 1, G_I8 = 2 };
 enum GemmLayout { L_ROW = 0, L_COL = 1 };
 enum GemmEpi {
-  E_SLAB = 0,   // fp32 partial sums of one k range to slab[split][batch][M][N]
+  E_SLAB = 0,   // fp32 partial sums of one k range to slab[split][batch][M][N up to a multiple of 8]
   E_OUT = 1,    // rounded to T: plain, bias, scales, dropout, residual
   E_GATED = 2,  // a(g) u, the N tile holding gate columns and up columns
   E_GATED_BWD = 3  // dg, du from dh and the recomputed g, u
@@ -599,7 +599,7 @@ void gemm_kernel(GemmArgs a) {
               if (n + e >= a.N) dg[k][e] = du[k][e] = 0.f;
           }
         } else if constexpr (EPI == E_SLAB) {
-          store8<float>(a.slab + (((long)split * a.batch + bat) * a.M + m) * a.N, n, a.N, vec, f);
+          store8<float>(a.slab + (((long)split * a.batch + bat) * a.M + m) * ((a.N + 7) & ~7), n, a.N, true, f);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) f[e] = fmaf(f[e], a.alpha, bias[k][e]);
@@ -797,21 +797,21 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
 
 // sum of the k ranges' partial sums in their order, then the epilogue of E_OUT
 template <typename T>
-__global__ __launch_bounds__(256) void gemm_join_kernel(GemmArgs a) {
+__global__ __launch_bounds__(64) void gemm_join_kernel(GemmArgs a) {
   const int n8 = (a.N + 7) >> 3;
-  const long t = (long)blockIdx.x * 256 + threadIdx.x;
+  const long t = (long)blockIdx.x * 64 + threadIdx.x;
   if (t >= (long)a.batch * a.M * n8) return;
   const int n = (int)(t % n8) * 8;
   const long bm = t / n8;  // batch * M + m
   const int bat = (int)(bm / a.M), m = (int)(bm - (long)bat * a.M);
-  const long pitch = (long)a.batch * a.M * a.N;
-  const float* s = a.slab + bm * a.N;
+  const long pitch = (long)a.batch * a.M * (n8 * 8);
+  const float* s = a.slab + bm * (n8 * 8);
   const bool vec = a.vec != 0;
   float f[8] = {};
 #pragma unroll 4
   for (int k = 0; k < a.splits; ++k) {
     float q[8];
-    load8<float>(s + k * pitch, n, a.N, vec, q);
+    load8<float>(s + k * pitch, n, a.N, true, q);
 #pragma unroll
     for (int e = 0; e < 8; ++e) f[e] += q[e];
   }
@@ -931,7 +931,7 @@ struct GemmPlan {
 // 128-wide tile takes 1.3 times that (1147), a 64-wide one 2 to 3 times (502 .. 704): its waves read
 // twice to four times the fragments per product. fp32's matrix instructions are 16 times slower and
 // hide all of that. A CU with one or two workgroups waits for memory instead: 0.8 us
-// a step and its products. A round ends with its epilogue, 4 us of a 256-wide tile. Against the
+// a step and half its products. A round ends with its epilogue, 4 us of a 256-wide tile. Against the
 // tile stand the rounds: tiles are dealt to 256 CUs whole. Splitting k costs the partial sums' way to
 // memory and back (4.5 TB/s) and a second launch (5 us).
 static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int batch, bool can_split) {
@@ -951,7 +951,7 @@ static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int
     for (int split = 1; split <= 64; split *= 2) {
       if (split > 1 && (!can_split || n * split > slots || steps / split < 4)) break;
       const double rounds = (double)((n * split + 255) / 256), each = (double)((steps + split - 1) / split);
-      double t = std::max(rounds * step, 0.8 + step) * each + rounds * 4.0 * b * b / 65536;
+      double t = std::max(rounds * step, 0.8 + 0.5 * step) * each + rounds * 4.0 * b * b / 65536;
       if (split > 1) t += 5 + 8.0 * split * batch * M * N / 4.5e6;
       if (t < least) {
         least = t;
@@ -960,7 +960,7 @@ static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int
       }
     }
   }
-  best.slab = best.splits > 1 ? (long)best.splits * batch * M * N * 4 : 0;
+  best.slab = best.splits > 1 ? best.splits * batch * M * up_to(N, 8) * 4 : 0;
   return best;
 }
 

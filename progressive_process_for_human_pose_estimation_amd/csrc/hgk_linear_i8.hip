@@ -100,56 +100,56 @@ static void launch_quant(hipStream_t st, const void* x, int8_t* q, float* s, lon
 }
 
 // ---- wide maps of few channels (K <= 256, N <= 256: the pointwise products of the pixel levels) ----
-// The weights stay in LDS and a workgroup walks 128-row tiles: a tile's rows are read once as T, quantised
-// in registers (4 lanes a row) and written to LDS as bytes, so the quantised rows never go through memory:
-// 4 bytes an element of x and y in all. The next tile is on its way from memory while this one's products
-// run. Bound by memory.
-static constexpr int kMapK = 256, kMapN = 256, kMapRows = 128;
+// A wave keeps its 64 columns of the weights in registers, a workgroup of 4 waves walks 32-row tiles: a
+// tile's rows are read once as T, quantised in registers (8 lanes a row) and written to LDS as bytes, so
+// the quantised rows never go through memory: 4 bytes an element of x and y in all. The next tile is on
+// its way from memory while this one's products run. Two workgroups a CU: the quantising and the
+// epilogue of one (18 us of VALU at 131072 x 256 x 256) run beside the memory of the other; one
+// workgroup of 8 waves with the weights in LDS took 45 us, one phase after the other.
+static constexpr int kMapK = 256, kMapN = 256, kMapRows = 32, kMapGroups = 512, kMapMin = 16384;
 template <typename T>
-__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void i8_map_kernel(GemmArgs a, int tiles) {
-  constexpr int V = Vec16<T>::N, NC = kMapK / V / 4;  // 16-byte chunks of a lane
-  __shared__ __attribute__((aligned(16))) char lw[kMapN * kMapK];
+  constexpr int V = Vec16<T>::N, NC = kMapK / V / 8;  // 16-byte chunks of a lane
   __shared__ __attribute__((aligned(16))) char lx[2][kMapRows * kMapK];
   __shared__ float ls[2][kMapRows];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
-  const int wm = wave >> 2, wn = wave & 3;  // wave tile: 64 rows x 64 columns
-  const int K = a.km, halves = (K + 63) / 64;
-  // byte chunk c of row r sits at slot c ^ (r & 7) of its group of 8: the 8 rows of a b128 read differ
-  for (int i = tid; i < kMapN * (kMapK / 16); i += 512) {
-    const int r = i / (kMapK / 16), c = i % (kMapK / 16);
-    const int n = min(r, a.N - 1);
-    const uint4 v = c * 16 < K ? *reinterpret_cast<const uint4*>(a.n0 + (long)n * K + c * 16) : make_uint4(0, 0, 0, 0);
-    *reinterpret_cast<uint4*>(lw + r * kMapK + ((c ^ (r & 7)) << 4)) = v;
-  }
-  const int qr = tid >> 2, ql = tid & 3;
+  const int K = a.km;
+  i32x4 w[4][4];
+#pragma unroll
+  for (int h = 0; h < 4; ++h)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {  // the order of the N rows as in gemm_kernel
+      const int n = min(wave * 64 + (j >> 1) * 32 + 8 * (lr >> 2) + 4 * (j & 1) + (lr & 3), a.N - 1);
+      const int k = h * 64 + lg * 16;
+      w[h][j] = k < K ? *reinterpret_cast<const i32x4*>(a.n0 + (long)n * K + k) : i32x4{0, 0, 0, 0};
+    }
+  const int qr = tid >> 3, ql = tid & 7;
   typename Vec16<T>::type xv[NC];
   auto load = [&](int tile) __attribute__((always_inline)) {
     const T* row = (const T*)a.m0 + min((long)tile * kMapRows + qr, (long)a.M - 1) * K;
 #pragma unroll
-    for (int j = 0; j < NC; ++j) {
-      const int c = ql + 4 * j;
-      if (c * V < K) xv[j] = load16(row + c * V);
-    }
+    for (int j = 0; j < NC; ++j)
+      if ((ql + 8 * j) * V < K) xv[j] = load16(row + (ql + 8 * j) * V);
   };
   auto quantise = [&](int buf) __attribute__((always_inline)) {
     uint32_t m = 0;
     float f[V];
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      if ((ql + 4 * j) * V < K) {
+      if ((ql + 8 * j) * V < K) {
         unpack16<T>(xv[j], f);
         m = max_bits<V>(f, m);
       }
     }
-    m = max(m, (uint32_t)__shfl_xor((int)m, 1, 4));
-    m = max(m, (uint32_t)__shfl_xor((int)m, 2, 4));
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 8));
     QuantScale z;
     const float sc = quant_scale(m, z);
     if (ql == 0) ls[buf][qr] = sc;
 #pragma unroll
     for (int j = 0; j < NC; ++j) {
-      const int at = (ql + 4 * j) * V;  // byte in the row
+      const int at = (ql + 8 * j) * V;  // byte in the row; past K: zero
       uint32_t b[V];
 #pragma unroll
       for (int e = 0; e < V; ++e) b[e] = 0;
@@ -157,43 +157,38 @@ void i8_map_kernel(GemmArgs a, int tiles) {
         unpack16<T>(xv[j], f);
         quant_bytes<V>(f, z, b);
       }
-      char* p = lx[buf] + qr * kMapK + ((((at >> 4) ^ (qr & 7))) << 4) + (at & 15);
+      // byte chunk c of row r sits at slot c ^ (r & 7) of its group of 8: the 8 rows of a b128 read differ
+      char* p = lx[buf] + qr * kMapK + (((at >> 4) ^ (qr & 7)) << 4) + (at & 15);
 #pragma unroll
       for (int e = 0; e < V; e += 4) *reinterpret_cast<uint32_t*>(p + e) = pack_bytes(b + e);
     }
   };
   int tile = blockIdx.x, buf = 0;
   if (tile < tiles) load(tile);
+#pragma unroll 1
   for (; tile < tiles; tile += gridDim.x, buf ^= 1) {  // the whole workgroup
     quantise(buf);
     __syncthreads();  // also: every wave is done with this buffer's last tile but one
     if (tile + (int)gridDim.x < tiles) load(tile + gridDim.x);
-    i32x4 acc[4][4];
+    if (wave * 64 >= a.N) continue;  // a wave without columns quantises only
+    i32x4 acc[4][2];
 #pragma unroll
     for (int j = 0; j < 4; ++j)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
-    for (int h = 0; h < halves; ++h) {
-      i32x4 fm[4], fn[4];
-      const int c = h * 4 + lg;
+      for (int i = 0; i < 2; ++i) acc[j][i] = i32x4{0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {  // the order of the N rows as in gemm_kernel
-        const int r = wn * 64 + (j >> 1) * 32 + 8 * (lr >> 2) + 4 * (j & 1) + (lr & 3);
-        fn[j] = *reinterpret_cast<const i32x4*>(lw + r * kMapK + ((c ^ (r & 7)) << 4));
+    for (int h = 0; h < 4; ++h) {
+      if (h * 64 >= K) break;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const i32x4 x = *reinterpret_cast<const i32x4*>(lx[buf] + (i * 16 + lr) * kMapK + (((h * 4 + lg) ^ (lr & 7)) << 4));
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j][i] = mma<G_I8>(w[h][j], x, acc[j][i]);
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = wm * 64 + i * 16 + lr;
-        fm[i] = *reinterpret_cast<const i32x4*>(lx[buf] + r * kMapK + ((c ^ (r & 7)) << 4));
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j][i] = mma<G_I8>(fn[j], fm[i], acc[j][i]);
     }
 #pragma unroll
     for (int g = 0; g < 2; ++g) {
-      const int n = wn * 64 + 32 * g + 8 * lg;
+      const int n = wave * 64 + 32 * g + 8 * lg;
       if (n >= a.N) continue;
       float cs[8], bias[8];
 #pragma unroll
@@ -203,8 +198,8 @@ void i8_map_kernel(GemmArgs a, int tiles) {
         bias[e] = a.bias ? a.bias[c] : 0.f;
       }
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = wm * 64 + i * 16 + lr;
+      for (int i = 0; i < 2; ++i) {
+        const int r = i * 16 + lr;
         const long m = (long)tile * kMapRows + r;
         if (m >= a.M) continue;
         const float rs = ls[buf][r];
@@ -228,9 +223,7 @@ enum I8Way { W_FEW_FUSED, W_FEW, W_MAP, W_TILES };
 static I8Way i8_way(long M, int K, int N, bool gated) {
   if (M <= kQuantRows && K <= kQuantK && K % 16 == 0) return W_FEW_FUSED;
   if (M <= 64) return W_FEW;
-  // at least two row tiles a CU: 131072 x 256 x 256 takes 33 us against 51 of the quantiser and the tiled
-  // product; with fewer the CUs that stay empty cost more than the second launch
-  if (!gated && K <= kMapK && K % 16 == 0 && N <= kMapN && M >= 512 * kMapRows) return W_MAP;
+  if (!gated && K <= kMapK && K % 16 == 0 && N <= kMapN && M >= kMapMin && !route(HGK_ROUTE_FFN_TILE)) return W_MAP;
   return W_TILES;
 }
 
@@ -285,7 +278,7 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
     a.m0 = (const char*)x;
     if (way == W_MAP) {
       const int tiles = (int)((M + kMapRows - 1) / kMapRows);
-      hipLaunchKernelGGL((i8_map_kernel<T>), dim3(256), dim3(512), 0, st, a, tiles);
+      hipLaunchKernelGGL((i8_map_kernel<T>), dim3(std::min(tiles, kMapGroups)), dim3(256), 0, st, a, tiles);
     } else {
       hipLaunchKernelGGL((skinny_kernel<G_I8, T, 1, GATED, true>), dim3((unsigned)((N + 15) / 16)), dim3(512), 0, st, a);
     }

@@ -238,17 +238,17 @@ class _DropoutAdd(torch.autograd.Function):
     def forward(ctx, x, res, rows_per_mask, p, seed, offset, step):
         if step is not None:
             ctx.save_for_backward(step)
-        ctx.args = (rows_per_mask, p, seed, offset)
+        ctx.args = (rows_per_mask, p, seed, offset, step is not None)
         return _dropout(_dense(x), None if res is None else _dense(res), rows_per_mask, p, seed, offset, step)
 
     @staticmethod
     @_once
     def backward(ctx, dy):
-        saved = ctx.saved_tensors
-        dx = None
-        if ctx.needs_input_grad[0]:
-            dx = _dropout(_dense(dy), None, *ctx.args, saved[0] if saved else None)
-        return dx, dy if ctx.needs_input_grad[1] else None, None, None, None, None, None
+        rows_per_mask, p, seed, offset, has_step = ctx.args
+        step = ctx.saved_tensors[0] if has_step else None
+        of_x, of_res = ctx.needs_input_grad[:2]
+        dx = _dropout(_dense(dy), None, rows_per_mask, p, seed, offset, step) if of_x else None
+        return dx, dy if of_res else None, None, None, None, None, None
 
 
 def dropout_add(x, residual=None, p=0.5, seed=0, offset=0, step=None, rows_per_mask=1):
