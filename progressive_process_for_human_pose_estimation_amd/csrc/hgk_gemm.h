@@ -849,11 +849,11 @@ __global__ __launch_bounds__(256) void pad_rows_kernel(PadArgs a) {
   if (t >= a.chunks) return;
   const int k = a.n > 2 && t >= a.j[2].first ? 2 : a.n > 1 && t >= a.j[1].first ? 1 : 0;
   const PadJob& j = a.j[k];
-  const uint32_t cp = j.Kp / V;
-  const uint32_t l = (uint32_t)(t - j.first);  // host: a job's chunks are less than 2^32
-  const uint32_t r = l / cp;
+  const int cp = j.Kp / V;
+  const long l = t - j.first;
+  const long r = a.chunks >> 32 ? l / cp : (long)((uint32_t)l / (uint32_t)cp);
   const int c0 = (int)(l - r * cp) * V;
-  const char* src = j.src + ((long)r * j.K + c0) * (long)sizeof(E);
+  const char* src = j.src + (r * j.K + c0) * (long)sizeof(E);
   const int left = (j.K - c0) * (int)sizeof(E);  // bytes of the row from here on
   uint4 v = make_uint4(0, 0, 0, 0);
   auto take = [&](auto word) __attribute__((always_inline)) {

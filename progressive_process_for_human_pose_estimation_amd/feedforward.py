@@ -55,15 +55,14 @@ def _dense(t):
 
 
 def _check(what, x, k, *others):
-    """x [..., k] and the other operands: on one GPU, in x's type (None: any)"""
+    """x [..., k] and the other operands: on one device, each of its type"""
     if x.dim() < 1 or x.shape[-1] != k:
         raise H.HgkError(f"{what}: expected rows of {k} channels, got shape {tuple(x.shape)}")
+    device = x.device
     for t, dtype in others:
-        if t is None:
-            continue
-        if t.device != x.device:
-            raise H.HgkError(f"{what}: operands on {x.device} and {t.device}")
-        if t.dtype != dtype:
+        if t is not None and (t.dtype is not dtype or t.device != device):
+            if t.device != device:
+                raise H.HgkError(f"{what}: operands on {device} and {t.device}")
             raise H.HgkError(f"{what}: expected {dtype}, got {t.dtype}")
 
 
@@ -72,10 +71,10 @@ def _gpu(what, x):
         raise H.HgkError(f"{what}: tensors must live on the GPU")
 
 
-def _check_weights(what, *ws):
-    w = ws[0]
-    if w.dim() != 2 or w.shape[0] < 1 or w.shape[1] < 1 or any(v.shape != w.shape for v in ws):
-        raise H.HgkError(f"{what}: weights are [out, in], got {[tuple(v.shape) for v in ws]}")
+def _check_weights(what, w, v=None):
+    if w.dim() != 2 or 0 in w.shape or (v is not None and v.shape != w.shape):
+        raise H.HgkError(f"{what}: weights are [out, in], got {[tuple(t.shape) for t in (w, v) if t is not None]}")
+    return w.shape
 
 
 def _check_dropout(p, seed, offset, step, device):
@@ -87,8 +86,9 @@ def _check_dropout(p, seed, offset, step, device):
         raise H.HgkError(f"dropout: step is an int64 tensor of one element on {device}")
 
 
-def _grads(*ts):
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+def _grads(a, b, c=None):
+    return (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad)) \
+        and torch.is_grad_enabled()
 
 
 def _launch(x, fn, *args):

@@ -107,10 +107,10 @@ def philox(counter, key):
     return np.stack(c, 1)
 
 
-def kept(rows, C, p, seed, offset, rows_per_mask=1):
-    """bool [rows, C]"""
+def kept(rows, C, p, seed, offset, rows_per_mask=1, first=0):
+    """bool [rows, C], from mask row `first` on"""
     masks, groups = -(-rows // rows_per_mask), -(-C // 8)
-    gid = np.arange(masks * groups, dtype=np.uint64)
+    gid = np.arange(first * groups, (first + masks) * groups, dtype=np.uint64)
     offset %= 1 << 64
     c = np.stack([gid & np.uint64(0xFFFFFFFF), gid >> np.uint64(32),
                   np.full_like(gid, offset & 0xFFFFFFFF), np.full_like(gid, offset >> 32)], 1)

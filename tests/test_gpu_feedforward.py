@@ -475,6 +475,49 @@ def test_two_streams_at_once():
     assert all(torch.equal(u, v) for o in outs for u, v in zip(o, want))
 
 
+def test_offsets_past_32_bits():
+    """Tensors of more than 2^32 elements and more than 4 GB: the last rows against the oracle"""
+    M, C = (1 << 24) + 21, 264
+    x = torch.zeros(M, C, device=DEV, dtype=BF16)
+    x[-70:] = rnd(0, 70, C, dtype=BF16)
+    y = F.dropout_add(x, None, 0.3, 9, 2)
+    keep = R.kept(70, C, 0.3, 9, 2, first=M - 70).to(DEV)
+    R.worst(y[-70:], R.dropout_add(x[-70:].double(), None, keep, 0.3, BF16))
+    y = None
+    wg, wu = rnd(1, 8, C, dtype=BF16, scale=C ** -0.5), rnd(2, 8, C, dtype=BF16, scale=C ** -0.5)
+    h = F.gated_linear(x, wg, wu)
+    R.worst(h[-70:], R.gated(x[-70:].double(), wg.double(), wu.double(), "silu", BF16), "h")
+    w8, s8 = F.quantize_rows(wg)
+    z = F.linear_i8(x, w8, s8)
+    q, s = R.quantize(x[-70:])
+    v, e = (t.to(DEV) for t in R.product_i8(q, s, w8.cpu(), s8.cpu()))
+    R.worst(z[-70:], (v, e + R.U[BF16] * (v.abs() + e)))
+    h = z = None
+    # wide results from few channels, and their gradients
+    small = x[:, :8].contiguous()
+    w = rnd(3, C, 8, dtype=BF16).requires_grad_()
+    small.requires_grad_()
+    y = F.linear_dropout_add(small, w, None, 0.3, 9, 2)
+    want = R.linear(small[-70:].detach().double(), w.detach().double(), None, keep, 0.3, BF16, x[-70:].double())
+    R.worst(y[-70:].detach(), want[0], "y")
+    dx, dw = torch.autograd.grad(y, (small, w), x)  # the gradient of all rows but the last 70 is zero
+    R.worst(dx[-70:], want[1], "dx")
+    R.worst(dw, want[2], "dw")  # adding the other rows' zeros rounds nothing
+
+
+def test_dropout_in_place():
+    """The C entry's y may be x or the residual"""
+    for C, group in ((64, 1), (64, 7), (250, 1)):
+        x, res = rnd(0, 100, C), rnd(1, 100, C)
+        want = F.dropout_add(x, res, 0.4, 1, 2, rows_per_mask=group)
+        for y in (x, res):
+            a, b = x.clone(), res.clone()
+            out = a if y is x else b
+            H.check(H.lib().hgk_dropout_add(H.stream_handle(), H.F32, a.data_ptr(), b.data_ptr(), out.data_ptr(), 100, C,
+                                            group, 0.4, 1, 2, None))
+            assert torch.equal(out, want)
+
+
 def test_gpu_refusals():
     x, w = rnd(0, 4, 8), rnd(1, 6, 8)
     with pytest.raises(H.HgkError, match="operands on"):
