@@ -128,6 +128,7 @@ template <typename T>
 static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* wu, void* h, long M,
                      int C, int F, int act, char* ws, int dtype) {
   constexpr int DT = TypeOf<T>::dt;
+  if (gated_rows_ok(dtype, M, C, F)) return gated_rows_fwd(st, x, wg, wu, h, M, C, F, act);
   const GatedWs w = gated_ws(dtype, M, C, F, false);
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
@@ -154,16 +155,21 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
   const char *xp = a.m0, *wgp = a.n0, *wup = a.n1;
-  a.dh = dh;
-  a.out = ws + w.dg;
-  a.out1 = ws + w.du;
-  a.npad = w.Fp;
-  a.act = act;
-  a.vec = F % 8 == 0;
-  const GemmPlan p = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, F, 2, a.spseg, 1, false);
-  run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p);
-  HGK_LAUNCH_CHECK();
-  if (dx) {
+  const bool rows = dx && gated_rows_ok(dtype, M, C, F);
+  if (rows) {  // Fp is F, Cp is C
+    if (int rc = gated_rows_bwd(st, x, wg, wu, dh, dwg ? ws + w.dg : nullptr, ws + w.du, dx, M, C, F, act)) return rc;
+  } else {
+    a.dh = dh;
+    a.out = ws + w.dg;
+    a.out1 = ws + w.du;
+    a.npad = w.Fp;
+    a.act = act;
+    a.vec = F % 8 == 0;
+    const GemmPlan p = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, F, 2, a.spseg, 1, false);
+    run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p);
+    HGK_LAUNCH_CHECK();
+  }
+  if (dx && !rows) {
     GemmArgs b = gemm_args();
     b.m0 = ws + w.dg;
     b.m1 = ws + w.du;

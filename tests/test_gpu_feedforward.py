@@ -66,6 +66,46 @@ def test_gated_wide_tiles(M, C, Fh):
         R.worst(g, w, what)
 
 
+# wide maps of few channels: the row kernels, each channel class, ragged rows and columns, one chunk and many
+@pytest.mark.parametrize("M,C,Fh", [(16384, 8, 8), (16384 + 5, 64, 40), (16500, 72, 136), (20000, 128, 32), (16384 + 127, 136, 72),
+                                    (16385, 256, 264), (17000, 248, 1000)])
+@pytest.mark.parametrize("name", ["silu", "gelu", "relu", "sigmoid"])
+def test_gated_rows(M, C, Fh, name):
+    got, (x, wg, wu, dh) = gated_case(M, C, Fh, BF16, name, seed=7)
+    want = R.gated(*(v.detach().double() for v in (x, wg, wu)), name, BF16, dh.double())
+    for g, w, what in zip(got, want, ("h", "dx", "dw_gate", "dw_up")):
+        R.worst(g, w, what)
+
+
+def test_gated_rows_one_gradient_at_a_time():
+    _, (x, wg, wu, dh) = gated_case(16400, 128, 72, BF16, "silu")
+    both = torch.autograd.grad(F.gated_linear(x, wg, wu), (x, wg, wu), dh)
+    dx, = torch.autograd.grad(F.gated_linear(x, wg.detach(), wu.detach()), x, dh)
+    dwg, dwu = torch.autograd.grad(F.gated_linear(x.detach(), wg, wu), (wg, wu), dh)
+    assert torch.equal(dx, both[0])
+    want = R.gated(*(v.detach().double() for v in (x, wg, wu)), "silu", BF16, dh.double())
+    for g, w in ((dx, want[1]), (dwg, want[2]), (dwu, want[3])):
+        R.worst(g, w)
+
+
+def test_gated_rows_infinite_weights_and_rows_stay_in_place():
+    x, wg, wu = rnd(0, 16400, 64, dtype=BF16), rnd(1, 40, 64, dtype=BF16), rnd(2, 40, 64, dtype=BF16)
+    clean = F.gated_linear(x, wg, wu)
+    x[3, 5], x[16399, 63] = float("inf"), float("nan")
+    wg[39, 0] = float("inf")  # the last row of the weights, in a chunk that is not full
+    h = F.gated_linear(x, wg, wu)
+    rest = torch.tensor([i for i in range(16400) if i not in (3, 16399)], device=DEV)
+    assert torch.equal(h[rest][:, :39], clean[rest][:, :39])
+    xg = x.clone()
+    xg[3, 5], xg[16399, 63] = 0, 0
+    xg.requires_grad_()
+    dh = rnd(3, 16400, 40, dtype=BF16)
+    dh[:, 39] = 0
+    wg[39, 0] = 1.0
+    dx, = torch.autograd.grad(F.gated_linear(xg, wg, wu), xg, dh)
+    assert bool(dx.isfinite().all())
+
+
 # every tile size on sizes that do not fill it, one step of k and several, k past the ring's depth
 @pytest.mark.parametrize("tile", [64, 128, 256])
 @pytest.mark.parametrize("M,C,Fh", [(65, 8, 9), (300, 72, 40), (129, 33, 257), (700, 264, 300), (1000, 520, 129)])
