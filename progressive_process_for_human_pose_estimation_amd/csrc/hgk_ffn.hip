@@ -128,7 +128,7 @@ template <typename T>
 static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* wu, void* h, long M,
                      int C, int F, int act, char* ws, int dtype) {
   constexpr int DT = TypeOf<T>::dt;
-  if (gated_rows_ok(dtype, M, C, F)) return gated_rows_fwd(st, x, wg, wu, h, M, C, F, act);
+  if (gated_rows_ok(dtype, M, C, F, false)) return gated_rows_fwd(st, x, wg, wu, h, M, C, F, act);
   const GatedWs w = gated_ws(dtype, M, C, F, false);
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
@@ -155,7 +155,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
   const char *xp = a.m0, *wgp = a.n0, *wup = a.n1;
-  const bool rows = dx && gated_rows_ok(dtype, M, C, F);
+  const bool rows = dx && gated_rows_ok(dtype, M, C, F, true);
   if (rows) {  // Fp is F, Cp is C
     if (int rc = gated_rows_bwd(st, x, wg, wu, dh, dwg ? ws + w.dg : nullptr, ws + w.du, dx, M, C, F, act)) return rc;
   } else {

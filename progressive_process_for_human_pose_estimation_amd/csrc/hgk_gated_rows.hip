@@ -1,17 +1,27 @@
-// The gated product of wide maps of few channels (bf16, C <= 256: the pixel levels), forward, and its
-// backward up to dg, du AND dx, one pass over the rows each.
+// The gated product of wide maps of few channels (bf16: the pixel levels), forward (C <= 128), and its
+// backward up to dg, du AND dx (C <= 256), one pass over the rows each.
 //
 // The hidden width F is walked in chunks of 32: a wave holds 16 rows of x in registers for all of it, the
-// chunk's 32 gate and 32 up rows of the weights stand in LDS (a ring of three, LDS-DMA), and per chunk
+// chunk's 32 gate and 32 up rows of the weights stand in LDS (a ring of four, LDS-DMA), and per chunk
 //   g, u = x Wg^T, x Wu^T          (the chunk's columns, 8 consecutive of one row a lane)
 //   forward:   h = a(g) u, stored
 //   backward:  dg = dh u a'(g), du = dh a(g), rounded to bf16 and stored for the weight gradients;
 //              dx += dg Wg + du Wu: what a lane holds of dg and du IS the matrix instruction's operand
 //              (row = lane % 16, k = 8 (lane / 16) ..), and the weights are the same LDS tile, read as
 //              transposed fragments. dg and du are not read back for dx.
-// Against the tiled products (hgk_gemm.h), which for K = C = 256 spend half of their time between the
-// products of one tile and the next: activations and stores of one wave run beside the products of the
-// other on its SIMD all the way.
+// Against the tiled products (hgk_gemm.h), which at K = C <= 256 spend half of their time between the
+// products of one tile and the next: two waves share a SIMD, half a chunk apart, and the activations and
+// stores of one run beside the products of the other all the way. What bounds it: LDS reads (each wave reads
+// the whole chunk for its 16 rows) at C = 256, the stores of h, dg and du at C <= 128.
+//
+// Measured, us, rows here / best tile (F = 4 C; backward up to dx):
+//   C    M = 16384              24576                 32768                 40000
+//   64   f 7.9/6.4  b 11/17     f 8.4/9.1  b 12/24    f 8.7/9.7  b 13/27    f 11/13    b 18/32
+//   128  f 15/11    b 27/32     f 15/17    b 29/40    f 18/19    b 32/49    f 24/26    b 51/59
+//   192  f 28/19    b 52/49     f 30/28    b 53/67    f 35/31    b 57/82    f 54/39    b 98/103
+//   256  f 36/24    b 65/63     f 41/35    b 66/91    f 46/46    b 84/121   f 73/57    b 130/148
+// and at M = 131072, C = 128: forward 59 / 77, backward 143 / 202. A workgroup takes 128 rows, so 16384 are half
+// of the card's CUs. Hence gated_rows_ok().
 #include "hgk_gemm.h"
 
 namespace hgk {
@@ -228,8 +238,10 @@ void gated_rows_kernel(RowsArgs a) {
   }
 }
 
-bool gated_rows_ok(int dtype, long M, int C, int F) {
-  return dtype == HGK_BF16 && C <= 256 && C % 8 == 0 && F % 8 == 0 && M >= kGatedRows && !route(HGK_ROUTE_FFN_TILE);
+bool gated_rows_ok(int dtype, long M, int C, int F, bool bwd) {
+  if (dtype != HGK_BF16 || C % 8 != 0 || F % 8 != 0 || route(HGK_ROUTE_FFN_TILE)) return false;
+  if (C <= 128) return M >= (bwd ? 16384 : 24576);
+  return bwd && C <= 256 && M >= 24576;
 }
 
 template <bool BWD, int ACT>
@@ -237,7 +249,7 @@ static void launch_rows_act(hipStream_t st, const RowsArgs& a) {
   const dim3 grid((unsigned)((a.M + 127) / 128));
   if (a.C <= 64) hipLaunchKernelGGL((gated_rows_kernel<2, BWD, ACT>), grid, dim3(512), 0, st, a);
   else if (a.C <= 128) hipLaunchKernelGGL((gated_rows_kernel<4, BWD, ACT>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((gated_rows_kernel<8, BWD, ACT>), grid, dim3(512), 0, st, a);
+  else if constexpr (BWD) hipLaunchKernelGGL((gated_rows_kernel<8, true, ACT>), grid, dim3(512), 0, st, a);
 }
 template <bool BWD>
 static int launch_rows(hipStream_t st, const RowsArgs& a) {

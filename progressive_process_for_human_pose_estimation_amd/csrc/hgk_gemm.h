@@ -887,9 +887,8 @@ static __global__ __launch_bounds__(256) void zero_kernel(uint32_t* p, long word
 // hgk_dropout.hip
 int dropout_mask(hipStream_t st, int dtype, const void* dy, void* dz, long rows, int C, const DropArgs& d);
 
-// hgk_gated_rows.hip: the gated product of at least kGatedRows rows of few channels
-static constexpr long kGatedRows = 16384;
-bool gated_rows_ok(int dtype, long M, int C, int F);
+// hgk_gated_rows.hip: the gated product of many rows of few channels
+bool gated_rows_ok(int dtype, long M, int C, int F, bool bwd);
 int gated_rows_fwd(hipStream_t st, const void* x, const void* wg, const void* wu, void* h, long M, int C, int F, int act);
 int gated_rows_bwd(hipStream_t st, const void* x, const void* wg, const void* wu, const void* dh, void* dg, void* du,
                    void* dx, long M, int C, int F, int act);

@@ -68,7 +68,8 @@ def test_gated_wide_tiles(M, C, Fh):
 
 # wide maps of few channels: the row kernels, each channel class, ragged rows and columns, one chunk and many
 @pytest.mark.parametrize("M,C,Fh", [(16384, 8, 8), (16384 + 5, 64, 40), (16500, 72, 136), (20000, 128, 32), (16384 + 127, 136, 72),
-                                    (16385, 256, 264), (17000, 248, 1000)])
+                                    (16385, 256, 264), (17000, 248, 1000), (24576, 8, 16), (24577, 64, 40),
+                                    (24700, 128, 136), (24576 + 127, 136, 72), (24580, 256, 264)])
 @pytest.mark.parametrize("name", ["silu", "gelu", "relu", "sigmoid"])
 def test_gated_rows(M, C, Fh, name):
     got, (x, wg, wu, dh) = gated_case(M, C, Fh, BF16, name, seed=7)
@@ -78,7 +79,7 @@ def test_gated_rows(M, C, Fh, name):
 
 
 def test_gated_rows_one_gradient_at_a_time():
-    _, (x, wg, wu, dh) = gated_case(16400, 128, 72, BF16, "silu")
+    _, (x, wg, wu, dh) = gated_case(24600, 128, 72, BF16, "silu")
     both = torch.autograd.grad(F.gated_linear(x, wg, wu), (x, wg, wu), dh)
     dx, = torch.autograd.grad(F.gated_linear(x, wg.detach(), wu.detach()), x, dh)
     dwg, dwu = torch.autograd.grad(F.gated_linear(x.detach(), wg, wu), (wg, wu), dh)
@@ -89,17 +90,17 @@ def test_gated_rows_one_gradient_at_a_time():
 
 
 def test_gated_rows_infinite_weights_and_rows_stay_in_place():
-    x, wg, wu = rnd(0, 16400, 64, dtype=BF16), rnd(1, 40, 64, dtype=BF16), rnd(2, 40, 64, dtype=BF16)
+    x, wg, wu = rnd(0, 24600, 64, dtype=BF16), rnd(1, 40, 64, dtype=BF16), rnd(2, 40, 64, dtype=BF16)
     clean = F.gated_linear(x, wg, wu)
-    x[3, 5], x[16399, 63] = float("inf"), float("nan")
+    x[3, 5], x[24599, 63] = float("inf"), float("nan")
     wg[39, 0] = float("inf")  # the last row of the weights, in a chunk that is not full
     h = F.gated_linear(x, wg, wu)
-    rest = torch.tensor([i for i in range(16400) if i not in (3, 16399)], device=DEV)
+    rest = torch.tensor([i for i in range(24600) if i not in (3, 24599)], device=DEV)
     assert torch.equal(h[rest][:, :39], clean[rest][:, :39])
     xg = x.clone()
-    xg[3, 5], xg[16399, 63] = 0, 0
+    xg[3, 5], xg[24599, 63] = 0, 0
     xg.requires_grad_()
-    dh = rnd(3, 16400, 40, dtype=BF16)
+    dh = rnd(3, 24600, 40, dtype=BF16)
     dh[:, 39] = 0
     wg[39, 0] = 1.0
     dx, = torch.autograd.grad(F.gated_linear(xg, wg, wu), xg, dh)
