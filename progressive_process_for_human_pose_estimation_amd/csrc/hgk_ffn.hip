@@ -234,7 +234,7 @@ static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) 
     w.dw = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, N, K, 1, (int)((M + ks - 1) / ks), 1, true);
     w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
   } else {
-    w.slab = c.take(w.fwd.slab);
+    w.slab = c.take(M <= kSkinnyRows ? 0 : w.fwd.slab);
   }
   w.total = c.at;
   return w;

@@ -19,7 +19,8 @@ again. An element is dropped with probability p to the nearest 2^-16 and the res
 inverse of the probability that is kept. The same (seed, offset) gives the same mask: pass another
 offset for each use. `step`, an int64 GPU tensor of one element, is added to the offset on the
 device, so that a captured graph draws other masks at each replay; it must not change between a
-forward and its backward. Everything here can be captured; there is no CPU fallback.
+forward and its backward. Everything here can be captured (a backward together with its forward, on
+leaves of which no eager graph is alive); there is no CPU fallback.
 """
 import math
 
@@ -341,32 +342,36 @@ def gated_linear_i8(x, w_gate, gate_scale, w_up, up_scale, activation="silu"):
 
 # ---- modules ----
 class _Masks(nn.Module):
-    """The (seed, offset, step) of a module's dropout. The seed is drawn from torch's generator at
-    construction (torch.manual_seed governs it); every training call takes the next offset. Under
-    graph capture the host's offset is frozen, so a device counter moves on at each replay and the
-    call keeps the value that it saw for its backward."""
+    """The (seed, offset, step) of a module's dropout. The seed is drawn from torch's CPU generator at
+    construction and the offset in every training call, so that torch.manual_seed governs the masks and
+    torch.utils.checkpoint, which puts the generator back, draws the same ones again. `offset` keeps
+    the last one. Under graph capture the host's offset is frozen, so a device counter moves on at each
+    replay and the call keeps the value that it saw for its backward."""
 
     def __init__(self, p):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise H.HgkError(f"dropout: p = {p} is no probability")
         self.p = p
-        self.seed = int(torch.randint(0, 2 ** 62, (1,)).item())
-        self.calls = 0
+        self.seed, self.offset = self._draw(), 0
         self.register_buffer("step", torch.zeros(1, dtype=torch.int64), persistent=False)
+
+    @staticmethod
+    def _draw():
+        return int(torch.randint(0, 1 << 62, (1,), device="cpu").item())
 
     def next_mask(self, x):
         """keyword arguments of the next use, on x's device"""
         if not self.training or self.p == 0.0:
             return {"p": 0.0}
-        self.calls = (self.calls + 1) & 0xffffffff
+        self.offset = self._draw()
         step = None
         if x.is_cuda and torch.cuda.is_current_stream_capturing():
             if self.step.device != x.device:
                 raise H.HgkError(f"dropout: move the module to {x.device} before capturing it")
             self.step.add_(1 << 32)
             step = self.step.clone()
-        return {"p": self.p, "seed": self.seed, "offset": self.calls, "step": step}
+        return {"p": self.p, "seed": self.seed, "offset": self.offset, "step": step}
 
 
 class Dropout(_Masks):
@@ -424,6 +429,15 @@ class GatedFeedForwardI8(nn.Module):
             q, s = quantize_rows(getattr(block, "w_" + name).detach())
             self.register_buffer("w_" + name, q)
             self.register_buffer(name + "_scale", s)
+
+    def _apply(self, fn, *args, **kwargs):
+        # .to(dtype), .bfloat16() and the like: the scales stay fp32, whatever they are moved to
+        scales = {n: getattr(self, n) for n in ("gate_scale", "up_scale", "down_scale")}
+        super()._apply(fn, *args, **kwargs)
+        for n, s in scales.items():
+            if getattr(self, n).dtype is not s.dtype:
+                setattr(self, n, s.to(getattr(self, n).device))
+        return self
 
     @torch.no_grad()
     def forward(self, x):

@@ -3,6 +3,7 @@ oracle against published vectors and differences."""
 import numpy as np
 import pytest
 import torch
+from torch.utils.checkpoint import checkpoint
 
 import feedforward_oracle as R
 from progressive_process_for_human_pose_estimation_amd import feedforward as F
@@ -152,3 +153,21 @@ def test_module_masks_advance_and_follow_the_seed():
     assert len({v["offset"] for v in m}) == 3 and all(v["seed"] == a.seed for v in m)
     assert a.eval().next_mask(t(2, 8)) == {"p": 0.0}
     assert set(a.state_dict()) == {"w_gate", "w_up", "w_down"}
+
+
+def test_module_masks_are_drawn_again_by_a_checkpoint():
+    d, seen = F.Dropout(0.5), []
+
+    def part(x):
+        seen.append(d.next_mask(x)["offset"])
+        return x.sin()
+
+    for _ in range(2):
+        checkpoint(part, torch.ones(3, requires_grad=True), use_reentrant=False).sum().backward()
+    assert len(seen) == 4 and seen[0] == seen[1] and seen[2] == seen[3] and seen[0] != seen[2]
+
+
+def test_module_masks_do_not_follow_the_default_device():
+    with torch.device("meta"):
+        d = F.Dropout(0.5)
+        assert d.next_mask(t(2, 8))["offset"] == d.offset
