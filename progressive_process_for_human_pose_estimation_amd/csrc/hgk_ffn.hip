@@ -283,7 +283,12 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
   const LinearWs w = linear_ws(dtype, M, K, N, drop, true);
   const char *dz = (const char*)dy, *xp = (const char*)x, *wp = (const char*)wt;
   Pads p;
-  if (w.pad_n) {
+  const bool rows = dx && linear_rows_ok(dtype, M, K, N, drop);
+  if (rows) {  // nothing to pad
+    void* z = drop && dw ? ws + w.dz : nullptr;
+    if (int rc = linear_rows_bwd(st, dy, wt, z, dx, M, K, N, d)) return rc;
+    if (drop) dz = ws + w.dz;
+  } else if (w.pad_n) {
     p.add(dy, ws + w.dz, M, N, w.Np, es, drop ? &d : nullptr);
     dz = ws + w.dz;
   } else if (drop) {
@@ -299,7 +304,7 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
   p.launch<raw>(st);
   HGK_LAUNCH_CHECK();
   const float alpha = drop ? d.scale : 1.f;
-  if (dx) {
+  if (dx && !rows) {
     GemmArgs b = gemm_args();
     b.m0 = dz;
     b.ldm = (long)w.Np * es;

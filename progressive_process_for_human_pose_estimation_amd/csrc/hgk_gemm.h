@@ -893,6 +893,11 @@ int gated_rows_fwd(hipStream_t st, const void* x, const void* wg, const void* wu
 int gated_rows_bwd(hipStream_t st, const void* x, const void* wg, const void* wu, const void* dh, void* dg, void* du,
                    void* dx, long M, int C, int F, int act);
 
+// hgk_linear_rows.hip: dz and dx of many rows of few output channels
+bool linear_rows_ok(int dtype, long M, int K, int N, bool drop);
+int linear_rows_bwd(hipStream_t st, const void* dy, const void* w, void* dz, void* dx, long M, int K, int N,
+                    const DropArgs& d);
+
 static inline long up_to(long n, long q) { return (n + q - 1) / q * q; }
 
 // collects the rows to pad, then one launch

@@ -200,6 +200,35 @@ def test_linear_wide_tiles(M, K, N):
         R.worst(g, v, what)
 
 
+# wide maps of few output channels: the row kernel of the input gradient, each channel class, ragged
+# rows, one chunk of columns and many
+@pytest.mark.parametrize("M,K,N", [(24576, 8, 8), (24576 + 5, 64, 64), (24700, 136, 72), (25000, 40, 128), (24576 + 127, 72, 136),
+                                   (24577, 264, 256), (25000, 1000, 248)])
+@pytest.mark.parametrize("p", [0.0, 0.2])
+def test_linear_rows(M, K, N, p):
+    x, w = rnd(1, M, K, dtype=BF16).requires_grad_(), rnd(2, N, K, dtype=BF16, scale=K ** -0.5).requires_grad_()
+    res, dy = rnd(3, M, N, dtype=BF16), rnd(4, M, N, dtype=BF16)
+    y = F.linear_dropout_add(x, w, res, p, seed=5, offset=6)
+    got = (y.detach(), *torch.autograd.grad(y, (x, w), dy))
+    want = R.linear(x.detach().double(), w.detach().double(), res.double(), R.kept(M, N, p, 5, 6).to(DEV), p, BF16, dy.double())
+    for g, v, what in zip(got, want, ("y", "dx", "dw")):
+        R.worst(g, v, what)
+    dx, = torch.autograd.grad(F.linear_dropout_add(x, w.detach(), res, p, seed=5, offset=6), x, dy)
+    assert torch.equal(dx, got[1])
+
+
+def test_linear_rows_dropped_infinities_vanish():
+    M, K, N = 24600, 72, 40
+    x, w, dy = rnd(1, M, K, dtype=BF16).requires_grad_(), rnd(2, N, K, dtype=BF16), rnd(4, M, N, dtype=BF16)
+    clean, = torch.autograd.grad(F.linear_dropout_add(x, w, None, 0.3, 5, 6), x, dy)
+    keep = R.kept(M, N, 0.3, 5, 6).to(DEV)
+    bad = torch.where(keep, dy, torch.full_like(dy, float("inf")))
+    bad[7] = float("nan")
+    dx, = torch.autograd.grad(F.linear_dropout_add(x, w, None, 0.3, 5, 6), x, bad)
+    rest = torch.tensor([i for i in range(M) if i != 7], device=DEV)
+    assert torch.equal(dx[rest], clean[rest]) and bool(dx[7].isnan().all())
+
+
 def test_linear_all_dropped_is_the_residual():
     x, w, res = rnd(0, 70, 24), rnd(1, 10, 24), rnd(2, 70, 10)
     assert torch.equal(F.linear_dropout_add(x, w, res, 1.0), res)
