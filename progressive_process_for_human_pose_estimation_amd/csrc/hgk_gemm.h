@@ -941,10 +941,13 @@ struct GemmPlan {
 // 1.5 us of a CU in bf16 (1467 TFLOP/s over the chip at 8192 x 4096 x 8192); per unit of work a
 // 128-wide tile takes 1.3 times that (1147), a 64-wide one 2 to 3 times (502 .. 704): its waves read
 // twice to four times the fragments per product. fp32's matrix instructions are 16 times slower and
-// hide all of that. A CU with one or two workgroups waits for memory instead: 0.8 us
-// a step and half its products. A round ends with its epilogue, 4 us of a 256-wide tile. Against the
-// tile stand the rounds: tiles are dealt to 256 CUs whole. Splitting k costs the partial sums' way to
-// memory and back (4.5 TB/s) and a second launch (5 us).
+// hide all of that. A CU with one or two workgroups waits for memory instead: 0.16 us and 0.8 of its
+// products a step. A round ends with its epilogue, 4 us of a 256-wide tile. Against the tile stand the
+// rounds: tiles are dealt to 256 CUs whole. Splitting k costs the partial sums' way to memory and back
+// (4.6 TB/s) and a second launch (4.7 us). The constants of waiting and splitting are fitted to 29 weight
+// gradients (64 x 256 .. 2048 x 512 over 2000 .. 131072 rows, all tiles, 4 to 256 splits): what they choose
+// is 1 % slower on average than the best of each (256 x 1024 over 32768 rows: 30.7 us in 16 splits of
+// 128-wide tiles, 35.6 in 32, 38.6 in 64-wide tiles).
 static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int batch, bool can_split) {
   GemmPlan best;
   double least = 1e30;
@@ -962,8 +965,8 @@ static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int
     for (int split = 1; split <= 64; split *= 2) {
       if (split > 1 && (!can_split || n * split > slots || steps / split < 4)) break;
       const double rounds = (double)((n * split + 255) / 256), each = (double)((steps + split - 1) / split);
-      double t = std::max(rounds * step, 0.8 + 0.5 * step) * each + rounds * 4.0 * b * b / 65536;
-      if (split > 1) t += 5 + 8.0 * split * batch * M * N / 4.5e6;
+      double t = std::max(rounds * step, 0.16 + 0.8 * step) * each + rounds * 4.0 * b * b / 65536;
+      if (split > 1) t += 4.7 + 8.0 * split * batch * M * N / 4.6e6;
       if (t < least) {
         least = t;
         best = p;
