@@ -32,14 +32,26 @@ static int run_product(hipStream_t st, GemmArgs& a, const GemmPlan& p, char* sla
   return HGK_OK;
 }
 
+// Up to this many rows stream the weights (skinny_kernel), more take tiles. The linear's tiles can split k, so
+// they take over early. Measured, us, rows / tiles: bf16 gated 1024 -> 4096: 6.1 at 32, 6.9 at 33 / 6.4; linear
+// 4096 -> 1024: 9.4 at 16, 10.5 at 17 / 9.0 (1024 -> 256: 4.2, 4.6, 5.3 at 32 / 6.8); fp32 gated: 17.7 at 64 /
+// 22.1, linear 16.6 at 16, 23.7 at 32 / 16.3.
+template <typename T>
+static constexpr int skinny_rows(bool dual) {
+  return !dual ? 16 : sizeof(T) == 2 ? 32 : 64;
+}
 template <int DT, typename T, bool DUAL>
 static void run_skinny(hipStream_t st, const GemmArgs& a) {
+  constexpr int most = skinny_rows<T>(DUAL);
   const dim3 grid((unsigned)((a.N + 15) / 16));
   if (a.M <= 16) hipLaunchKernelGGL((skinny_kernel<DT, T, 1, DUAL>), grid, dim3(512), 0, st, a);
-  else if (a.M <= 32) hipLaunchKernelGGL((skinny_kernel<DT, T, 2, DUAL>), grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL((skinny_kernel<DT, T, 4, DUAL>), grid, dim3(512), 0, st, a);
+  if constexpr (most > 16) {
+    if (a.M > 16 && a.M <= 32) hipLaunchKernelGGL((skinny_kernel<DT, T, 2, DUAL>), grid, dim3(512), 0, st, a);
+  }
+  if constexpr (most > 32) {
+    if (a.M > 32) hipLaunchKernelGGL((skinny_kernel<DT, T, 4, DUAL>), grid, dim3(512), 0, st, a);
+  }
 }
-static constexpr int kSkinnyRows = 64;
 
 template <typename T>
 struct TypeOf;
@@ -135,7 +147,7 @@ static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* 
   a.out = h;
   a.act = act;
   a.vec = F % 8 == 0;
-  if (M <= kSkinnyRows) {
+  if (M <= skinny_rows<T>(true)) {
     run_skinny<DT, T, true>(st, a);
   } else {
     const GemmPlan p = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, F, 2, a.spseg, 1, false);
@@ -234,7 +246,7 @@ static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) 
     w.dw = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, N, K, 1, (int)((M + ks - 1) / ks), 1, true);
     w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
   } else {
-    w.slab = c.take(M <= kSkinnyRows ? 0 : w.fwd.slab);
+    w.slab = c.take(M <= skinny_rows<float>(false) ? 0 : w.fwd.slab);  // the same for every type
   }
   w.total = c.at;
   return w;
@@ -265,7 +277,7 @@ static int linear_fwd(hipStream_t st, const void* x, const void* wt, const void*
   a.vec = N % 8 == 0;
   a.drop = d.thr != 0;
   a.d = d;
-  if (M <= kSkinnyRows) {
+  if (M <= skinny_rows<T>(false)) {
     run_skinny<DT, T, false>(st, a);
     HGK_LAUNCH_CHECK();
     return HGK_OK;

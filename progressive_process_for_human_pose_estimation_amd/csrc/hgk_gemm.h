@@ -237,6 +237,12 @@ __device__ __forceinline__ void store8(T* p, int n, int N, bool vec, const float
       if (n + e < N) p[n + e] = from_f<T>(f[e]);
   }
 }
+// a + b that no product before it is fused into: the kernels of the 8-bit products round alike, so a row's
+// result does not depend on the rows beside it
+__device__ __forceinline__ float plus(float a, float b) {
+#pragma clang fp contract(off)
+  return a + b;
+}
 // dropout of the 8 outputs of one group of row m
 __device__ __forceinline__ void drop8(const GemmArgs& a, int m, int n, float* f, uint64_t off) {
   const uint64_t gid = (uint64_t)m * ((a.N + 7) >> 3) + (n >> 3);
@@ -696,15 +702,15 @@ __device__ __forceinline__ float quant_row(const T* row, int8_t* q, int K, int l
 // A workgroup owns 16 output columns (gated: 16 gate and 16 up), its 8 waves take every 8th K-step
 // of 128 bytes, the partial sums meet in LDS in wave order. Bound by the weights' bytes: one
 // column group of 16 rows x 128 bytes per load pair, M rows of x from the caches.
-// QUANT (8-bit integers, M <= kQuantRows, K <= kQuantK): x is T, and every workgroup quantises its few rows
-// into LDS itself, in place of a launch and a trip through memory.
-static constexpr int kQuantRows = 4, kQuantK = 8192;
+// QUANT (8-bit integers, M <= kQuantRows, M K <= kQuantBytes): x is T, and every workgroup quantises its few
+// rows into LDS itself, in place of a launch and a trip through memory.
+static constexpr int kQuantRows = 16, kQuantBytes = 32768;
 template <int DT, typename T, int MT, bool DUAL, bool QUANT = false>
 __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
   constexpr int es = GT<DT>::es, P = DUAL ? 2 : 1, NW = 8;
   typedef typename GT<DT>::acc acc_t;
   __shared__ acc_t red[NW][P * MT][64];
-  __shared__ __attribute__((aligned(16))) int8_t xq[QUANT ? kQuantRows * kQuantK : 16];
+  __shared__ __attribute__((aligned(16))) int8_t xq[QUANT ? kQuantBytes : 16];
   __shared__ float xs[QUANT ? kQuantRows : 1];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
   const int n0 = blockIdx.x * 16;
@@ -715,9 +721,9 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
 #pragma unroll
   for (int i = 0; i < MT; ++i) x[i] = a.m0 + (long)min(i * 16 + lr, a.M - 1) * a.ldm;
   if constexpr (QUANT) {
-    if (wave < a.M) {
-      const float sc = quant_row<T>((const T*)a.m0 + (long)wave * a.km, xq + wave * a.km, a.km, lane);
-      if (lane == 0) xs[wave] = sc;
+    for (int r = wave; r < a.M; r += NW) {
+      const float sc = quant_row<T>((const T*)a.m0 + (long)r * a.km, xq + r * a.km, a.km, lane);
+      if (lane == 0) xs[r] = sc;
     }
     __syncthreads();
   }
@@ -787,9 +793,9 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
     const long at = (long)m * a.N + n + e;
     float v = f[0][e];
     if constexpr (!DUAL) {
-      if (a.bias) v += a.bias[n + e];
+      if (a.bias) v = plus(v, a.bias[n + e]);
       if (a.drop) v = (keep >> e) & 1u ? v * a.d.scale : 0.f;
-      if (a.res) v += to_f(((const T*)a.res)[at]);
+      if (a.res) v = plus(v, to_f(((const T*)a.res)[at]));
     }
     ((T*)a.out)[at] = from_f<T>(v);
   }

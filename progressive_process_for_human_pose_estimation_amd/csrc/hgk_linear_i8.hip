@@ -99,14 +99,14 @@ static void launch_quant(hipStream_t st, const void* x, int8_t* q, float* s, lon
     launch_quant_as<T, false>(st, (const T*)x, q, s, rows, K, Kp);
 }
 
-// ---- wide maps of few channels (K <= 256, N <= 256: the pointwise products of the pixel levels) ----
+// ---- few channels (K <= 256, N <= 256: the pointwise products of the pixel levels) ----
 // A wave keeps its 64 columns of the weights in registers, a workgroup of 4 waves walks 32-row tiles: a
 // tile's rows are read once as T, quantised in registers (8 lanes a row) and written to LDS as bytes, so
 // the quantised rows never go through memory: 4 bytes an element of x and y in all. The next tile is on
 // its way from memory while this one's products run. Two workgroups a CU: the quantising and the
 // epilogue of one (18 us of VALU at 131072 x 256 x 256) run beside the memory of the other; one
 // workgroup of 8 waves with the weights in LDS took 45 us, one phase after the other.
-static constexpr int kMapK = 256, kMapN = 256, kMapRows = 32, kMapGroups = 512, kMapMin = 16384;
+static constexpr int kMapK = 256, kMapN = 256, kMapRows = 32, kMapGroups = 512;
 template <typename T>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2)))
 void i8_map_kernel(GemmArgs a, int tiles) {
@@ -205,12 +205,12 @@ void i8_map_kernel(GemmArgs a, int tiles) {
         const float rs = ls[buf][r];
         float f[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) f[e] = (float)acc[2 * g + (e >> 2)][i][e & 3] * rs * cs[e] + bias[e];
+        for (int e = 0; e < 8; ++e) f[e] = plus((float)acc[2 * g + (e >> 2)][i][e & 3] * rs * cs[e], bias[e]);
         if (a.res) {
           float q[8];
           load8<T>((const T*)a.res + m * a.N, n, a.N, a.vec, q);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) f[e] += q[e];
+          for (int e = 0; e < 8; ++e) f[e] = plus(f[e], q[e]);
         }
         store8<T>((T*)a.out + m * a.N, n, a.N, a.vec, f);
       }
@@ -218,12 +218,20 @@ void i8_map_kernel(GemmArgs a, int tiles) {
   }
 }
 
-// which kernel a call takes, and what it needs
+// Which kernel a call takes, and what it needs. Measured, us, this way / the other:
+//   rows quantised by the product's workgroups / by a launch of their own (bf16, gated 1024 -> 4096): 4.7 / 6.1 at
+//     5 rows, 4.8 / 6.2 at 8; 256 -> 1024 4.3 / 5.3 at 16. 32 KB of quantised rows leave LDS for three
+//     workgroups a CU.
+//   few channels: the map kernel / the best of quantising launch + tiles (256 x 256 bf16): 5.8 / 6.7 at 65 rows, 6.6
+//     / 9.4 at 8192, 13.7 / 19.9 at 32768, 35 / 46 at 131072; fp32 6.4 / 6.6, 8.1 / 10, 19 / 21, 64 / 65 (256 ->
+//     64 in fp32 at 131072 the other way: 46 / 40). Up to 64 rows against the weight-streaming kernel: 5.8 / 6.2
+//     in bf16, 6.4 / 6.0 in fp32 at 64, 5.6 / 5.2 and 6.2 / 5.0 at 17.
+//   weight-streaming / tiles (bf16, gated 1024 -> 4096): 8.6 at 64 rows / 8.4 at 65; linear 4096 -> 1024 17 / 18.
 enum I8Way { W_FEW_FUSED, W_FEW, W_MAP, W_TILES };
 static I8Way i8_way(long M, int K, int N, bool gated) {
-  if (M <= kQuantRows && K <= kQuantK && K % 16 == 0) return W_FEW_FUSED;
+  if (M <= kQuantRows && M * K <= kQuantBytes && K % 16 == 0) return W_FEW_FUSED;
   if (M <= 64) return W_FEW;
-  if (!gated && K <= kMapK && K % 16 == 0 && N <= kMapN && M >= kMapMin && !route(HGK_ROUTE_FFN_TILE)) return W_MAP;
+  if (!gated && K <= kMapK && K % 16 == 0 && N <= kMapN && !route(HGK_ROUTE_FFN_TILE)) return W_MAP;
   return W_TILES;
 }
 

@@ -297,7 +297,8 @@ def test_expanded_input_gradient():
 # ---- 8-bit integers ----
 I8 = [(1, 8, 8), (1, 1, 1), (2, 17, 5), (16, 1000, 40), (17, 64, 129), (64, 130, 16), (65, 128, 128), (200, 257, 66),
       (333, 96, 515), (8192 + 5, 48, 2064), (20, 5000, 24), (4, 20000, 8),
-      (1, 8192, 33), (4, 16, 7), (3, 4096, 100), (4, 8208, 20),              # rows quantised by each workgroup
+      (1, 8192, 33), (4, 16, 7), (3, 4096, 100), (4, 8208, 20), (4, 8192, 24), (16, 2048, 24), (16, 2064, 24),
+      (1, 32768, 20), (1, 32784, 20), (9, 3632, 40),  # rows quantised by each workgroup
       (65536 + 3, 256, 256), (65535, 64, 40), (65536 + 200, 48, 129), (70000, 16, 1), (65536, 240, 255)]  # wide maps
 
 
@@ -371,6 +372,17 @@ def test_quantised_steps_at_the_borders(M, K):
     one = torch.ones(len(wq), device=DEV)
     y = F.linear_i8(x.to(DEV), wq, one).cpu()
     assert torch.equal(y, q0[:, :len(wq)].float() * s0[:, None])
+
+
+@pytest.mark.parametrize("K,N", [(64, 40), (256, 256), (512, 72), (272, 1000)])
+@pytest.mark.parametrize("dtype", TYPES)
+def test_i8_rows_do_not_depend_on_the_rows_beside_them(K, N, dtype):
+    w, s = F.quantize_rows(rnd(1, N, K))
+    x, res, bias = rnd(2, 9000, K, dtype=dtype), rnd(3, 9000, N, dtype=dtype), rnd(4, N)
+    y, h = F.linear_i8(x, w, s, bias, res), F.gated_linear_i8(x, w, s, w, s, "gelu")
+    for M in (1, 4, 5, 16, 17, 64, 65, 200, 4096):
+        assert torch.equal(F.linear_i8(x[:M], w, s, bias, res[:M]), y[:M]), M
+        assert torch.equal(F.gated_linear_i8(x[:M], w, s, w, s, "gelu"), h[:M]), M
 
 
 def test_i8_largest_sums_are_exact():
