@@ -390,7 +390,7 @@ int hgk_gated_fwd(hgk_stream_t stream, int dtype, const void* x, const void* wg,
   HGK_CHECK_ARG(x && wg && wu && h, "gated: null pointer");
   HGK_CHECK_ARG(al16(x) && al16(wg) && al16(wu) && al16(h) && al16(workspace),
                 "gated: pointers must be 16-byte aligned");
-  HGK_CHECK_ARG(ws_bytes >= hgk_gated_workspace(dtype, M, C, F, 0), "gated: workspace of %zu bytes is too small", ws_bytes);
+  HGK_CHECK_WORKSPACE("gated", workspace, ws_bytes, hgk_gated_workspace(dtype, M, C, F, 0));
   HGK_DISPATCH_DTYPE(dtype, T, return gated_fwd<T>((hipStream_t)stream, x, wg, wu, h, M, C, F, act,
                                                    (char*)workspace, dtype));
 }
@@ -411,8 +411,7 @@ int hgk_gated_bwd(hgk_stream_t stream, int dtype, const void* x, const void* wg,
   HGK_CHECK_ARG(x && wg && wu && dh, "gated: null pointer");
   HGK_CHECK_ARG(al16(x) && al16(wg) && al16(wu) && al16(dh) && al16(dx) && al16(dwg) && al16(dwu) &&
                     al16(workspace), "gated: pointers must be 16-byte aligned");
-  HGK_CHECK_ARG(workspace && ws_bytes >= hgk_gated_workspace(dtype, M, C, F, 1),
-                "gated: workspace of %zu bytes is too small", ws_bytes);
+  HGK_CHECK_WORKSPACE("gated", workspace, ws_bytes, hgk_gated_workspace(dtype, M, C, F, 1));
   HGK_DISPATCH_DTYPE(dtype, T, return gated_bwd<T>((hipStream_t)stream, x, wg, wu, dh, dx, dwg, dwu, M, C,
                                                    F, act, (char*)workspace, dtype));
 }
@@ -432,8 +431,7 @@ int hgk_linear_fwd(hgk_stream_t stream, int dtype, const void* x, const void* w,
   HGK_CHECK_ARG(al16(x) && al16(w) && al16(res) && al16(y) && al16(workspace),
                 "linear: pointers must be 16-byte aligned");
   const DropArgs d = make_drop(p, seed, offset, step);
-  HGK_CHECK_ARG(ws_bytes >= hgk_linear_workspace(dtype, M, K, N, d.thr != 0, 0),
-                "linear: workspace of %zu bytes is too small", ws_bytes);
+  HGK_CHECK_WORKSPACE("linear", workspace, ws_bytes, hgk_linear_workspace(dtype, M, K, N, d.thr != 0, 0));
   HGK_DISPATCH_DTYPE(dtype, T, return linear_fwd<T>((hipStream_t)stream, x, w, res, y, M, K, N, d,
                                                     (char*)workspace, dtype));
 }
@@ -452,8 +450,7 @@ int hgk_linear_bwd(hgk_stream_t stream, int dtype, const void* x, const void* w,
   HGK_CHECK_ARG(al16(x) && al16(w) && al16(dy) && al16(dx) && al16(dw) && al16(workspace),
                 "linear: pointers must be 16-byte aligned");
   const DropArgs d = make_drop(p, seed, offset, step);
-  HGK_CHECK_ARG(ws_bytes >= hgk_linear_workspace(dtype, M, K, N, d.thr != 0, 1),
-                "linear: workspace of %zu bytes is too small", ws_bytes);
+  HGK_CHECK_WORKSPACE("linear", workspace, ws_bytes, hgk_linear_workspace(dtype, M, K, N, d.thr != 0, 1));
   HGK_DISPATCH_DTYPE(dtype, T, return linear_bwd<T>((hipStream_t)stream, x, w, dy, dx, dw, M, K, N, d,
                                                     (char*)workspace, dtype));
 }

@@ -904,6 +904,9 @@ bool linear_rows_ok(int dtype, long M, int K, int N, bool drop);
 int linear_rows_bwd(hipStream_t st, const void* dy, const void* w, void* dz, void* dx, long M, int K, int N,
                     const DropArgs& d);
 
+#define HGK_CHECK_WORKSPACE(what, workspace, bytes, need) \
+  HGK_CHECK_ARG((bytes) >= (need) && ((workspace) || (need) == 0), what ": workspace of %zu bytes is too small", (size_t)(bytes))
+
 static inline long up_to(long n, long q) { return (n + q - 1) / q * q; }
 
 // collects the rows to pad, then one launch

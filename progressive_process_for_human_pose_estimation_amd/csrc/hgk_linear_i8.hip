@@ -353,7 +353,7 @@ int hgk_linear_i8(hgk_stream_t stream, int dtype, const void* x, const void* wq,
   if (M == 0) return HGK_OK;
   HGK_CHECK_ARG(x && wq && wscale && y, "linear_i8: null pointer");
   HGK_CHECK_ARG(al16(x) && al16(wq) && al16(res) && al16(y) && al16(workspace), "linear_i8: pointers must be 16-byte aligned");
-  HGK_CHECK_ARG(ws_bytes >= hgk_linear_i8_workspace(M, K, N, 0) && (workspace || !hgk_linear_i8_workspace(M, K, N, 0)), "linear_i8: workspace of %zu bytes is too small", ws_bytes);
+  HGK_CHECK_WORKSPACE("linear_i8", workspace, ws_bytes, hgk_linear_i8_workspace(M, K, N, 0));
   HGK_DISPATCH_DTYPE(dtype, T, return (linear_i8<T, false>((hipStream_t)stream, x, wq, wscale, nullptr, nullptr,
                                                            bias, res, y, M, K, N, 0, (char*)workspace)));
 }
@@ -367,7 +367,7 @@ int hgk_gated_i8(hgk_stream_t stream, int dtype, const void* x, const void* wqg,
   if (M == 0) return HGK_OK;
   HGK_CHECK_ARG(x && wqg && sg && wqu && su && h, "gated_i8: null pointer");
   HGK_CHECK_ARG(al16(x) && al16(wqg) && al16(wqu) && al16(h) && al16(workspace), "gated_i8: pointers must be 16-byte aligned");
-  HGK_CHECK_ARG(ws_bytes >= hgk_linear_i8_workspace(M, C, F, 1) && (workspace || !hgk_linear_i8_workspace(M, C, F, 1)), "gated_i8: workspace of %zu bytes is too small", ws_bytes);
+  HGK_CHECK_WORKSPACE("gated_i8", workspace, ws_bytes, hgk_linear_i8_workspace(M, C, F, 1));
   HGK_DISPATCH_DTYPE(dtype, T, return (linear_i8<T, true>((hipStream_t)stream, x, wqg, sg, wqu, su, nullptr, nullptr, h,
                                                           M, C, F, act, (char*)workspace)));
 }

@@ -82,6 +82,16 @@ def test_abi_refusals():
     refused(L.hgk_gated_i8(None, 0, A, A + 8, A, A, A, A, 4, 8, 8, 0, A, big), "16-byte")
 
 
+def test_abi_refuses_a_workspace_that_is_not_there():
+    L = H.load_library()
+    big = 1 << 40
+    refused(L.hgk_gated_fwd(None, 1, A, A, A, A, 4, 9, 8, 0, None, big), "too small")
+    refused(L.hgk_linear_fwd(None, 1, A, A, None, A, 4, 9, 8, 0.0, 0, 0, None, None, big), "too small")
+    refused(L.hgk_linear_bwd(None, 1, A, A, A, A, A, 4, 8, 8, 0.5, 0, 0, None, None, big), "too small")
+    refused(L.hgk_linear_i8(None, 0, A, A, A, None, None, A, 100, 512, 8, None, big), "too small")
+    refused(L.hgk_gated_i8(None, 0, A, A, A, A, A, A, 100, 512, 8, 0, None, big), "too small")
+
+
 def test_no_rows_launches_nothing():
     L = H.load_library()
     assert L.hgk_gated_fwd(None, 0, None, None, None, None, 0, 8, 8, 0, None, 0) == 0
@@ -95,7 +105,8 @@ def test_workspaces():
     assert L.hgk_gated_workspace(1, 4096, 256, 1024, 0) == 0       # rows of whole 16-byte chunks
     assert L.hgk_gated_workspace(1, 4096, 257, 1024, 0) >= 4096 * 264 * 2 + 2 * 1024 * 264 * 2
     assert L.hgk_gated_workspace(1, 4096, 256, 1024, 1) >= 2 * 4096 * 1024 * 2
-    assert L.hgk_linear_i8_workspace(100, 64, 64, 0) >= 100 * 64 + 100 * 4
+    assert L.hgk_linear_i8_workspace(100, 512, 64, 0) >= 100 * 512 + 100 * 4
+    assert L.hgk_linear_i8_workspace(100, 64, 64, 0) == 0          # quantised on the way
     for bad in ((7, 4, 8, 8, 0), (0, 0, 8, 8, 0), (0, 4, 0, 8, 1)):
         assert L.hgk_gated_workspace(*bad) == 0
 
