@@ -12,16 +12,19 @@
 // Against the tiled products (hgk_gemm.h), which at K = C <= 256 spend half of their time between the
 // products of one tile and the next: two waves share a SIMD, half a chunk apart, and the activations and
 // stores of one run beside the products of the other all the way. What bounds it: LDS reads (each wave reads
-// the whole chunk for its 16 rows) at C = 256, the stores of h, dg and du at C <= 128.
+// the whole chunk for its rows) at C = 256, the stores of h, dg and du at C <= 128. Hence waves of 32 rows in
+// the forward of many rows, which read half as much a row; the backward of 256 channels has no registers
+// for that (dx alone takes 128 more), and of 128 it gains nothing (210 / 215 us with dW at 131072 rows).
 //
-// Measured, us, rows here / best tile (F = 4 C; backward up to dx):
-//   C    M = 16384              24576                 32768                 40000
-//   64   f 7.9/6.4  b 11/17     f 8.4/9.1  b 12/24    f 8.7/9.7  b 13/27    f 11/13    b 18/32
-//   128  f 15/11    b 27/32     f 15/17    b 29/40    f 18/19    b 32/49    f 24/26    b 51/59
-//   192  f 28/19    b 52/49     f 30/28    b 53/67    f 35/31    b 57/82    f 54/39    b 98/103
-//   256  f 36/24    b 65/63     f 41/35    b 66/91    f 46/46    b 84/121   f 73/57    b 130/148
-// and at M = 131072, C = 128: forward 59 / 77, backward 143 / 202. A workgroup takes 128 rows, so 16384 are half
-// of the card's CUs. Hence gated_rows_ok().
+// Measured, us, rows here / best tile (F = 4 C; f forward, b backward up to dx; at C > 128 f in waves of 32 rows):
+//   C    M = 16384          24576              32768              65536              131072
+//   64   f 7.9/6.4 b 11/17  f 8.7/9.4 b 12/24  f 9.4/10 b 13/27   f 14/17            f 21/31
+//   128  f 15/11   b 27/32  f 15/18   b 29/40  f 17/19  b 32/49   f 28/36            f 47/66 (waves of 16: 53)
+//   192           b 52/49   f 38/29   b 53/67  f 38/31  b 57/82   f 47/58            f 94/111
+//   256           b 65/63   f 49/34   b 66/91  f 50/44  b 84/121  f 67/84            f 145/187
+// (forward at C = 256 and 49152 rows 58/65, at 80000 rows 105/105; C = 192: 41/47 and 78/73; C = 128 in waves of 32 and
+// of 16 rows: 25 and 17 at 32768, 27 and 28 at 65536, 37 and 36 at 80000, 75 and 85 at 200000.) A workgroup takes
+// 128 or 256 rows, so 16384 are half of the card's CUs or less. Hence gated_rows_ok() and kTwoGroups.
 #include "hgk_gemm.h"
 
 namespace hgk {
@@ -32,20 +35,19 @@ struct RowsArgs {
   int M, C, F, act;
 };
 
-// NK: 32-channel K-steps, C <= 32 NK
-template <int NK, bool BWD, int ACT>
+// NK: 32-channel K-steps, C <= 32 NK. RW: groups of 16 rows of a wave
+template <int NK, bool BWD, int ACT, int RW>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 void gated_rows_kernel(RowsArgs a) {
   constexpr int PITCH = NK * 64, SLOT = 64 * PITCH, ND = NK / 2;  // LDS row and chunk bytes; DMAs of a wave
   constexpr int DP = 2, DB = 3;  // fragments are read this many K-steps (pairs) ahead: an LDS read under load takes
                                  // longer than the 4 (2) matrix instructions between
   static_assert(NK >= 2 && NK <= 8 && NK % 2 == 0, "channels");
+  static_assert(RW == 1 || !BWD, "the backward takes one group");
   __shared__ __attribute__((aligned(16))) char lds[4 * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
-  const int m = blockIdx.x * 128 + wave * 16 + lr;
-  const bool row_in = m < a.M;
-  const long mc = min(m, a.M - 1);
+  const int m0 = (blockIdx.x * 8 + wave) * (16 * RW) + lr;  // of group i: + 16 i
   const int nc = (a.F + 31) / 32;
 
   // ---- weights: row r of a part (gate, up) has its 16-byte chunk c at slot c ^ s(r), s(r) = (r & 3) |
@@ -74,14 +76,17 @@ void gated_rows_kernel(RowsArgs a) {
   send(0, 0);
   if (nc > 1) send(1, 1);
 
-  i32x4 xf[NK];
+  i32x4 xf[RW][NK];
 #pragma unroll
-  for (int k = 0; k < NK; ++k) {
-    const int c = k * 32 + lg * 8;
-    xf[k] = c < a.C ? *reinterpret_cast<const i32x4*>(a.x + mc * a.C + c) : i32x4{0, 0, 0, 0};
-  }
+  for (int i = 0; i < RW; ++i)
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const int c = k * 32 + lg * 8;
+      const long m = min(m0 + 16 * i, a.M - 1);
+      xf[i][k] = c < a.C ? *reinterpret_cast<const i32x4*>(a.x + m * a.C + c) : i32x4{0, 0, 0, 0};
+    }
   uint4 dhv;  // past the last column: the last group again, unused
-  const bf16_t* dhp = BWD ? a.dh + mc * a.F : nullptr;
+  const bf16_t* dhp = BWD ? a.dh + (long)min(m0, a.M - 1) * a.F : nullptr;
   auto load_dh = [&](int chunk) __attribute__((always_inline)) { dhv = load16(dhp + min(chunk * 32 + lg * 8, a.F - 8)); };
   if (BWD) load_dh(0);
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -102,7 +107,7 @@ void gated_rows_kernel(RowsArgs a) {
 #pragma unroll
   for (int g = 0; g < (BWD ? NK : 1); ++g) acc[g][0] = acc[g][1] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-  f32x4 p[4];  // the chunk's g (halves 0, 1) and u
+  f32x4 p[RW][4];  // the chunk's g (halves 0, 1) and u
   auto products = [&](int c) __attribute__((always_inline)) {
     const char* w = lds + (c & 3) * SLOT;
     i32x4 wf[DP + 1][4];  // gate o = 0, 1, up o = 0, 1 of a K-step and of the DP next
@@ -113,14 +118,18 @@ void gated_rows_kernel(RowsArgs a) {
         wf[k % (DP + 1)][j] = *reinterpret_cast<const i32x4*>(t + ((j >> 1) * 32 + (j & 1) * 4) * PITCH);
     };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) p[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < RW; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) p[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < DP && k < NK; ++k) read(k);
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
       if (k + DP < NK) read(k + DP);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) p[j] = mma<G_BF16>(wf[k % (DP + 1)][j], xf[k], p[j]);
+      for (int i = 0; i < RW; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[i][j] = mma<G_BF16>(wf[k % (DP + 1)][j], xf[i][k], p[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
@@ -130,30 +139,35 @@ void gated_rows_kernel(RowsArgs a) {
     const bool f_in = f0 < a.F;
     // dh of this chunk, and what this wave sent for of the chunk after the one in the products
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    float dh[8], v0[8], v1[8];
+    float dh[8];
     if (BWD) unpack16<bf16_t>(dhv, dh);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float g = p[e >> 2][e & 3], u = p[2 + (e >> 2)][e & 3];
-      if constexpr (BWD) {
-        float av, sl;
-        act_slope<ACT, true>(g, av, sl);
-        v0[e] = f_in ? dh[e] * u * sl : 0.f;
-        v1[e] = f_in ? dh[e] * av : 0.f;
+    for (int i = 0; i < RW; ++i) {
+      const int m = m0 + 16 * i;
+      float v0[8], v1[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float g = p[i][e >> 2][e & 3], u = p[i][2 + (e >> 2)][e & 3];
+        if constexpr (BWD) {
+          float av, sl;
+          act_slope<ACT, true>(g, av, sl);
+          v0[e] = f_in ? dh[e] * u * sl : 0.f;
+          v1[e] = f_in ? dh[e] * av : 0.f;
+        } else {
+          v0[e] = act_f<ACT, true>(g) * u;
+        }
+      }
+      b0 = pack16<bf16_t>(v0);
+      if constexpr (!BWD) {
+        if (m < a.M && f_in) store16(a.h + (long)m * a.F + f0, b0);
       } else {
-        v0[e] = act_f<ACT, true>(g) * u;
+        b1 = pack16<bf16_t>(v1);
+        if (a.dg && m < a.M && f_in) {
+          store16(a.dg + (long)m * a.F + f0, b0);
+          store16(a.du + (long)m * a.F + f0, b1);
+        }
+        load_dh(min(c + 1, nc - 1));
       }
-    }
-    b0 = pack16<bf16_t>(v0);
-    if constexpr (!BWD) {
-      if (row_in && f_in) store16(a.h + (long)m * a.F + f0, b0);
-    } else {
-      b1 = pack16<bf16_t>(v1);
-      if (a.dg && row_in && f_in) {
-        store16(a.dg + (long)m * a.F + f0, b0);
-        store16(a.du + (long)m * a.F + f0, b1);
-      }
-      load_dh(min(c + 1, nc - 1));
     }
   };
   auto back = [&](int c) __attribute__((always_inline)) {
@@ -221,7 +235,7 @@ void gated_rows_kernel(RowsArgs a) {
     meet();
   }
   if constexpr (BWD) {
-    if (!row_in) return;
+    if (m0 >= a.M) return;
     const bool swapped = lg >> 1;
 #pragma unroll
     for (int g = 0; g < NK; ++g) {
@@ -233,23 +247,30 @@ void gated_rows_kernel(RowsArgs a) {
         f[e] = swapped ? acc[g][1][e] : acc[g][0][e];
         f[4 + e] = swapped ? acc[g][0][e] : acc[g][1][e];
       }
-      store16(a.dx + (long)m * a.C + n, pack16<bf16_t>(f));
+      store16(a.dx + (long)m0 * a.C + n, pack16<bf16_t>(f));
     }
   }
 }
 
+static constexpr int kTwoGroups = 98304;  // rows
 bool gated_rows_ok(int dtype, long M, int C, int F, bool bwd) {
   if (dtype != HGK_BF16 || C % 8 != 0 || F % 8 != 0 || route(HGK_ROUTE_FFN_TILE)) return false;
   if (C <= 128) return M >= (bwd ? 16384 : 24576);
-  return bwd && C <= 256 && M >= 24576;
+  return C <= 256 && M >= (bwd ? 24576 : 49152);
 }
 
+template <int NK, bool BWD, int ACT, int RW>
+static void launch_rows_as(hipStream_t st, const RowsArgs& a) {
+  constexpr int rows = 128 * RW;
+  hipLaunchKernelGGL((gated_rows_kernel<NK, BWD, ACT, RW>), dim3((unsigned)((a.M + rows - 1) / rows)), dim3(512), 0, st, a);
+}
 template <bool BWD, int ACT>
 static void launch_rows_act(hipStream_t st, const RowsArgs& a) {
-  const dim3 grid((unsigned)((a.M + 127) / 128));
-  if (a.C <= 64) hipLaunchKernelGGL((gated_rows_kernel<2, BWD, ACT>), grid, dim3(512), 0, st, a);
-  else if (a.C <= 128) hipLaunchKernelGGL((gated_rows_kernel<4, BWD, ACT>), grid, dim3(512), 0, st, a);
-  else if constexpr (BWD) hipLaunchKernelGGL((gated_rows_kernel<8, true, ACT>), grid, dim3(512), 0, st, a);
+  if (a.C <= 64) launch_rows_as<2, BWD, ACT, 1>(st, a);
+  else if constexpr (BWD) a.C <= 128 ? launch_rows_as<4, true, ACT, 1>(st, a) : launch_rows_as<8, true, ACT, 1>(st, a);
+  else if (a.C > 128) launch_rows_as<8, false, ACT, 2>(st, a);
+  else if (a.M >= kTwoGroups) launch_rows_as<4, false, ACT, 2>(st, a);
+  else launch_rows_as<4, false, ACT, 1>(st, a);
 }
 template <bool BWD>
 static int launch_rows(hipStream_t st, const RowsArgs& a) {

@@ -70,7 +70,8 @@ def test_gated_wide_tiles(M, C, Fh):
 # wide maps of few channels: the row kernels, each channel class, ragged rows and columns, one chunk and many
 @pytest.mark.parametrize("M,C,Fh", [(16384, 8, 8), (16384 + 5, 64, 40), (16500, 72, 136), (20000, 128, 32), (16384 + 127, 136, 72),
                                     (16385, 256, 264), (17000, 248, 1000), (24576, 8, 16), (24577, 64, 40),
-                                    (24700, 128, 136), (24576 + 127, 136, 72), (24580, 256, 264)])
+                                    (24700, 128, 136), (24576 + 127, 136, 72), (24580, 256, 264),
+                                    (49152 + 17, 136, 40), (50000, 256, 72), (98304 + 250, 128, 32), (98304, 72, 40)])
 @pytest.mark.parametrize("name", ["silu", "gelu", "relu", "sigmoid"])
 def test_gated_rows(M, C, Fh, name):
     got, (x, wg, wu, dh) = gated_case(M, C, Fh, BF16, name, seed=7)
