@@ -6,19 +6,20 @@
 // LDS (a ring of three, LDS-DMA) and are read as transposed fragments. Against the tiled product this
 // spares the launch that writes dz and its read.
 //
-// Measured, us, here / best tile (the tile with the launch that writes dz; K = 4 N):
-//   N     M = 16384    24576      32768      40000      131072
-//   64    6.4/10.6     6.8/12     7.3/13     9.7/18     17/38        dropped
-//         5.8/7.3      6.1/8.6    6.5/9.2    9.0/12     16/25        p = 0
-//   128   12/15        13/21      14/22      18/30      34/65        dropped
-//         10.7/10.2    12/14      13/15      16/20      32/48        p = 0
-//   192   21/22        23/31      23/35      41/40      87/104       dropped
-//         19/15        21/22      22/25      37/29      82/83        p = 0
-//   256   27/26        27/37      29/43      52/55      120/141      dropped
-//         26/17        26/28      28/33      47/42      118/134      p = 0
-// (40000 rows are 313 workgroups, one a CU at N > 128: two rounds.) Hence linear_rows_ok(). At N = 256 and 32768
-// rows it moves 96 MB at 3.3 TB/s; the LDS reads of the fragments, 1 KB a matrix instruction, would take
-// half of that time.
+// Measured, us, here / best tile (the tile with the launch that writes dz; K = 4 N; N > 128: waves of 16 rows, from
+// 49152 rows on of 32, which read half as much LDS a row):
+//   N     M = 16384    24576      32768      49152      65536      131072
+//   64    6.4/10.6     6.8/12     7.2/14     10/19      12/21      17/39         dropped
+//         5.8/7.3      6.1/8.6    6.5/9.2    9.7/12     11/13      17/25         p = 0
+//   128   12/15        13/21      13/22      18/31      19/40      36/64         dropped
+//         10.7/10.2    12/14      13/14      18/23      20/25      34/47         p = 0
+//   192   21/22        22/30      23/36      34/46      35/57      68/103        dropped
+//         19/15        21/22      23/25      30/35      31/45      61/81         p = 0
+//   256   27/26        27/37      30/45      42/60      46/75      104/142       dropped
+//         26/17        26/27      30/33      39/49      43/62      97/134        p = 0
+// and at 40000 rows, 313 workgroups of 128 one a CU, with nothing dropped 37/29 (192) and 47/42 (256); waves of 16
+// rows at 49152: 43 (192) and 53 (256), dropped. 80000 rows, 313 workgroups of 256: 63/68, 80/93, p = 0 55/54, 73/76.
+// Hence linear_rows_ok() and kTwoGroups. At N = 256 and 131072 rows: 402 MB at 3.9 TB/s.
 #include "hgk_gemm.h"
 
 namespace hgk {
@@ -32,8 +33,8 @@ struct LinearRowsArgs {
   DropArgs d;
 };
 
-// NK: 32-channel steps of the contraction, N <= 32 NK
-template <int NK>
+// NK: 32-channel steps of the contraction, N <= 32 NK. RW: groups of 16 rows of a wave
+template <int NK, int RW>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
 void linear_rows_kernel(LinearRowsArgs a) {
   constexpr int SLOT = NK * 32 * 128, ND = NK / 2, DP = 2;  // DMAs of a wave; fragments are read DP steps ahead
@@ -41,9 +42,8 @@ void linear_rows_kernel(LinearRowsArgs a) {
   __shared__ __attribute__((aligned(16))) char lds[3 * SLOT];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 15, lg = lane >> 4;
-  const int m = blockIdx.x * 128 + wave * 16 + lr;
-  const bool row_in = m < a.M;
-  const long mc = min(m, a.M - 1);
+  const int m0 = (blockIdx.x * 8 + wave) * (16 * RW) + lr;  // of group i: + 16 i
+  auto row_of = [&](int i) __attribute__((always_inline)) { return (long)min(m0 + 16 * i, a.M - 1); };
   const int nc = (a.K + 63) / 64;
 
   // weights: 8 chunks of 16 bytes of row n, swizzled as gemm_kernel's N side (tiles of 64 columns)
@@ -69,25 +69,29 @@ void linear_rows_kernel(LinearRowsArgs a) {
   send(0, 0);
   if (nc > 1) send(1, 1);
 
-  uint4 z[NK];
+  uint4 z[RW][NK];
 #pragma unroll
-  for (int k = 0; k < NK; ++k) {
-    const int c = k * 32 + lg * 8;
-    z[k] = c < a.N ? load16(a.dy + mc * a.N + c) : make_uint4(0, 0, 0, 0);
-  }
+  for (int i = 0; i < RW; ++i)
+#pragma unroll
+    for (int k = 0; k < NK; ++k) {
+      const int c = k * 32 + lg * 8;
+      z[i][k] = c < a.N ? load16(a.dy + row_of(i) * a.N + c) : make_uint4(0, 0, 0, 0);
+    }
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the first chunks have landed
   if (a.drop) {
     const uint64_t off = drop_offset(a.d);
 #pragma unroll
-    for (int k = 0; k < NK; ++k) {
-      const int c = k * 32 + lg * 8;
-      const uint32_t keep = drop_mask8((uint64_t)mc * (a.N >> 3) + (c >> 3), off, a.d.seed, a.d.thr);
-      uint32_t* v = &z[k].x;
+    for (int i = 0; i < RW; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        v[e] &= ((keep >> (2 * e)) & 1u ? 0xffffu : 0u) | ((keep >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
-      if (a.dz && row_in && c < a.N) store16(a.dz + mc * a.N + c, z[k]);
-    }
+      for (int k = 0; k < NK; ++k) {
+        const int c = k * 32 + lg * 8;
+        const uint32_t keep = drop_mask8((uint64_t)row_of(i) * (a.N >> 3) + (c >> 3), off, a.d.seed, a.d.thr);
+        uint32_t* v = &z[i][k].x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          v[e] &= ((keep >> (2 * e)) & 1u ? 0xffffu : 0u) | ((keep >> (2 * e + 1)) & 1u ? 0xffff0000u : 0u);
+        if (a.dz && m0 + 16 * i < a.M && c < a.N) store16(a.dz + row_of(i) * a.N + c, z[i][k]);
+      }
   }
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
@@ -100,7 +104,7 @@ void linear_rows_kernel(LinearRowsArgs a) {
 #pragma unroll 1
   for (int c = 0; c < nc; ++c) {
     const char* t = lds + slot * SLOT + row;
-    f32x4 acc[4];
+    f32x4 acc[RW][4];
     i32x4 wf[DP + 1][4];
     auto read = [&](int k) __attribute__((always_inline)) {
 #pragma unroll
@@ -114,14 +118,19 @@ void linear_rows_kernel(LinearRowsArgs a) {
       }
     };
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < RW; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int k = 0; k < DP && k < NK; ++k) read(k);
 #pragma unroll
     for (int k = 0; k < NK; ++k) {
       if (k + DP < NK) read(k + DP);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[j] = mma<G_BF16>(wf[k % (DP + 1)][j], __builtin_bit_cast(i32x4, z[k]), acc[j]);
+      for (int i = 0; i < RW; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          acc[i][j] = mma<G_BF16>(wf[k % (DP + 1)][j], __builtin_bit_cast(i32x4, z[i][k]), acc[i][j]);
       __builtin_amdgcn_sched_barrier(0);
     }
     // this wave's share of chunk c + 1 has landed (and its stores of a chunk ago are done); chunk c + 2 goes where
@@ -130,17 +139,19 @@ void linear_rows_kernel(LinearRowsArgs a) {
     if (c + 2 < nc) send(c + 2, slot == 0 ? 2 : slot - 1);
     const bool swapped = lg & 1;
 #pragma unroll
-    for (int g = 0; g < 2; ++g) {
-      const int n = c * 64 + 32 * g + 8 * lg;
-      float f[8];
+    for (int i = 0; i < RW; ++i)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = acc[2 * g][e] * a.alpha, y = acc[2 * g + 1][e] * a.alpha;
-        f[e] = swapped ? y : x;
-        f[4 + e] = swapped ? x : y;
+      for (int g = 0; g < 2; ++g) {
+        const int n = c * 64 + 32 * g + 8 * lg;
+        float f[8];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float x = acc[i][2 * g][e] * a.alpha, y = acc[i][2 * g + 1][e] * a.alpha;
+          f[e] = swapped ? y : x;
+          f[4 + e] = swapped ? x : y;
+        }
+        if (m0 + 16 * i < a.M && n < a.K) store16(a.dx + row_of(i) * a.K + n, pack16<bf16_t>(f));
       }
-      if (row_in && n < a.K) store16(a.dx + mc * a.K + n, pack16<bf16_t>(f));
-    }
     asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
@@ -148,12 +159,18 @@ void linear_rows_kernel(LinearRowsArgs a) {
   }
 }
 
+static constexpr int kTwoGroups = 49152;  // rows from which waves take 32 (N > 128)
 bool linear_rows_ok(int dtype, long M, int K, int N, bool drop) {
   if (dtype != HGK_BF16 || N % 8 != 0 || K % 8 != 0 || route(HGK_ROUTE_FFN_TILE)) return false;
   if (N <= 128) return M >= 16384;
-  return drop && N <= 256 && M >= 24576;
+  return N <= 256 && M >= (drop ? 24576 : kTwoGroups);
 }
 
+template <int NK, int RW>
+static void launch_as(hipStream_t st, const LinearRowsArgs& a) {
+  constexpr int rows = 128 * RW;
+  hipLaunchKernelGGL((linear_rows_kernel<NK, RW>), dim3((unsigned)((a.M + rows - 1) / rows)), dim3(512), 0, st, a);
+}
 int linear_rows_bwd(hipStream_t st, const void* dy, const void* w, void* dz, void* dx, long M, int K, int N,
                     const DropArgs& d) {
   LinearRowsArgs a;
@@ -167,10 +184,10 @@ int linear_rows_bwd(hipStream_t st, const void* dy, const void* w, void* dz, voi
   a.drop = d.thr != 0;
   a.alpha = a.drop ? d.scale : 1.f;
   a.d = d;
-  const dim3 grid((unsigned)((M + 127) / 128));
-  if (N <= 64) hipLaunchKernelGGL(linear_rows_kernel<2>, grid, dim3(512), 0, st, a);
-  else if (N <= 128) hipLaunchKernelGGL(linear_rows_kernel<4>, grid, dim3(512), 0, st, a);
-  else hipLaunchKernelGGL(linear_rows_kernel<8>, grid, dim3(512), 0, st, a);
+  if (N <= 64) launch_as<2, 1>(st, a);
+  else if (N <= 128) launch_as<4, 1>(st, a);
+  else if (M < kTwoGroups) launch_as<8, 1>(st, a);
+  else launch_as<8, 2>(st, a);
   HGK_LAUNCH_CHECK();
   return HGK_OK;
 }

@@ -204,7 +204,7 @@ def test_linear_wide_tiles(M, K, N):
 # wide maps of few output channels: the row kernel of the input gradient, each channel class, ragged
 # rows, one chunk of columns and many
 @pytest.mark.parametrize("M,K,N", [(24576, 8, 8), (24576 + 5, 64, 64), (24700, 136, 72), (25000, 40, 128), (24576 + 127, 72, 136),
-                                   (24577, 264, 256), (25000, 1000, 248)])
+                                   (24577, 264, 256), (25000, 1000, 248), (49152 + 33, 72, 136), (50000, 200, 256)])
 @pytest.mark.parametrize("p", [0.0, 0.2])
 def test_linear_rows(M, K, N, p):
     x, w = rnd(1, M, K, dtype=BF16).requires_grad_(), rnd(2, N, K, dtype=BF16, scale=K ** -0.5).requires_grad_()
