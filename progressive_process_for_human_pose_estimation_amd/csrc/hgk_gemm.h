@@ -673,29 +673,32 @@ __device__ __forceinline__ uint32_t max_bits(const float* v, uint32_t m) {
   for (int e = 0; e < V; ++e) m = max(m, __float_as_uint(v[e]) & 0x7fffffffu);
   return m;
 }
-// a wave quantises one row of K elements (K a multiple of 16 bytes of T) in two passes, the second from the cache
+// Largest magnitude of the chunks first, first + step .. of a row of nc 16-byte chunks, over the wave
 template <typename T>
-__device__ __forceinline__ float quant_row(const T* row, int8_t* q, int K, int lane) {
+__device__ __forceinline__ uint32_t row_max(const T* row, int first, int step, int nc) {
   constexpr int V = Vec16<T>::N;
   uint32_t m = 0;
-  for (int c = lane; c < K / V; c += 64) {
+  for (int c = first; c < nc; c += step) {
     float f[V];
-    unpack16<T>(load16(row + c * V), f);
+    unpack16<T>(load16(row + (long)c * V), f);
     m = max_bits<V>(f, m);
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, 64));
-  QuantScale z;
-  const float sc = quant_scale(m, z);
-  for (int c = lane; c < K / V; c += 64) {
+  return m;
+}
+// those chunks in bytes (from the cache)
+template <typename T>
+__device__ __forceinline__ void row_bytes(const T* row, int8_t* q, const QuantScale& z, int first, int step, int nc) {
+  constexpr int V = Vec16<T>::N;
+  for (int c = first; c < nc; c += step) {
     float f[V];
     uint32_t b[V];
-    unpack16<T>(load16(row + c * V), f);
+    unpack16<T>(load16(row + (long)c * V), f);
     quant_bytes<V>(f, z, b);
 #pragma unroll
-    for (int e = 0; e < V; e += 4) *reinterpret_cast<uint32_t*>(q + c * V + e) = pack_bytes(b + e);
+    for (int e = 0; e < V; e += 4) *reinterpret_cast<uint32_t*>(q + (long)c * V + e) = pack_bytes(b + e);
   }
-  return sc;
 }
 
 // ---- few rows (M <= 16 MT): the weights stream once from memory into fragments, no LDS tiles ----
@@ -703,7 +706,8 @@ __device__ __forceinline__ float quant_row(const T* row, int8_t* q, int K, int l
 // of 128 bytes, the partial sums meet in LDS in wave order. Bound by the weights' bytes: one
 // column group of 16 rows x 128 bytes per load pair, M rows of x from the caches.
 // QUANT (8-bit integers, M <= kQuantRows, M K <= kQuantBytes): x is T, and every workgroup quantises its few
-// rows into LDS itself, in place of a launch and a trip through memory.
+// rows into LDS itself, in place of a launch and a trip through memory. All eight waves share them (one wave a
+// row: 1 x 8192 -> 1024 in 11.9 us, so 7.7).
 static constexpr int kQuantRows = 16, kQuantBytes = 32768;
 template <int DT, typename T, int MT, bool DUAL, bool QUANT = false>
 __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
@@ -712,6 +716,7 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
   __shared__ acc_t red[NW][P * MT][64];
   __shared__ __attribute__((aligned(16))) int8_t xq[QUANT ? kQuantBytes : 16];
   __shared__ float xs[QUANT ? kQuantRows : 1];
+  __shared__ uint32_t xm[QUANT ? kQuantRows : 1][NW];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, lr = lane & 15, lg = lane >> 4;
   const int n0 = blockIdx.x * 16;
   const char* w[P];
@@ -721,9 +726,21 @@ __global__ __launch_bounds__(512) void skinny_kernel(GemmArgs a) {
 #pragma unroll
   for (int i = 0; i < MT; ++i) x[i] = a.m0 + (long)min(i * 16 + lr, a.M - 1) * a.ldm;
   if constexpr (QUANT) {
-    for (int r = wave; r < a.M; r += NW) {
-      const float sc = quant_row<T>((const T*)a.m0 + (long)r * a.km, xq + r * a.km, a.km, lane);
-      if (lane == 0) xs[r] = sc;
+    // W waves a row, so that the eight share few rows evenly
+    const int W = a.M == 1 ? 8 : a.M == 2 ? 4 : a.M <= 4 ? 2 : 1, part = wave & (W - 1);
+    const int first = part * 64 + lane, nc = a.km / Vec16<T>::N;
+    for (int r = wave / W; r < a.M; r += NW / W) {
+      const uint32_t m = row_max<T>((const T*)a.m0 + (long)r * a.km, first, W * 64, nc);
+      if (lane == 0) xm[r][part] = m;
+    }
+    __syncthreads();
+    for (int r = wave / W; r < a.M; r += NW / W) {
+      uint32_t m = xm[r][0];
+      for (int i = 1; i < W; ++i) m = max(m, xm[r][i]);
+      QuantScale z;
+      const float sc = quant_scale(m, z);
+      row_bytes<T>((const T*)a.m0 + (long)r * a.km, xq + r * a.km, z, first, W * 64, nc);
+      if (part == 0 && lane == 0) xs[r] = sc;
     }
     __syncthreads();
   }

@@ -71,6 +71,23 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const T* __restrict__ x
   for (int c = K + lane; c < Kp; c += L) qrow[c] = 0;
 }
 
+// long rows (K > 4096 of bf16, 2048 of fp32): a workgroup a row, in two passes, the second from the cache
+template <typename T>
+__global__ __launch_bounds__(256) void quant_long_kernel(const T* __restrict__ x, int8_t* __restrict__ q,
+                                                         float* __restrict__ s, int K, int Kp) {
+  __shared__ uint32_t xm[4];
+  const long r = blockIdx.x;
+  const int tid = threadIdx.x, nc = K / Vec16<T>::N;
+  const uint32_t part = row_max<T>(x + r * K, tid, 256, nc);
+  if ((tid & 63) == 0) xm[tid >> 6] = part;
+  __syncthreads();
+  QuantScale z;
+  const float sc = quant_scale(max(max(xm[0], xm[1]), max(xm[2], xm[3])), z);
+  row_bytes<T>(x + r * K, q + r * Kp, z, tid, 256, nc);
+  if (tid == 0) s[r] = sc;
+  for (int c = K + tid; c < Kp; c += 256) q[r * Kp + c] = 0;
+}
+
 template <typename T, bool VEC>
 static void launch_quant_as(hipStream_t st, const T* x, int8_t* q, float* s, long rows, int K, int Kp) {
   const int nc = VEC ? K / Vec16<T>::N : K;
@@ -85,6 +102,7 @@ static void launch_quant_as(hipStream_t st, const T* x, int8_t* q, float* s, lon
   else if (nc <= 128) HGK_QUANT(64, 2);
   else if (nc <= 256) HGK_QUANT(64, 4);
   else if (nc <= 512) HGK_QUANT(64, 8);
+  else if constexpr (VEC) hipLaunchKernelGGL((quant_long_kernel<T>), dim3((unsigned)rows), blk, 0, st, x, q, s, K, Kp);
   else HGK_QUANT(64, 0);
 #undef HGK_QUANT
 }
@@ -219,9 +237,9 @@ void i8_map_kernel(GemmArgs a, int tiles) {
 }
 
 // Which kernel a call takes, and what it needs. Measured, us, this way / the other:
-//   rows quantised by the product's workgroups / by a launch of their own (bf16, gated 1024 -> 4096): 4.7 / 6.1 at
-//     5 rows, 4.8 / 6.2 at 8; 256 -> 1024 4.3 / 5.3 at 16. 32 KB of quantised rows leave LDS for three
-//     workgroups a CU.
+//   rows quantised by the product's workgroups / by a launch of their own at a row 16 longer (bf16): 1 x 32768 ->
+//     1024 22.6 / 27.5, 2 x 16384 13.8 / 15.1, 3 x 5456 7.5 / 8.4, 4 x 4096 -> 2048 6.9 / 7.6, 8 x 2048 -> 4096 6.1 /
+//     7.4, 16 x 1024 6.1 / 6.1. Twice as much was slower: 8 x 4096 10.9 / 8.4, 16 x 2048 8.4 / 7.6.
 //   few channels: the map kernel / the best of quantising launch + tiles (256 x 256 bf16): 5.8 / 6.7 at 65 rows, 6.6
 //     / 9.4 at 8192, 13.7 / 19.9 at 32768, 35 / 46 at 131072; fp32 6.4 / 6.6, 8.1 / 10, 19 / 21, 64 / 65 (256 ->
 //     64 in fp32 at 131072 the other way: 46 / 40). Up to 64 rows against the weight-streaming kernel: 5.8 / 6.2
@@ -229,7 +247,7 @@ void i8_map_kernel(GemmArgs a, int tiles) {
 //   weight-streaming / tiles (bf16, gated 1024 -> 4096): 8.6 at 64 rows / 8.4 at 65; linear 4096 -> 1024 17 / 18.
 enum I8Way { W_FEW_FUSED, W_FEW, W_MAP, W_TILES };
 static I8Way i8_way(long M, int K, int N, bool gated) {
-  if (M <= kQuantRows && M * K <= kQuantBytes && K % 16 == 0) return W_FEW_FUSED;
+  if (M <= kQuantRows && M * K <= (M <= 2 ? kQuantBytes : kQuantBytes / 2) && K % 16 == 0) return W_FEW_FUSED;
   if (M <= 64) return W_FEW;
   if (!gated && K <= kMapK && K % 16 == 0 && N <= kMapN && !route(HGK_ROUTE_FFN_TILE)) return W_MAP;
   return W_TILES;

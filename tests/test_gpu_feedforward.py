@@ -299,7 +299,8 @@ def test_expanded_input_gradient():
 I8 = [(1, 8, 8), (1, 1, 1), (2, 17, 5), (16, 1000, 40), (17, 64, 129), (64, 130, 16), (65, 128, 128), (200, 257, 66),
       (333, 96, 515), (8192 + 5, 48, 2064), (20, 5000, 24), (4, 20000, 8),
       (1, 8192, 33), (4, 16, 7), (3, 4096, 100), (4, 8208, 20), (4, 8192, 24), (16, 2048, 24), (16, 2064, 24),
-      (1, 32768, 20), (1, 32784, 20), (9, 3632, 40),  # rows quantised by each workgroup
+      (1, 32768, 20), (1, 32784, 20), (9, 3632, 40), (2, 16384, 24), (2, 16400, 24), (3, 5456, 24), (8, 2048, 40), (16, 1024, 40),
+      (7, 1008, 40),  # rows quantised by each workgroup
       (65536 + 3, 256, 256), (65535, 64, 40), (65536 + 200, 48, 129), (70000, 16, 1), (65536, 240, 255)]  # wide maps
 
 
