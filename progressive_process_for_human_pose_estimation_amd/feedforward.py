@@ -26,6 +26,7 @@ import math
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import hgk as H
 
@@ -92,6 +93,13 @@ def _grads(a, b, c=None):
         and torch.is_grad_enabled()
 
 
+def _by_function(a, b=None, c=None):
+    """Whether a call goes through its autograd function: where a gradient is wanted, under torch.jit.trace
+    (which records functions; of a bare launch it would record the allocation of the result) and in forward
+    mode (where a function refuses the tangent that a bare launch would lose)"""
+    return _grads(a, b, c) or torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
+
+
 def _launch(x, fn, *args):
     """fn(stream, *args) on x's device and that device's current stream"""
     dev = x.get_device()
@@ -121,7 +129,20 @@ def _once(backward):
     return call
 
 
+# The operands are checked where they are launched, not before the autograd function: a traced graph calls
+# the function by itself, with other operands.
+
 # ---- the gated product ----
+def _gated_operands(x, w_gate, w_up, activation):
+    """(x, w_gate, w_up, activation) as the kernels take them, or HgkError"""
+    _check_weights("gated_linear", w_gate, w_up)
+    _check("gated_linear", x, w_gate.shape[1], (w_gate, x.dtype), (w_up, x.dtype))
+    _code("gated_linear", x)
+    act = _act(activation)
+    _gpu("gated_linear", x)
+    return _dense(x), _dense(w_gate), _dense(w_up), act
+
+
 def _gated_fwd(x, wg, wu, act):
     F, C = wg.shape
     M, dt, lib = x.numel() // C, _DTYPES[x.dtype], H.lib()
@@ -134,8 +155,8 @@ def _gated_fwd(x, wg, wu, act):
 
 class _Gated(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wg, wu, act):
-        x, wg, wu = _dense(x), _dense(wg), _dense(wu)
+    def forward(ctx, x, wg, wu, activation):
+        x, wg, wu, act = _gated_operands(x, wg, wu, activation)
         ctx.save_for_backward(x, wg, wu)
         ctx.act = act
         return _gated_fwd(x, wg, wu, act)
@@ -160,17 +181,23 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
     """act(x w_gate^T) * (x w_up^T): x [..., C], w_gate and w_up [F, C] -> [..., F]. Both products, the
     activation and the product of the two in one kernel; the backward computes them again and keeps
     nothing but the inputs. activation: silu, gelu (erf), relu, sigmoid."""
-    _check_weights("gated_linear", w_gate, w_up)
-    _check("gated_linear", x, w_gate.shape[1], (w_gate, x.dtype), (w_up, x.dtype))
-    _code("gated_linear", x)
-    act = _act(activation)
-    _gpu("gated_linear", x)
-    if _grads(x, w_gate, w_up):
-        return _Gated.apply(x, w_gate, w_up, act)
-    return _gated_fwd(_dense(x), _dense(w_gate), _dense(w_up), act)
+    if _by_function(x, w_gate, w_up):
+        return _Gated.apply(x, w_gate, w_up, activation)
+    return _gated_fwd(*_gated_operands(x, w_gate, w_up, activation))
 
 
 # ---- product, dropout and residual ----
+def _linear_operands(x, w, residual, p, seed, offset, step):
+    _check_weights("linear_dropout_add", w)
+    _check("linear_dropout_add", x, w.shape[1], (w, x.dtype), (residual, x.dtype))
+    _code("linear_dropout_add", x)
+    if residual is not None and residual.shape != (*x.shape[:-1], w.shape[0]):
+        raise H.HgkError(f"linear_dropout_add: residual of shape {tuple(residual.shape)}")
+    _check_dropout(p, seed, offset, step, x.device)
+    _gpu("linear_dropout_add", x)
+    return _dense(x), _dense(w), None if residual is None else _dense(residual)
+
+
 def _linear_fwd(x, w, res, p, seed, offset, step):
     N, K = w.shape
     M, dt, lib = x.numel() // K, _DTYPES[x.dtype], H.lib()
@@ -184,10 +211,10 @@ def _linear_fwd(x, w, res, p, seed, offset, step):
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, res, p, seed, offset, step):
-        x, w = _dense(x), _dense(w)
+        x, w, res = _linear_operands(x, w, res, p, seed, offset, step)
         ctx.save_for_backward(x, w, step)
         ctx.drop = (p, seed, offset)
-        return _linear_fwd(x, w, None if res is None else _dense(res), p, seed, offset, step)
+        return _linear_fwd(x, w, res, p, seed, offset, step)
 
     @staticmethod
     @_once
@@ -210,20 +237,26 @@ class _Linear(torch.autograd.Function):
 def linear_dropout_add(x, w, residual=None, p=0.0, seed=0, offset=0, step=None):
     """residual + dropout(x w^T): x [..., K], w [N, K], residual [..., N] or None -> [..., N]; dropout
     and residual in the product's epilogue. The mask is dropout_add's over the output."""
-    _check_weights("linear_dropout_add", w)
-    _check("linear_dropout_add", x, w.shape[1], (w, x.dtype), (residual, x.dtype))
-    _code("linear_dropout_add", x)
-    if residual is not None and residual.shape != (*x.shape[:-1], w.shape[0]):
-        raise H.HgkError(f"linear_dropout_add: residual of shape {tuple(residual.shape)}")
-    _check_dropout(p, seed, offset, step, x.device)
-    _gpu("linear_dropout_add", x)
-    if _grads(x, w, residual):
+    if _by_function(x, w, residual):
         return _Linear.apply(x, w, residual, p, seed, offset, step)
-    return _linear_fwd(_dense(x), _dense(w), None if residual is None else _dense(residual), p, seed,
-                       offset, step)
+    return _linear_fwd(*_linear_operands(x, w, residual, p, seed, offset, step), p, seed, offset, step)
 
 
 # ---- dropout ----
+def _dropout_operands(x, residual, rows_per_mask, p, seed, offset, step):
+    if x.dim() < 1:
+        raise H.HgkError("dropout_add: expected [..., C]")
+    _check("dropout_add", x, x.shape[-1], (residual, x.dtype))
+    _code("dropout_add", x)
+    if residual is not None and residual.shape != x.shape:
+        raise H.HgkError(f"dropout_add: residual of shape {tuple(residual.shape)} to {tuple(x.shape)}")
+    if rows_per_mask < 1:
+        raise H.HgkError(f"dropout_add: rows_per_mask = {rows_per_mask}")
+    _check_dropout(p, seed, offset, step, x.device)
+    _gpu("dropout_add", x)
+    return _dense(x), None if residual is None else _dense(residual)
+
+
 def _dropout(x, res, rows_per_mask, p, seed, offset, step):
     C = x.shape[-1]
     y = torch.empty_like(x)
@@ -237,10 +270,11 @@ def _dropout(x, res, rows_per_mask, p, seed, offset, step):
 class _DropoutAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, res, rows_per_mask, p, seed, offset, step):
+        x, res = _dropout_operands(x, res, rows_per_mask, p, seed, offset, step)
         if step is not None:
             ctx.save_for_backward(step)
         ctx.args = (rows_per_mask, p, seed, offset, step is not None)
-        return _dropout(_dense(x), None if res is None else _dense(res), rows_per_mask, p, seed, offset, step)
+        return _dropout(x, res, rows_per_mask, p, seed, offset, step)
 
     @staticmethod
     @_once
@@ -256,43 +290,81 @@ def dropout_add(x, residual=None, p=0.5, seed=0, offset=0, step=None, rows_per_m
     """residual + dropout(x) over [..., C]. rows_per_mask: that many consecutive rows share a mask row
     (H * W of an NHWC map drops whole channels of each image); what is dropped is selected away, so
     an infinity or NaN there does not reach the result."""
-    if x.dim() < 1:
-        raise H.HgkError("dropout_add: expected [..., C]")
-    _check("dropout_add", x, x.shape[-1], (residual, x.dtype))
-    _code("dropout_add", x)
-    if residual is not None and residual.shape != x.shape:
-        raise H.HgkError(f"dropout_add: residual of shape {tuple(residual.shape)} to {tuple(x.shape)}")
-    if rows_per_mask < 1:
-        raise H.HgkError(f"dropout_add: rows_per_mask = {rows_per_mask}")
-    _check_dropout(p, seed, offset, step, x.device)
-    _gpu("dropout_add", x)
-    if _grads(x, residual):
+    if _by_function(x, residual):
         return _DropoutAdd.apply(x, residual, rows_per_mask, p, seed, offset, step)
-    return _dropout(_dense(x), None if residual is None else _dense(residual), rows_per_mask, p, seed,
+    return _dropout(*_dropout_operands(x, residual, rows_per_mask, p, seed, offset, step), rows_per_mask, p, seed,
                     offset, step)
 
 
 # ---- 8-bit integers ----
-def quantize_rows(x):
-    """(q int8 [..., K], scale fp32 [...]): scale = max |row| / 127, q = rint(row / scale). A row of
-    zeros has scale 0; a row that holds an infinity or a NaN has scale NaN."""
+def _no_gradient(ctx, *grads):
+    raise H.HgkError("the 8-bit operators have no gradient")
+
+
+class _QuantizeRows(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x):
+        q, s = _quantize_rows(x)
+        ctx.mark_non_differentiable(q, s)
+        return q, s
+
+    backward = staticmethod(_no_gradient)
+
+
+def _quantize_rows(x):
     _check("quantize_rows", x, x.shape[-1] if x.dim() else 0)
-    dt = _code("quantize_rows", x)
+    _code("quantize_rows", x)
     if x.dim() < 1 or x.shape[-1] < 1:
         raise H.HgkError("quantize_rows: expected [..., K]")
     _gpu("quantize_rows", x)
     x = _dense(x)
     q = torch.empty(x.shape, dtype=torch.int8, device=x.device)
     s = torch.empty(x.shape[:-1], dtype=torch.float32, device=x.device)
-    _launch(x, H.lib().hgk_quantize_rows_i8, dt, x.data_ptr(), q.data_ptr(), s.data_ptr(), s.numel(),
+    _launch(x, H.lib().hgk_quantize_rows_i8, _DTYPES[x.dtype], x.data_ptr(), q.data_ptr(), s.data_ptr(), s.numel(),
             x.shape[-1])
     return q, s
 
 
-def _scale(what, s, n):
+def quantize_rows(x):
+    """(q int8 [..., K], scale fp32 [...]): scale = max |row| / 127, q = rint(row / scale). A row of
+    zeros has scale 0; a row that holds an infinity or a NaN has scale NaN. No gradient."""
+    return _QuantizeRows.apply(x) if _by_function(x) else _quantize_rows(x)
+
+
+def _check_scale(what, s, n):
     if s is not None and tuple(s.shape) != (n,):
         raise H.HgkError(f"{what}: expected {n} values, got shape {tuple(s.shape)}")
-    return None if s is None else _dense(s)
+
+
+def _linear_i8(x, w, w_scale, bias, residual):
+    _check_weights("linear_i8", w)
+    N, K = w.shape
+    _check("linear_i8", x, K, (w, torch.int8), (w_scale, torch.float32), (bias, torch.float32),
+           (residual, x.dtype))
+    _code("linear_i8", x)
+    if residual is not None and residual.shape != (*x.shape[:-1], N):
+        raise H.HgkError(f"linear_i8: residual of shape {tuple(residual.shape)}")
+    _check_scale("linear_i8", w_scale, N)
+    _check_scale("linear_i8", bias, N)
+    _gpu("linear_i8", x)
+    x, w, w_scale = _dense(x), _dense(w), _dense(w_scale)
+    bias, residual = (None if t is None else _dense(t) for t in (bias, residual))
+    M, lib = x.numel() // K, H.lib()
+    y = x.new_empty((*x.shape[:-1], N))
+    wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, K, N, 0), x)
+    _launch(x, lib.hgk_linear_i8, _DTYPES[x.dtype], x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), H.ptr(bias),
+            H.ptr(residual), y.data_ptr(), M, K, N, wp, n)
+    return y
+
+
+class _LinearI8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *operands):
+        y = _linear_i8(*operands)
+        ctx.mark_non_differentiable(y)
+        return y
+
+    backward = staticmethod(_no_gradient)
 
 
 def linear_i8(x, w, w_scale, bias=None, residual=None):
@@ -300,44 +372,43 @@ def linear_i8(x, w, w_scale, bias=None, residual=None):
     (quantize_rows), w is int8 [N, K] with w_scale fp32 [N] (quantize_rows of the weights), bias fp32
     [N], residual [..., N] in x's type, which is the result's. The integer sums are exact (K <=
     131072). No gradient."""
-    _check_weights("linear_i8", w)
-    N, K = w.shape
-    _check("linear_i8", x, K, (w, torch.int8), (w_scale, torch.float32), (bias, torch.float32),
-           (residual, x.dtype))
-    dt = _code("linear_i8", x)
-    if residual is not None:
-        if residual.shape != (*x.shape[:-1], N):
-            raise H.HgkError(f"linear_i8: residual of shape {tuple(residual.shape)}")
-    w_scale, bias = _scale("linear_i8", w_scale, N), _scale("linear_i8", bias, N)
-    _gpu("linear_i8", x)
-    x, w = _dense(x), _dense(w)
-    residual = None if residual is None else _dense(residual)
-    M, lib = x.numel() // K, H.lib()
-    y = x.new_empty((*x.shape[:-1], N))
-    wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, K, N, 0), x)
-    _launch(x, lib.hgk_linear_i8, dt, x.data_ptr(), w.data_ptr(), w_scale.data_ptr(), H.ptr(bias),
-            H.ptr(residual), y.data_ptr(), M, K, N, wp, n)
-    return y
+    call = _LinearI8.apply if _by_function(x, residual) else _linear_i8
+    return call(x, w, w_scale, bias, residual)
+
+
+def _gated_i8(x, wg, sg, wu, su, activation):
+    _check_weights("gated_linear_i8", wg, wu)
+    F, C = wg.shape
+    _check("gated_linear_i8", x, C, (wg, torch.int8), (wu, torch.int8), (sg, torch.float32), (su, torch.float32))
+    _code("gated_linear_i8", x)
+    act = _act(activation)
+    _check_scale("gated_linear_i8", sg, F)
+    _check_scale("gated_linear_i8", su, F)
+    _gpu("gated_linear_i8", x)
+    x, wg, sg, wu, su = (_dense(t) for t in (x, wg, sg, wu, su))
+    M, lib = x.numel() // C, H.lib()
+    h = x.new_empty((*x.shape[:-1], F))
+    wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, C, F, 1), x)
+    _launch(x, lib.hgk_gated_i8, _DTYPES[x.dtype], x.data_ptr(), wg.data_ptr(), sg.data_ptr(), wu.data_ptr(),
+            su.data_ptr(), h.data_ptr(), M, C, F, act, wp, n)
+    return h
+
+
+class _GatedI8(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, *operands):
+        h = _gated_i8(*operands)
+        ctx.mark_non_differentiable(h)
+        return h
+
+    backward = staticmethod(_no_gradient)
 
 
 def gated_linear_i8(x, w_gate, gate_scale, w_up, up_scale, activation="silu"):
     """gated_linear with both products in 8-bit integers (see linear_i8): w_gate and w_up int8 [F, C]
     with a scale for each row. No gradient."""
-    _check_weights("gated_linear_i8", w_gate, w_up)
-    F, C = w_gate.shape
-    _check("gated_linear_i8", x, C, (w_gate, torch.int8), (w_up, torch.int8), (gate_scale, torch.float32),
-           (up_scale, torch.float32))
-    dt = _code("gated_linear_i8", x)
-    act = _act(activation)
-    sg, su = _scale("gated_linear_i8", gate_scale, F), _scale("gated_linear_i8", up_scale, F)
-    _gpu("gated_linear_i8", x)
-    x, wg, wu = _dense(x), _dense(w_gate), _dense(w_up)
-    M, lib = x.numel() // C, H.lib()
-    h = x.new_empty((*x.shape[:-1], F))
-    wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, C, F, 1), x)
-    _launch(x, lib.hgk_gated_i8, dt, x.data_ptr(), wg.data_ptr(), sg.data_ptr(), wu.data_ptr(),
-            su.data_ptr(), h.data_ptr(), M, C, F, act, wp, n)
-    return h
+    call = _GatedI8.apply if _by_function(x) else _gated_i8
+    return call(x, w_gate, gate_scale, w_up, up_scale, activation)
 
 
 # ---- modules ----

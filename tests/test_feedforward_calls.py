@@ -1,0 +1,94 @@
+"""The feed-forward operators' Python side without a GPU, the launches replaced by feedforward_standin.py:
+ways of calling other than eager ones."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import feedforward_standin
+from progressive_process_for_human_pose_estimation_amd import feedforward as F
+
+
+@pytest.fixture(autouse=True)
+def standin(monkeypatch):
+    feedforward_standin.install(monkeypatch)
+
+
+def rnd(seed, *shape):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+W, V, D = rnd(1, 6, 8), rnd(2, 6, 8), rnd(3, 8, 8)
+Q = torch.randint(-127, 128, (8, 8), generator=torch.Generator().manual_seed(4), dtype=torch.int8)
+S = rnd(5, 8).abs()
+
+# each operator with one [4, 8] operand
+CALLS = {
+    "gated_linear": lambda x: F.gated_linear(x, W, V, "relu"),
+    "linear_dropout_add": lambda x: F.linear_dropout_add(x, D, x),
+    "linear without residual": lambda x: F.linear_dropout_add(x, D),
+    "dropout_add": lambda x: F.dropout_add(x, x, 0.0),
+    "dropout without residual": lambda x: F.dropout_add(x, None, 0.0),
+    "quantize_rows": lambda x: F.quantize_rows(x),
+    "linear_i8": lambda x: F.linear_i8(x, Q, S),
+    "linear_i8 with all operands": lambda x: F.linear_i8(x, Q, S, S, x),
+    "gated_linear_i8": lambda x: F.gated_linear_i8(x, Q, S, Q, S, "relu"),
+}
+
+
+def same(a, b):
+    return all(torch.equal(u, v) for u, v in zip(a, b)) if isinstance(a, tuple) else torch.equal(a, b)
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_traced_without_gradients(name):
+    call, x, other = CALLS[name], rnd(6, 4, 8), rnd(7, 11, 8)
+    with torch.no_grad():
+        traced = torch.jit.trace(call, x, check_trace=False)
+        assert same(traced(x), call(x))
+        assert same(traced(other), call(other))  # other values and another number of rows
+
+
+@pytest.mark.parametrize("name", ["gated_linear", "linear_dropout_add", "dropout_add"])
+def test_traced_with_gradients(name):
+    call, x = CALLS[name], rnd(6, 4, 8).requires_grad_()
+    traced = torch.jit.trace(call, x, check_trace=False)
+    y, z = traced(x), call(x)
+    assert torch.equal(y, z)
+    d = rnd(8, *y.shape)
+    assert torch.equal(torch.autograd.grad(y, x, d)[0], torch.autograd.grad(z, x, d)[0])
+
+
+@pytest.mark.parametrize("name", CALLS)
+@pytest.mark.parametrize("grad", [True, False])
+def test_forward_mode_is_refused(name, grad):
+    """A result without a tangent would count as one whose derivative is zero."""
+    call, x = CALLS[name], rnd(6, 4, 8)
+    with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+        assert same(call(x), call(x.clone()))  # no tangent, nothing to refuse
+        with pytest.raises(NotImplementedError, match="jvp"):
+            call(forward_ad.make_dual(x, torch.ones_like(x)))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_functional_forward_mode_is_refused(name):
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.func.jvp(CALLS[name], (rnd(6, 4, 8),), (torch.ones(4, 8),))
+
+
+def test_traced_calls_check_their_operands():
+    """A traced graph may be called with anything: it must not launch on it."""
+    with torch.no_grad():
+        linear = torch.jit.trace(lambda x, w: F.linear_dropout_add(x, w), (rnd(6, 4, 8), D), check_trace=False)
+        gated = torch.jit.trace(lambda x, w: F.gated_linear(x, w, w), (rnd(6, 4, 8), D), check_trace=False)
+        i8 = torch.jit.trace(lambda x, s: F.linear_i8(x, Q, s), (rnd(6, 4, 8), S), check_trace=False)
+    for bad in (lambda: linear(rnd(6, 4, 7), D), lambda: gated(rnd(6, 4, 9), D)):
+        with pytest.raises(RuntimeError, match="rows of 8"):
+            bad()
+    for bad in (lambda: linear(rnd(6, 4, 8), D.bfloat16()), lambda: gated(rnd(6, 4, 8).bfloat16(), D),
+                lambda: i8(rnd(6, 4, 8), S.double())):
+        with pytest.raises(RuntimeError, match="expected torch"):
+            bad()
+    with pytest.raises(RuntimeError, match="8 values"):
+        i8(rnd(6, 4, 8), S[:7])
+    with pytest.raises(RuntimeError, match="operands on"):
+        linear(rnd(6, 4, 8), D.to("meta"))
