@@ -58,6 +58,8 @@ def _dense(t):
 
 def _check(what, x, k, *others):
     """x [..., k] and the other operands: on one device, each of its type"""
+    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+        raise H.HgkError(f"{what}: make_fx cannot record it (torch.jit.trace can)")
     if x.dim() < 1 or x.shape[-1] != k:
         raise H.HgkError(f"{what}: expected rows of {k} channels, got shape {tuple(x.shape)}")
     device = x.device

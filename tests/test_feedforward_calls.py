@@ -3,9 +3,11 @@ ways of calling other than eager ones."""
 import pytest
 import torch
 from torch.autograd import forward_ad
+from torch.fx.experimental.proxy_tensor import make_fx
 
 import feedforward_standin
 from progressive_process_for_human_pose_estimation_amd import feedforward as F
+from progressive_process_for_human_pose_estimation_amd import hgk as H
 
 
 @pytest.fixture(autouse=True)
@@ -92,3 +94,10 @@ def test_traced_calls_check_their_operands():
         i8(rnd(6, 4, 8), S[:7])
     with pytest.raises(RuntimeError, match="operands on"):
         linear(rnd(6, 4, 8), D.to("meta"))
+
+
+@pytest.mark.parametrize("name", CALLS)
+def test_dispatch_tracing_is_refused(name):
+    """make_fx sees what torch dispatches, so not the launches: its graph would return what it allocates."""
+    with pytest.raises(H.HgkError, match="make_fx"):
+        make_fx(CALLS[name])(rnd(6, 4, 8))
