@@ -30,7 +30,7 @@
 extern "C" {
 #endif
 
-#define HGK_ABI_VERSION 40
+#define HGK_ABI_VERSION 41
 
 enum { HGK_F32 = 0, HGK_BF16 = 1 };
 enum { HGK_OK = 0, HGK_ERR_ARG = -1, HGK_ERR_UNSUPPORTED = -2, HGK_ERR_HIP = -3 };
@@ -688,6 +688,8 @@ int hgk_gated_bwd(hgk_stream_t stream, int dtype, const void* x, const void* wg,
 int hgk_dropout_add(hgk_stream_t stream, int dtype, const void* x, const void* res, void* y, long rows,
                     int C, long rows_per_mask, double p, unsigned long long seed,
                     unsigned long long offset, const unsigned long long* step);
+/* Which graph capture a stream is in: a number of its own for each capture, 0 outside of one (ABI 41). */
+unsigned long long hgk_capture_id(hgk_stream_t stream);
 /* y [M][N] = res + D(x w^T), x [M][K], w [N][K], res nullable, D as hgk_dropout_add's with
  * rows_per_mask = 1 over y's elements, in the product's epilogue. */
 size_t hgk_linear_workspace(int dtype, long M, int K, int N, int dropout, int backward);

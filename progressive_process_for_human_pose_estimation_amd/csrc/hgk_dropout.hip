@@ -195,6 +195,13 @@ int dropout_mask(hipStream_t st, int dtype, const void* dy, void* dz, long rows,
 
 using namespace hgk;
 
+extern "C" unsigned long long hgk_capture_id(hgk_stream_t stream) {
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  if (hipStreamGetCaptureInfo((hipStream_t)stream, &status, &id) != hipSuccess) return 0;
+  return status == hipStreamCaptureStatusActive ? id : 0;
+}
+
 extern "C" int hgk_dropout_add(hgk_stream_t stream, int dtype, const void* x, const void* res, void* y,
                                long rows, int C, long rows_per_mask, double p,
                                unsigned long long seed, unsigned long long offset,

@@ -419,7 +419,7 @@ class _Masks(nn.Module):
     construction and the offset in every training call, so that torch.manual_seed governs the masks and
     torch.utils.checkpoint, which puts the generator back, draws the same ones again. `offset` keeps
     the last one. Under graph capture the host's offset is frozen, so a device counter moves on at each
-    replay and the call keeps the value that it saw for its backward."""
+    replay and each use keeps the value that it saw, for its backward and for a checkpoint's recompute."""
 
     def __init__(self, p):
         super().__init__()
@@ -428,6 +428,7 @@ class _Masks(nn.Module):
         self.p = p
         self.seed, self.offset = self._draw(), 0
         self.register_buffer("step", torch.zeros(1, dtype=torch.int64), persistent=False)
+        self._uses = (0, {})  # the last capture, and the counter's value in each of its uses by their offset
 
     @staticmethod
     def _draw():
@@ -438,13 +439,24 @@ class _Masks(nn.Module):
         if not self.training or self.p == 0.0:
             return {"p": 0.0}
         self.offset = self._draw()
-        step = None
-        if x.is_cuda and torch.cuda.is_current_stream_capturing():
-            if self.step.device != x.device:
-                raise H.HgkError(f"dropout: move the module to {x.device} before capturing it")
-            self.step.add_(1 << 32)
-            step = self.step.clone()
+        step = self._captured_step(x) if x.is_cuda and torch.cuda.is_current_stream_capturing() else None
         return {"p": self.p, "seed": self.seed, "offset": self.offset, "step": step}
+
+    def _captured_step(self, x):
+        if self.step.device != x.device:
+            raise H.HgkError(f"dropout: move the module to {x.device} before capturing it")
+        # a forward within a backward is a recompute. It may be captured apart from its forward
+        capture, recompute = H.capture_id(x.device), torch._C._current_graph_task_id() != -1
+        if capture != self._uses[0] and not recompute:
+            self._uses = (capture, {})
+        uses = self._uses[1]
+        if self.offset not in uses:
+            if recompute:
+                raise H.HgkError("dropout: a recompute under capture that does not draw its forward's mask: checkpoint "
+                                 "with preserve_rng_state=True, and recompute before the module is captured anew")
+            self.step.add_(1 << 32)
+            uses[self.offset] = self.step.clone()
+        return uses[self.offset]
 
 
 class Dropout(_Masks):

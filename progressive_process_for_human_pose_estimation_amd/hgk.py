@@ -13,7 +13,7 @@ LIB_PATH = os.path.join(_PKG, "libhgk.so")
 
 F32, BF16 = 0, 1
 UP_BILINEAR_AC, UP_NEAREST = 0, 1
-ABI_VERSION = 40
+ABI_VERSION = 41
 
 _c_void_p = ctypes.c_void_p
 _c_int = ctypes.c_int
@@ -266,6 +266,7 @@ SIGNATURES = {
                                _c_void_p, _c_size_t]),
     "hgk_dropout_add": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 3 + [_c_long, _c_int, _c_long,
                                  _c_double, _c_u64, _c_u64, _c_void_p]),
+    "hgk_capture_id": (_c_u64, [_c_void_p]),
     "hgk_linear_workspace": (_c_size_t, [_c_int, _c_long] + [_c_int] * 4),
     "hgk_linear_fwd": (_c_int, [_c_void_p, _c_int] + [_c_void_p] * 4 + [_c_long, _c_int, _c_int,
                                 _c_double, _c_u64, _c_u64, _c_void_p, _c_void_p, _c_size_t]),
@@ -386,6 +387,13 @@ def dtype_code(dt):
 
 def stream_handle():
     return torch.cuda.current_stream().cuda_stream
+
+
+def capture_id(device):
+    """A number for the graph capture that the device's current stream is in, 0 outside of one"""
+    if device.type != "cuda":
+        return 0
+    return lib().hgk_capture_id(torch._C._cuda_getCurrentRawStream(device.index))
 
 
 def ptr(t):
