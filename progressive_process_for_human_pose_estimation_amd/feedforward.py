@@ -418,8 +418,8 @@ class _Masks(nn.Module):
     """The (seed, offset, step) of a module's dropout. The seed is drawn from torch's CPU generator at
     construction and the offset in every training call, so that torch.manual_seed governs the masks and
     torch.utils.checkpoint, which puts the generator back, draws the same ones again. `offset` keeps
-    the last one. Under graph capture the host's offset is frozen, so a device counter moves on at each
-    replay and each use keeps the value that it saw, for its backward and for a checkpoint's recompute."""
+    the last one. Under graph capture and in a trace the host's offset is frozen, so a device counter moves
+    on at each replay and each use keeps the value that it saw, for its backward and for a checkpoint's recompute."""
 
     def __init__(self, p):
         super().__init__()
@@ -438,13 +438,19 @@ class _Masks(nn.Module):
         """keyword arguments of the next use, on x's device"""
         if not self.training or self.p == 0.0:
             return {"p": 0.0}
-        self.offset = self._draw()
-        step = self._captured_step(x) if x.is_cuda and torch.cuda.is_current_stream_capturing() else None
-        return {"p": self.p, "seed": self.seed, "offset": self.offset, "step": step}
+        tracing = torch._C._get_tracing_state() is not None
+        self.offset = 0 if tracing else self._draw()  # a trace is compared with another one: no number of its own
+        return {"p": self.p, "seed": self.seed, "offset": self.offset, "step": self._recorded_step(x, tracing)}
 
-    def _captured_step(self, x):
+    def _recorded_step(self, x, tracing):
+        """The device counter's value for this use, None where neither a graph nor a trace records it"""
+        if not tracing and not (x.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return None
         if self.step.device != x.device:
-            raise H.HgkError(f"dropout: move the module to {x.device} before capturing it")
+            raise H.HgkError(f"dropout: move the module to {x.device} before capturing or tracing it")
+        if tracing:
+            self.step.add_(1 << 32)
+            return self.step.clone()
         # a forward within a backward is a recompute. It may be captured apart from its forward
         capture, recompute = H.capture_id(x.device), torch._C._current_graph_task_id() != -1
         if capture != self._uses[0] and not recompute:

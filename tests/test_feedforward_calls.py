@@ -1,5 +1,7 @@
 """The feed-forward operators' Python side without a GPU, the launches replaced by feedforward_standin.py:
 ways of calling other than eager ones."""
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -180,3 +182,24 @@ def test_recompute_that_draws_another_mask_is_refused(capture):
     y = checkpoint(part, torch.ones(3, requires_grad=True), use_reentrant=False, preserve_rng_state=False)
     with pytest.raises(H.HgkError, match="recompute"):
         y.sum().backward()
+
+
+@pytest.mark.parametrize("alone", [True, False])
+@pytest.mark.parametrize("check", [True, False])
+def test_traced_modules_draw_another_mask_in_each_call(monkeypatch, alone, check):
+    """A trace holds the host's offset still: the counter has to be part of the traced graph."""
+    seen = []
+
+    def launch(x, fn, dt, px, res, y, M, C, group, p, seed, offset, step):
+        seen.append((seed, offset, int(feedforward_standin.at(step, 1, of=ctypes.c_int64)[0]) if step else None))
+
+    monkeypatch.setattr(F, "_launch", launch)
+    d, x = F.Dropout(0.5), rnd(6, 4, 8).requires_grad_()
+    traced = torch.jit.trace(d if alone else torch.nn.Sequential(torch.nn.Tanh(), d), x, check_trace=check)
+    seen.clear()
+    for _ in range(3):
+        traced(x).sum().backward()
+    forward, backward = seen[::2], seen[1::2]
+    assert forward == backward and len(set(forward)) == 3
+    assert {v[:2] for v in forward} == {(d.seed, 0)}
+    assert [b[2] - a[2] for a, b in zip(forward, forward[1:])] == [1 << 32] * 2

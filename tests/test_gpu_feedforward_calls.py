@@ -114,3 +114,22 @@ def test_captured_checkpointed_step_replays(reentrant):
         y = F.linear_dropout_add(F.gated_linear(*leaves[:3]), leaves[3], leaves[0], 0.25, mask["seed"], mask["offset"] + moved)
         want = (y.detach(), *torch.autograd.grad(y, leaves, dy))
         assert all(torch.equal(u, v) for u, v in zip(out, want)), i
+
+
+def test_traced_training_block_draws_another_mask_in_each_call():
+    torch.manual_seed(2)
+    block = F.GatedFeedForward(48, 136, p=0.25).to(DEV)
+    x, dy = rnd(1, 2, 9, 11, 48).requires_grad_(), rnd(2, 2, 9, 11, 48)
+    traced = torch.jit.trace(block, x)
+    ys = []
+    for _ in range(3):
+        y = traced(x)
+        leaves = (x, block.w_gate, block.w_up, block.w_down)
+        got = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+        h = F.gated_linear(x, block.w_gate, block.w_up)
+        z = F.linear_dropout_add(h, block.w_down, x, 0.25, block.seed, int(block.step))
+        want = (z.detach(), *torch.autograd.grad(z, leaves, dy))
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+        ys.append(got[0])
+    assert not torch.equal(ys[0], ys[1]) and not torch.equal(ys[1], ys[2])
+    assert torch.equal(torch.jit.trace(block.eval(), x)(x), block(x))
