@@ -90,16 +90,20 @@ def _check_dropout(p, seed, offset, step, device):
         raise H.HgkError(f"dropout: step is an int64 tensor of one element on {device}")
 
 
-def _grads(a, b, c=None):
-    return (a.requires_grad or (b is not None and b.requires_grad) or (c is not None and c.requires_grad)) \
-        and torch.is_grad_enabled()
+def _grads(*operands):
+    if not torch.is_grad_enabled():
+        return False
+    for t in operands:
+        if t is not None and t.requires_grad:
+            return True
+    return False
 
 
-def _by_function(a, b=None, c=None):
+def _by_function(*operands):
     """Whether a call goes through its autograd function: where a gradient is wanted, under torch.jit.trace
     (which records functions; of a bare launch it would record the allocation of the result) and in forward
     mode (where a function refuses the tangent that a bare launch would lose)"""
-    return _grads(a, b, c) or torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
+    return _grads(*operands) or torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
 
 
 def _launch(x, fn, *args):
@@ -300,7 +304,7 @@ def dropout_add(x, residual=None, p=0.5, seed=0, offset=0, step=None, rows_per_m
 
 # ---- 8-bit integers ----
 def _no_gradient(ctx, *grads):
-    raise H.HgkError("the 8-bit operators have no gradient")
+    raise H.HgkError("the 8-bit operators have no gradient: call them under torch.no_grad() or on detached operands")
 
 
 class _QuantizeRows(torch.autograd.Function):
@@ -362,9 +366,7 @@ def _linear_i8(x, w, w_scale, bias, residual):
 class _LinearI8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, *operands):
-        y = _linear_i8(*operands)
-        ctx.mark_non_differentiable(y)
-        return y
+        return _linear_i8(*operands)
 
     backward = staticmethod(_no_gradient)
 
@@ -373,8 +375,8 @@ def linear_i8(x, w, w_scale, bias=None, residual=None):
     """x w^T (+ bias + residual) in 8-bit integers: x [..., K] fp32 / bf16 is quantised row by row
     (quantize_rows), w is int8 [N, K] with w_scale fp32 [N] (quantize_rows of the weights), bias fp32
     [N], residual [..., N] in x's type, which is the result's. The integer sums are exact (K <=
-    131072). No gradient."""
-    call = _LinearI8.apply if _by_function(x, residual) else _linear_i8
+    131072). No gradient: a backward that reaches the result is refused."""
+    call = _LinearI8.apply if _by_function(x, w_scale, bias, residual) else _linear_i8
     return call(x, w, w_scale, bias, residual)
 
 
@@ -399,17 +401,15 @@ def _gated_i8(x, wg, sg, wu, su, activation):
 class _GatedI8(torch.autograd.Function):
     @staticmethod
     def forward(ctx, *operands):
-        h = _gated_i8(*operands)
-        ctx.mark_non_differentiable(h)
-        return h
+        return _gated_i8(*operands)
 
     backward = staticmethod(_no_gradient)
 
 
 def gated_linear_i8(x, w_gate, gate_scale, w_up, up_scale, activation="silu"):
     """gated_linear with both products in 8-bit integers (see linear_i8): w_gate and w_up int8 [F, C]
-    with a scale for each row. No gradient."""
-    call = _GatedI8.apply if _by_function(x) else _gated_i8
+    with a scale for each row. No gradient: a backward that reaches the result is refused."""
+    call = _GatedI8.apply if _by_function(x, gate_scale, up_scale) else _gated_i8
     return call(x, w_gate, gate_scale, w_up, up_scale, activation)
 
 
@@ -511,7 +511,7 @@ class GatedFeedForward(_Masks):
 
 class GatedFeedForwardI8(nn.Module):
     """A GatedFeedForward served in 8-bit integers: weights quantised once, with a scale for each
-    output channel; activations row by row in each call. No dropout, no gradients."""
+    output channel; activations row by row in each call. No dropout; a backward through it is refused."""
 
     def __init__(self, block):
         super().__init__()
@@ -530,7 +530,6 @@ class GatedFeedForwardI8(nn.Module):
                 setattr(self, n, s.to(getattr(self, n).device))
         return self
 
-    @torch.no_grad()
     def forward(self, x):
         h = gated_linear_i8(x, self.w_gate, self.gate_scale, self.w_up, self.up_scale, self.activation)
         return linear_i8(h, self.w_down, self.down_scale, residual=x if self.residual else None)

@@ -203,3 +203,39 @@ def test_traced_modules_draw_another_mask_in_each_call(monkeypatch, alone, check
     assert forward == backward and len(set(forward)) == 3
     assert {v[:2] for v in forward} == {(d.seed, 0)}
     assert [b[2] - a[2] for a, b in zip(forward, forward[1:])] == [1 << 32] * 2
+
+
+I8_OPERANDS = [
+    lambda v: F.linear_i8(v, Q, S),
+    lambda v: F.linear_i8(rnd(6, 4, 8), Q, S, None, v),
+    lambda v: F.linear_i8(rnd(6, 4, 8), Q, S, v[0]),
+    lambda v: F.linear_i8(rnd(6, 4, 8), Q, v[0].abs()),
+    lambda v: F.gated_linear_i8(v, Q, S, Q, S),
+    lambda v: F.gated_linear_i8(rnd(6, 4, 8), Q, v[0], Q, S),
+    lambda v: F.gated_linear_i8(rnd(6, 4, 8), Q, S, Q, v[0]),
+]
+
+
+@pytest.mark.parametrize("i", range(len(I8_OPERANDS)))
+def test_gradients_of_the_8_bit_products_are_refused(i):
+    """Not lost: a residual around a served product would pass on half of its gradient."""
+    v = rnd(7, 4, 8).requires_grad_()
+    y = I8_OPERANDS[i](v)
+    with pytest.raises(H.HgkError, match="no gradient"):
+        (y.sum() + v.sum()).backward()
+    with torch.no_grad():
+        assert torch.equal(I8_OPERANDS[i](v), y) and not I8_OPERANDS[i](v).requires_grad
+    assert not I8_OPERANDS[i](v.detach()).requires_grad
+
+
+def test_quantised_weights_take_no_part_in_gradients():
+    q, s = F.quantize_rows(rnd(6, 8, 8).requires_grad_())
+    assert not q.requires_grad and not s.requires_grad
+    assert not F.linear_i8(rnd(7, 4, 8), q, s).requires_grad
+
+
+def test_backward_through_a_served_block_is_refused():
+    served, x = F.GatedFeedForward(8, 16, activation="relu").quantized(), rnd(6, 4, 8).requires_grad_()
+    with pytest.raises(H.HgkError, match="no gradient"):
+        served(x).sum().backward()
+    assert not served(x.detach()).requires_grad
