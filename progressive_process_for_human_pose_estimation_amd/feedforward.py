@@ -84,7 +84,7 @@ def _check_weights(what, w, v=None):
 def _check_dropout(p, seed, offset, step, device):
     if not 0.0 <= p <= 1.0:
         raise H.HgkError(f"dropout: p = {p} is no probability")
-    if not (0 <= seed < _U64 and 0 <= offset < _U64):
+    if not (isinstance(seed, int) and isinstance(offset, int) and 0 <= seed < _U64 and 0 <= offset < _U64):
         raise H.HgkError("dropout: seed and offset are whole numbers of 64 bits")
     if step is not None and (step.dtype != torch.int64 or step.numel() != 1 or step.device != device):
         raise H.HgkError(f"dropout: step is an int64 tensor of one element on {device}")
@@ -256,7 +256,7 @@ def _dropout_operands(x, residual, rows_per_mask, p, seed, offset, step):
     _code("dropout_add", x)
     if residual is not None and residual.shape != x.shape:
         raise H.HgkError(f"dropout_add: residual of shape {tuple(residual.shape)} to {tuple(x.shape)}")
-    if rows_per_mask < 1:
+    if not (isinstance(rows_per_mask, int) and 1 <= rows_per_mask < _U64 >> 1):
         raise H.HgkError(f"dropout_add: rows_per_mask = {rows_per_mask}")
     _check_dropout(p, seed, offset, step, x.device)
     _gpu("dropout_add", x)
@@ -338,7 +338,9 @@ def quantize_rows(x):
 
 
 def _check_scale(what, s, n):
-    if s is not None and tuple(s.shape) != (n,):
+    if s is None:
+        raise H.HgkError(f"{what}: weights without their scales")
+    if tuple(s.shape) != (n,):
         raise H.HgkError(f"{what}: expected {n} values, got shape {tuple(s.shape)}")
 
 
@@ -351,7 +353,8 @@ def _linear_i8(x, w, w_scale, bias, residual):
     if residual is not None and residual.shape != (*x.shape[:-1], N):
         raise H.HgkError(f"linear_i8: residual of shape {tuple(residual.shape)}")
     _check_scale("linear_i8", w_scale, N)
-    _check_scale("linear_i8", bias, N)
+    if bias is not None:
+        _check_scale("linear_i8", bias, N)
     _gpu("linear_i8", x)
     x, w, w_scale = _dense(x), _dense(w), _dense(w_scale)
     bias, residual = (None if t is None else _dense(t) for t in (bias, residual))

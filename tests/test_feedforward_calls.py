@@ -239,3 +239,17 @@ def test_backward_through_a_served_block_is_refused():
     with pytest.raises(H.HgkError, match="no gradient"):
         served(x).sum().backward()
     assert not served(x.detach()).requires_grad
+
+
+@pytest.mark.parametrize("call,text", [
+    (lambda x: F.linear_i8(x, Q, None), "scale"),
+    (lambda x: F.gated_linear_i8(x, Q, None, Q, S), "scale"),
+    (lambda x: F.gated_linear_i8(x, Q, S, Q, None), "scale"),
+    (lambda x: F.dropout_add(x, rows_per_mask=(1 << 64) + 1), "rows_per_mask"),  # 1 in the C entry's 64 bits
+    (lambda x: F.dropout_add(x, rows_per_mask=1.5), "rows_per_mask"),
+    (lambda x: F.dropout_add(x, seed=0.5), "64 bits"),
+    (lambda x: F.linear_dropout_add(x, D, p=0.5, offset=1e3), "64 bits"),
+])
+def test_arguments_that_are_no_such_numbers(call, text):
+    with pytest.raises(H.HgkError, match=text):
+        call(rnd(6, 4, 8))
