@@ -256,11 +256,15 @@ def _dropout_operands(x, residual, rows_per_mask, p, seed, offset, step):
     _code("dropout_add", x)
     if residual is not None and residual.shape != x.shape:
         raise H.HgkError(f"dropout_add: residual of shape {tuple(residual.shape)} to {tuple(x.shape)}")
+    if rows_per_mask is None:
+        if x.dim() < 3:
+            raise H.HgkError(f"dropout_add: rows_per_mask = None takes [N, ..., C], got shape {tuple(x.shape)}")
+        rows_per_mask = max(1, int(math.prod(x.shape[1:-1])))
     if not (isinstance(rows_per_mask, int) and 1 <= rows_per_mask < _U64 >> 1):
         raise H.HgkError(f"dropout_add: rows_per_mask = {rows_per_mask}")
     _check_dropout(p, seed, offset, step, x.device)
     _gpu("dropout_add", x)
-    return _dense(x), None if residual is None else _dense(residual)
+    return _dense(x), None if residual is None else _dense(residual), rows_per_mask
 
 
 def _dropout(x, res, rows_per_mask, p, seed, offset, step):
@@ -276,7 +280,7 @@ def _dropout(x, res, rows_per_mask, p, seed, offset, step):
 class _DropoutAdd(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, res, rows_per_mask, p, seed, offset, step):
-        x, res = _dropout_operands(x, res, rows_per_mask, p, seed, offset, step)
+        x, res, rows_per_mask = _dropout_operands(x, res, rows_per_mask, p, seed, offset, step)
         if step is not None:
             ctx.save_for_backward(step)
         ctx.args = (rows_per_mask, p, seed, offset, step is not None)
@@ -294,12 +298,11 @@ class _DropoutAdd(torch.autograd.Function):
 
 def dropout_add(x, residual=None, p=0.5, seed=0, offset=0, step=None, rows_per_mask=1):
     """residual + dropout(x) over [..., C]. rows_per_mask: that many consecutive rows share a mask row
-    (H * W of an NHWC map drops whole channels of each image); what is dropped is selected away, so
-    an infinity or NaN there does not reach the result."""
+    (H * W of an NHWC map, or None, drops whole channels of each image); what is dropped is selected
+    away, so an infinity or NaN there does not reach the result."""
     if _by_function(x, residual):
         return _DropoutAdd.apply(x, residual, rows_per_mask, p, seed, offset, step)
-    return _dropout(*_dropout_operands(x, residual, rows_per_mask, p, seed, offset, step), rows_per_mask, p, seed,
-                    offset, step)
+    return _dropout(*_dropout_operands(x, residual, rows_per_mask, p, seed, offset, step), p, seed, offset, step)
 
 
 # ---- 8-bit integers ----
@@ -480,12 +483,9 @@ class Dropout(_Masks):
         kw = self.next_mask(x)
         if kw["p"] == 0.0 and residual is None:
             return x
-        rows = 1
-        if self.channels:
-            if x.dim() < 3:
-                raise H.HgkError("Dropout(channels=True): expected an NHWC map")
-            rows = max(1, math.prod(x.shape[1:-1]))
-        return dropout_add(x, residual, rows_per_mask=rows, **kw)
+        if self.channels and x.dim() < 3:
+            raise H.HgkError("Dropout(channels=True): expected an NHWC map")
+        return dropout_add(x, residual, rows_per_mask=None if self.channels else 1, **kw)
 
 
 class GatedFeedForward(_Masks):

@@ -253,3 +253,20 @@ def test_backward_through_a_served_block_is_refused():
 def test_arguments_that_are_no_such_numbers(call, text):
     with pytest.raises(H.HgkError, match=text):
         call(rnd(6, 4, 8))
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_traced_channel_dropout_follows_the_map(monkeypatch, grad):
+    """The rows of an image are the traced call's own, not those of the map that was traced."""
+    seen = []
+    monkeypatch.setattr(F, "_launch", lambda x, fn, dt, px, res, y, M, C, group, *mask: seen.append((M, C, group)))
+    d = F.Dropout(0.5, channels=True)
+    traced = torch.jit.trace(d, rnd(6, 2, 3, 5, 8).requires_grad_(grad), check_trace=False)
+    seen.clear()
+    for shape in ((2, 3, 5, 8), (4, 7, 2, 8), (3, 6, 8)):
+        y = traced(rnd(7, *shape).requires_grad_(grad))
+        if grad:
+            y.sum().backward()
+    assert seen[::1 + grad] == [(30, 8, 15), (56, 8, 14), (18, 8, 6)] and (not grad or seen[::2] == seen[1::2])
+    with pytest.raises(H.HgkError, match="N, ..., C"):
+        F.dropout_add(rnd(6, 4, 8), rows_per_mask=None)
