@@ -3,6 +3,7 @@
 //   y[r][c] = (kept(r, c) ? x[r][c] * scale : 0) (+ res[r][c])
 // One pass: x and res read once, y written once. What is dropped is selected away, not multiplied
 // by zero (an infinity or NaN in a dropped place does not reach y).
+// y may be x or res: no kernel says that they are apart, and each thread reads an element before it writes it.
 #include <algorithm>
 
 #include "hgk_philox.h"
@@ -29,9 +30,9 @@ __global__ __launch_bounds__(256) void dropout_vec_kernel(DropoutArgs a) {
   const int g = (int)(t % a.groups);
   if (r0 >= a.rows) return;
   const uint64_t off = drop_offset(a.d);
-  const T* __restrict__ x = (const T*)a.x;
-  const T* __restrict__ res = (const T*)a.res;
-  T* __restrict__ y = (T*)a.y;
+  const T* x = (const T*)a.x;
+  const T* res = (const T*)a.res;
+  T* y = (T*)a.y;
   typename Vec16<T>::type xv[R][NV], rv[R][NV];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -85,9 +86,9 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(DropoutArgs a, int RB
   for (int i = threadIdx.x; i < nm; i += 256)
     mask[i] = (uint8_t)drop_mask8((uint64_t)mr0 * a.groups + i, off, a.d.seed, a.d.thr);
   __syncthreads();
-  const T* __restrict__ x = (const T*)a.x + r0 * a.C;
-  const T* __restrict__ res = a.res ? (const T*)a.res + r0 * a.C : nullptr;
-  T* __restrict__ y = (T*)a.y + r0 * a.C;
+  const T* x = (const T*)a.x + r0 * a.C;
+  const T* res = a.res ? (const T*)a.res + r0 * a.C : nullptr;
+  T* y = (T*)a.y + r0 * a.C;
   const int n = nr * a.C;  // RB * C <= 2^24 (host)
   auto one = [&](float f, float q, int row, int col) __attribute__((always_inline)) {
     const int mi = a.rows_per_mask == 1 ? row : (int)((r0 + row) / a.rows_per_mask - mr0);

@@ -1,6 +1,7 @@
 """The feed-forward operators' Python side without a GPU, the launches replaced by feedforward_standin.py:
 ways of calling other than eager ones."""
 import ctypes
+import os
 
 import pytest
 import torch
@@ -270,3 +271,10 @@ def test_traced_channel_dropout_follows_the_map(monkeypatch, grad):
     assert seen[::1 + grad] == [(30, 8, 15), (56, 8, 14), (18, 8, 6)] and (not grad or seen[::2] == seen[1::2])
     with pytest.raises(H.HgkError, match="N, ..., C"):
         F.dropout_add(rnd(6, 4, 8), rows_per_mask=None)
+
+
+def test_dropout_kernels_promise_no_separate_operands():
+    """include/hgk.h lets y be x or res. A kernel that says __restrict__ of them is undefined then."""
+    csrc = os.path.join(os.path.dirname(H.LIB_PATH), "csrc")
+    with open(os.path.join(csrc, "hgk_dropout.hip")) as f:
+        assert "__restrict__" not in f.read()
