@@ -33,6 +33,8 @@ from . import hgk as H
 ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 _DTYPES = {torch.float32: H.F32, torch.bfloat16: H.BF16}
 _U64 = 1 << 64
+_PROXY = torch._C._TorchDispatchModeKey.PROXY
+_dispatch_mode, _tracing_state = torch._C._get_dispatch_mode, torch._C._get_tracing_state
 
 
 def _code(what, x):
@@ -58,7 +60,7 @@ def _dense(t):
 
 def _check(what, x, k, *others):
     """x [..., k] and the other operands: on one device, each of its type"""
-    if torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None:
+    if _dispatch_mode(_PROXY) is not None:
         raise H.HgkError(f"{what}: make_fx cannot record it (torch.jit.trace can)")
     if x.dim() < 1 or x.shape[-1] != k:
         raise H.HgkError(f"{what}: expected rows of {k} channels, got shape {tuple(x.shape)}")
@@ -103,7 +105,7 @@ def _by_function(*operands):
     """Whether a call goes through its autograd function: where a gradient is wanted, under torch.jit.trace
     (which records functions; of a bare launch it would record the allocation of the result) and in forward
     mode (where a function refuses the tangent that a bare launch would lose)"""
-    return _grads(*operands) or torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0
+    return _grads(*operands) or _tracing_state() is not None or forward_ad._current_level >= 0
 
 
 def _launch(x, fn, *args):
@@ -444,7 +446,7 @@ class _Masks(nn.Module):
         """keyword arguments of the next use, on x's device"""
         if not self.training or self.p == 0.0:
             return {"p": 0.0}
-        tracing = torch._C._get_tracing_state() is not None
+        tracing = _tracing_state() is not None
         self.offset = 0 if tracing else self._draw()  # a trace is compared with another one: no number of its own
         return {"p": self.p, "seed": self.seed, "offset": self.offset, "step": self._recorded_step(x, tracing)}
 
