@@ -1,0 +1,74 @@
+"""The feed-forward operators where their values are small: relative errors, which the bounds of
+feedforward_oracle.py (on the scale of the operands) do not see."""
+import pytest
+import torch
+
+import feedforward_oracle as R
+from progressive_process_for_human_pose_estimation_amd import feedforward as F
+
+pytestmark = pytest.mark.gpu
+DEV, BF16 = "cuda", torch.bfloat16
+
+
+def every_bf16(low, high):
+    """all bf16 values of low <= |v| <= high"""
+    v = torch.arange(1 << 16, dtype=torch.int32).to(torch.int16).view(BF16)
+    return v[(v.abs() >= low) & (v.abs() <= high)].to(DEV)
+
+
+def gate_alone(g, C=8):
+    """x, w_gate, w_up with x w_gate^T = g (exact: one product of g and 1) and x w_up^T = 1 in column 0"""
+    x = torch.zeros(g.numel(), C, device=DEV, dtype=BF16)
+    x[:, 0], x[:, 1] = g, 1
+    wg, wu = torch.zeros(8, C, device=DEV, dtype=BF16), torch.zeros(8, C, device=DEV, dtype=BF16)
+    wg[0, 0] = wu[0, 1] = 1
+    return x, wg, wu
+
+
+# A result in bf16 is rounded once (R.U), from a value whose own relative error is at most APPROX = 2^-13: 5.5e-5
+# of the polynomial for exp(x^2) erfc(x) (its largest error, on a grid), x^2 2^-24 of the exponential's argument, that
+# is 6e-6 at |g| = 13.2, where Phi leaves fp32's normal numbers, and units of 2^-24 beside.
+APPROX = 2.0 ** -13
+
+
+# few rows, tiles, rows kernel
+@pytest.mark.parametrize("rows", [32, 1000, 24576 + 40])
+def test_gelu_is_right_in_its_tail(rows):
+    g = every_bf16(2 ** -6, 16)
+    n = g.numel()
+    g = torch.cat([g] * -(-rows // n))[:max(n, rows)] if rows > n else g
+    want = g.double() * R.phi(g.double())
+    bound = (R.U[BF16] * (1 + APPROX) + APPROX) * want.abs() + 2 * R.TINY
+    for part, w, b in zip(g.split(rows), want.split(rows), bound.split(rows)):
+        R.worst(F.gated_linear(*gate_alone(part), "gelu")[:, 0], (w, b), "gelu")
+
+
+@pytest.mark.parametrize("rows", [1000, 24576 + 40])
+def test_gelu_slope_is_right_in_its_tail(rows):
+    """dx = slope(g): below g = -2 the slope's two parts are of other signs, and their errors up to 1.6 times its own"""
+    g = every_bf16(2, 16)
+    g = g[g < 0]
+    g = torch.cat([g] * -(-rows // g.numel()))[:rows]
+    x, wg, wu = gate_alone(g)
+    x.requires_grad_()
+    dh = torch.zeros(rows, 8, device=DEV, dtype=BF16)
+    dh[:, 0] = 1
+    dx, = torch.autograd.grad(F.gated_linear(x, wg, wu, "gelu"), x, dh)
+    want = R.slope("gelu", g.double())
+    e = 1.6 * APPROX
+    R.worst(dx[:, 0], (want, (R.U[BF16] * (1 + e) + e) * want.abs() + 32 * R.TINY), "slope")
+
+
+def test_gelu_of_8_bit_products_is_right_in_its_tail():
+    """G = U = g up to 4 roundings of fp32, to which Phi answers with g^2 times their size: 2^-14 at g = 14"""
+    g = every_bf16(2 ** -6, 14)
+    for rows in (8, 40, 2000):
+        x = torch.zeros(rows, 64, device=DEV, dtype=BF16)
+        x[:, 0] = torch.cat([g] * (1 + rows // g.numel()))[-rows:]
+        wq = torch.zeros(8, 64, device=DEV, dtype=torch.int8)
+        wq[0, 0] = 127
+        s = torch.full((8,), 1 / 127, device=DEV)
+        h = F.gated_linear_i8(x, wq, s, wq, s, "gelu")[:, 0]
+        v = x[:, 0].double()
+        want = v * R.phi(v) * v
+        R.worst(h, (want, (R.U[BF16] * 1.001 + APPROX + 2 ** -13) * want.abs() + 32 * R.TINY), rows)
