@@ -180,9 +180,11 @@ __device__ __forceinline__ void act_slope(float g, float& a, float& s) {
     a = g > 0.f || g != g ? g : 0.f;
     s = g > 0.f ? 1.f : 0.f;
   } else {
-    const float q = sigmoid_f<FAST>(g);
-    a = q;
-    s = q * (1.f - q);
+    // from exp(-|g|): 1 - q would leave nothing of the slope where q is next to 1
+    const float e = FAST ? __builtin_amdgcn_exp2f(fabsf(g) * -1.44269504f) : expf(-fabsf(g));
+    const float q = FAST ? __builtin_amdgcn_rcpf(1.f + e) : 1.f / (1.f + e);
+    a = g < 0.f ? e * q : q;
+    s = e * q * q;
   }
 }
 // f(constant) for the activation that `act` names: one branch, not one an element

@@ -72,3 +72,23 @@ def test_gelu_of_8_bit_products_is_right_in_its_tail():
         v = x[:, 0].double()
         want = v * R.phi(v) * v
         R.worst(h, (want, (R.U[BF16] * 1.001 + APPROX + 2 ** -13) * want.abs() + 32 * R.TINY), rows)
+
+
+# sigmoid's slope on both sides: relative to the value, which is exp(-|g|). bf16: the exponential's argument is off by
+# 2 units of 2^-24 of 115 at |g| = 80, 1e-5 of the value; fp32: R.FN of the exponential, the rest beside
+@pytest.mark.parametrize("dtype", [BF16, torch.float32])
+@pytest.mark.parametrize("rows", [1000, 24576 + 40])
+def test_sigmoid_slope_is_right_where_it_is_small(rows, dtype):
+    g = every_bf16(2 ** -6, 80)
+    if rows > g.numel():
+        g = torch.cat([g] * -(-rows // g.numel()))[-rows:]
+    e = 2.0 ** -16 if dtype is BF16 else 2 * R.FN
+    for part in g.split(rows):
+        x, wg, wu = (t.to(dtype) for t in gate_alone(part))
+        x.requires_grad_()
+        dh = torch.zeros(len(part), 8, device=DEV, dtype=dtype)
+        dh[:, 0] = 1
+        dx, = torch.autograd.grad(F.gated_linear(x, wg, wu, "sigmoid"), x, dh)
+        v = part.double()
+        want = torch.exp(-v.abs()) / (1 + torch.exp(-v.abs())) ** 2
+        R.worst(dx[:, 0], (want, (R.U[dtype] * (1 + e) + e) * want + R.TINY), "slope")
