@@ -669,6 +669,9 @@ int hgk_adam_step(hgk_stream_t stream, float* param, const float* grad, float* e
  * weight gradient over no rows is zero).
  * Activations of the gated product: x sigmoid(x), x Phi(x) (erf), max(x, 0), sigmoid(x). */
 enum { HGK_ACT_SILU = 0, HGK_ACT_GELU = 1, HGK_ACT_RELU = 2, HGK_ACT_SIGMOID = 3, HGK_ACT_COUNT = 4 };
+/* what a workspace is for (`backward` of the queries): 0 the forward, else a backward with every
+ * gradient, the input's alone or the weights' alone (ABI 41) */
+enum { HGK_BWD_ALL = 1, HGK_BWD_DX = 2, HGK_BWD_DW = 3 };
 /* h [M][F] = act(x wg^T) * (x wu^T); x [M][C], wg / wu [F][C]. workspace: hgk_gated_workspace()
  * bytes (0 unless rows of C elements are no multiple of 16 bytes). */
 size_t hgk_gated_workspace(int dtype, long M, int C, int F, int backward);

@@ -68,6 +68,13 @@ struct TypeOf<bf16_t> {
 
 static inline int es_of(int dtype) { return dtype == HGK_BF16 ? 2 : 4; }
 
+// which gradients a backward computes, from hgk.h's HGK_BWD_*
+struct Wanted {
+  bool dx, dw;
+};
+static inline Wanted wanted(int backward) { return {backward != HGK_BWD_DW, backward != HGK_BWD_DX}; }
+static inline int wanted_code(bool dx, bool dw) { return dx && dw ? HGK_BWD_ALL : dx ? HGK_BWD_DX : HGK_BWD_DW; }
+
 // workspace layout: offsets of the parts, each on a 256-byte border
 struct Carve {
   long at = 0;
@@ -81,10 +88,10 @@ struct Carve {
 struct GatedWs {
   long x, wg, wu, dg, du, slab, total;
   int Cp, Fp;
-  bool pad;
+  bool pad, rows;
   GemmPlan dx, dw;
 };
-static GatedWs gated_ws(int dtype, long M, int C, int F, bool bwd) {
+static GatedWs gated_ws(int dtype, long M, int C, int F, int bwd) {
   GatedWs w;
   const int es = es_of(dtype), q = 16 / es, ks = 128 / es;
   w.Cp = (int)up_to(C, q);
@@ -97,12 +104,17 @@ static GatedWs gated_ws(int dtype, long M, int C, int F, bool bwd) {
     w.wg = c.take((long)F * w.Cp * es);
     w.wu = c.take((long)F * w.Cp * es);
   }
+  w.rows = false;
   if (bwd) {
-    w.dg = c.take(M * w.Fp * es);
-    w.du = c.take(M * w.Fp * es);
+    const Wanted want = wanted(bwd);
+    w.rows = want.dx && gated_rows_ok(dtype, M, C, F, true);
+    if (!w.rows || want.dw) {  // the row kernel stores dg and du for the weight gradients alone
+      w.dg = c.take(M * w.Fp * es);
+      w.du = c.take(M * w.Fp * es);
+    }
     w.dx = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, C, 1, 2 * (int)((F + ks - 1) / ks), 1, true);
     w.dw = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, F, C, 1, (int)((M + ks - 1) / ks), 2, true);
-    w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
+    w.slab = c.take(std::max(want.dx && !w.rows ? w.dx.slab : 0, want.dw ? w.dw.slab : 0));
   }
   w.total = c.at;
   return w;
@@ -141,7 +153,7 @@ static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* 
                      int C, int F, int act, char* ws, int dtype) {
   constexpr int DT = TypeOf<T>::dt;
   if (gated_rows_ok(dtype, M, C, F, false)) return gated_rows_fwd(st, x, wg, wu, h, M, C, F, act);
-  const GatedWs w = gated_ws(dtype, M, C, F, false);
+  const GatedWs w = gated_ws(dtype, M, C, F, 0);
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
   a.out = h;
@@ -163,12 +175,11 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
                      int dtype) {
   constexpr int DT = TypeOf<T>::dt;
   constexpr int es = sizeof(T), ks = 128 / es;
-  const GatedWs w = gated_ws(dtype, M, C, F, true);
+  const GatedWs w = gated_ws(dtype, M, C, F, wanted_code(dx, dwg));
   GemmArgs a = gemm_args();
   gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
   const char *xp = a.m0, *wgp = a.n0, *wup = a.n1;
-  const bool rows = dx && gated_rows_ok(dtype, M, C, F, true);
-  if (rows) {  // Fp is F, Cp is C
+  if (w.rows) {  // Fp is F, Cp is C
     if (int rc = gated_rows_bwd(st, x, wg, wu, dh, dwg ? ws + w.dg : nullptr, ws + w.du, dx, M, C, F, act)) return rc;
   } else {
     a.dh = dh;
@@ -181,7 +192,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
     run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p);
     HGK_LAUNCH_CHECK();
   }
-  if (dx && !rows) {
+  if (dx && !w.rows) {
     GemmArgs b = gemm_args();
     b.m0 = ws + w.dg;
     b.m1 = ws + w.du;
@@ -223,10 +234,10 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
 struct LinearWs {
   long x, w, dz, slab, total;
   int Kp, Np;
-  bool pad_k, pad_n;
+  bool pad_k, pad_n, rows;
   GemmPlan fwd, dx, dw;
 };
-static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) {
+static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, int bwd) {
   LinearWs w;
   const int es = es_of(dtype), q = 16 / es, ks = 128 / es;
   w.Kp = (int)up_to(K, q);
@@ -234,17 +245,19 @@ static LinearWs linear_ws(int dtype, long M, int K, int N, bool drop, bool bwd) 
   w.pad_k = w.Kp != K;
   w.pad_n = w.Np != N;
   Carve c;
+  const Wanted want = wanted(bwd);
   w.x = w.w = w.dz = w.slab = 0;
-  if (w.pad_k) {
-    w.x = c.take(M * w.Kp * es);
-    w.w = c.take((long)N * w.Kp * es);
-  }
+  if (w.pad_k && (!bwd || want.dw)) w.x = c.take(M * w.Kp * es);
+  if (w.pad_k && (!bwd || want.dx)) w.w = c.take((long)N * w.Kp * es);
+  w.rows = false;
   w.fwd = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, N, 1, (int)((w.Kp + ks - 1) / ks), 1, true);
   if (bwd) {
-    if (drop || w.pad_n) w.dz = c.take(M * w.Np * es);
+    w.rows = want.dx && linear_rows_ok(dtype, M, K, N, drop);
+    // the row kernel stores dz for the weight gradient alone
+    if ((drop || w.pad_n) && (!w.rows || want.dw)) w.dz = c.take(M * w.Np * es);
     w.dx = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, K, 1, (N + ks - 1) / ks, 1, true);
     w.dw = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, N, K, 1, (int)((M + ks - 1) / ks), 1, true);
-    w.slab = c.take(std::max(w.dx.slab, w.dw.slab));
+    w.slab = c.take(std::max(want.dx && !w.rows ? w.dx.slab : 0, want.dw ? w.dw.slab : 0));
   } else {
     w.slab = c.take(M <= skinny_rows<float>(false) ? 0 : w.fwd.slab);  // the same for every type
   }
@@ -257,7 +270,7 @@ static int linear_fwd(hipStream_t st, const void* x, const void* wt, const void*
                       int K, int N, const DropArgs& d, char* ws, int dtype) {
   constexpr int DT = TypeOf<T>::dt;
   typedef typename TypeOf<T>::raw raw;
-  const LinearWs w = linear_ws(dtype, M, K, N, d.thr != 0, false);
+  const LinearWs w = linear_ws(dtype, M, K, N, d.thr != 0, 0);
   if (w.pad_k) {
     Pads p;
     p.add(x, ws + w.x, M, K, w.Kp, sizeof(T));
@@ -292,14 +305,13 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
   constexpr int es = sizeof(T), ks = 128 / es;
   typedef typename TypeOf<T>::raw raw;
   const bool drop = d.thr != 0;
-  const LinearWs w = linear_ws(dtype, M, K, N, drop, true);
+  const LinearWs w = linear_ws(dtype, M, K, N, drop, wanted_code(dx, dw));
   const char *dz = (const char*)dy, *xp = (const char*)x, *wp = (const char*)wt;
   Pads p;
-  const bool rows = dx && linear_rows_ok(dtype, M, K, N, drop);
-  if (rows) {  // nothing to pad
+  if (w.rows) {  // nothing to pad
     void* z = drop && dw ? ws + w.dz : nullptr;
     if (int rc = linear_rows_bwd(st, dy, wt, z, dx, M, K, N, d)) return rc;
-    if (drop) dz = ws + w.dz;
+    if (z) dz = ws + w.dz;
   } else if (w.pad_n) {
     p.add(dy, ws + w.dz, M, N, w.Np, es, drop ? &d : nullptr);
     dz = ws + w.dz;
@@ -316,7 +328,7 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
   p.launch<raw>(st);
   HGK_LAUNCH_CHECK();
   const float alpha = drop ? d.scale : 1.f;
-  if (dx && !rows) {
+  if (dx && !w.rows) {
     GemmArgs b = gemm_args();
     b.m0 = dz;
     b.ldm = (long)w.Np * es;
@@ -379,7 +391,7 @@ extern "C" {
 
 size_t hgk_gated_workspace(int dtype, long M, int C, int F, int backward) {
   if (M <= 0 || C <= 0 || F <= 0 || (dtype != HGK_F32 && dtype != HGK_BF16)) return 0;
-  return (size_t)gated_ws(dtype, M, C, F, backward != 0).total;
+  return (size_t)gated_ws(dtype, M, C, F, backward).total;
 }
 
 int hgk_gated_fwd(hgk_stream_t stream, int dtype, const void* x, const void* wg, const void* wu, void* h,
@@ -411,14 +423,14 @@ int hgk_gated_bwd(hgk_stream_t stream, int dtype, const void* x, const void* wg,
   HGK_CHECK_ARG(x && wg && wu && dh, "gated: null pointer");
   HGK_CHECK_ARG(al16(x) && al16(wg) && al16(wu) && al16(dh) && al16(dx) && al16(dwg) && al16(dwu) &&
                     al16(workspace), "gated: pointers must be 16-byte aligned");
-  HGK_CHECK_WORKSPACE("gated", workspace, ws_bytes, hgk_gated_workspace(dtype, M, C, F, 1));
+  HGK_CHECK_WORKSPACE("gated", workspace, ws_bytes, hgk_gated_workspace(dtype, M, C, F, wanted_code(dx, dwg)));
   HGK_DISPATCH_DTYPE(dtype, T, return gated_bwd<T>((hipStream_t)stream, x, wg, wu, dh, dx, dwg, dwu, M, C,
                                                    F, act, (char*)workspace, dtype));
 }
 
 size_t hgk_linear_workspace(int dtype, long M, int K, int N, int dropout, int backward) {
   if (M <= 0 || K <= 0 || N <= 0 || (dtype != HGK_F32 && dtype != HGK_BF16)) return 0;
-  return (size_t)linear_ws(dtype, M, K, N, dropout != 0, backward != 0).total;
+  return (size_t)linear_ws(dtype, M, K, N, dropout != 0, backward).total;
 }
 
 int hgk_linear_fwd(hgk_stream_t stream, int dtype, const void* x, const void* w, const void* res, void* y,
@@ -450,7 +462,8 @@ int hgk_linear_bwd(hgk_stream_t stream, int dtype, const void* x, const void* w,
   HGK_CHECK_ARG(al16(x) && al16(w) && al16(dy) && al16(dx) && al16(dw) && al16(workspace),
                 "linear: pointers must be 16-byte aligned");
   const DropArgs d = make_drop(p, seed, offset, step);
-  HGK_CHECK_WORKSPACE("linear", workspace, ws_bytes, hgk_linear_workspace(dtype, M, K, N, d.thr != 0, 1));
+  HGK_CHECK_WORKSPACE("linear", workspace, ws_bytes,
+                      hgk_linear_workspace(dtype, M, K, N, d.thr != 0, wanted_code(dx, dw)));
   HGK_DISPATCH_DTYPE(dtype, T, return linear_bwd<T>((hipStream_t)stream, x, w, dy, dx, dw, M, K, N, d,
                                                     (char*)workspace, dtype));
 }

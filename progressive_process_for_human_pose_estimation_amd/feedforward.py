@@ -128,6 +128,11 @@ def _workspace(n, x):
     return ws.data_ptr(), n, ws
 
 
+def _wanted(dx, dw):
+    """HGK_BWD_*: all, the input's or the weights' gradients"""
+    return 1 if dx and dw else 2 if dx else 3
+
+
 def _once(backward):
     """once_differentiable, whose bookkeeping is spared where no second derivative can be asked for"""
     checked = torch.autograd.function.once_differentiable(backward)
@@ -179,7 +184,7 @@ class _Gated(torch.autograd.Function):
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if dw else (None, None)
-        wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, 1), x)
+        wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, _wanted(dx is not None, dw)), x)
         _launch(x, lib.hgk_gated_bwd, dt, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), dh.data_ptr(),
                 H.ptr(dx), H.ptr(dwg), H.ptr(dwu), M, C, F, ctx.act, wp, n)
         return dx, dwg, dwu, None
@@ -236,7 +241,8 @@ class _Linear(torch.autograd.Function):
             g = _dense(dy)
             dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
             dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
-            wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, p > 0, 1), x)
+            drops = int(p * 65536 + 0.5) > 0
+            wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, drops, _wanted(dx is not None, dw is not None)), x)
             _launch(x, lib.hgk_linear_bwd, dt, x.data_ptr(), w.data_ptr(), g.data_ptr(), H.ptr(dx),
                     H.ptr(dw), M, K, N, p, seed, offset, H.ptr(step), wp, n)
         return dx, dw, dy if ctx.needs_input_grad[2] else None, None, None, None, None

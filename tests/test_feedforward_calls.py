@@ -278,3 +278,30 @@ def test_dropout_kernels_promise_no_separate_operands():
     csrc = os.path.join(os.path.dirname(H.LIB_PATH), "csrc")
     with open(os.path.join(csrc, "hgk_dropout.hip")) as f:
         assert "__restrict__" not in f.read()
+
+
+def test_backward_workspaces_hold_what_is_asked_for():
+    """1: every gradient, 2: the input's, 3: the weights'"""
+    gated, linear = H.lib().hgk_gated_workspace, H.lib().hgk_linear_workspace
+    M, C, Fh = 131072, 256, 1024
+    assert gated(1, M, C, Fh, 2) == 0                       # the row kernel stores neither dg nor du
+    assert gated(1, M, C, Fh, 3) >= 2 * M * Fh * 2
+    assert linear(1, M, Fh, C, 1, 2) == 0                   # nor dz
+    assert linear(1, M, Fh, C, 1, 3) >= M * C * 2
+    assert linear(1, M, Fh, C, 0, 2) == 0
+    # tiles: dx splits its long k here, the weight gradient has one K-step
+    small = gated(1, 40, 64, 4096, 3)
+    assert 2 * 40 * 4096 * 2 <= small < gated(1, 40, 64, 4096, 2) == gated(1, 40, 64, 4096, 1)
+    # rows of 33 bf16 are padded: x for dw, w for dx, dy for either
+    assert linear(1, 100, 33, 17, 0, 1) == linear(1, 100, 33, 17, 0, 2) + linear(1, 100, 33, 17, 0, 3) - 100 * 24 * 2 // 256 * 256 - 256
+    for q in (gated(1, 500, 100, 200, 1), gated(0, 500, 100, 200, 1)):
+        assert q > 0
+
+
+def test_backward_refuses_a_workspace_for_fewer_gradients():
+    L, A = H.lib(), 1 << 20  # an address on a 16-byte border: never read, the calls are refused before any launch
+    M, C, Fh = 131072, 256, 1024
+    n = L.hgk_gated_workspace(1, M, C, Fh, 2)
+    assert L.hgk_gated_bwd(None, 1, A, A, A, A, A, A, A, M, C, Fh, 0, A, n) == -1 and b"too small" in L.hgk_last_error()
+    n = L.hgk_linear_workspace(1, M, Fh, C, 1, 2)
+    assert L.hgk_linear_bwd(None, 1, A, A, A, A, A, M, Fh, C, 0.5, 0, 0, None, A, n) == -1 and b"too small" in L.hgk_last_error()

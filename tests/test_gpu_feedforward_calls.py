@@ -155,3 +155,24 @@ def test_dropout_into_an_operand(M, C, group, shift, dtype):
             H.check(H.lib().hgk_dropout_add(H.stream_handle(), F._DTYPES[dtype], a.data_ptr(), b.data_ptr() if use else None,
                                             (a, b)[into].data_ptr(), M, C, group, 0.4, 1, 2, None))
             assert torch.equal((a, b)[into], want if use else alone)
+
+
+# tiles with and without partial sums, padded rows, the row kernels; p = 1e-6 drops nothing
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("M,C,Fh", [(40, 64, 4096), (1000, 33, 17), (129, 72, 264), (700, 1000, 12), (25000, 64, 72), (30000, 200, 256)])
+def test_one_gradient_at_a_time(M, C, Fh, dtype):
+    x, wg, wu, dh = rnd(1, M, C, dtype=dtype), rnd(2, Fh, C, dtype=dtype), rnd(3, Fh, C, dtype=dtype), rnd(4, M, Fh, dtype=dtype)
+
+    def gated(*wanted):
+        leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate((x, wg, wu))]
+        return torch.autograd.grad(F.gated_linear(*leaves), [leaves[i] for i in wanted], dh)
+
+    every = gated(0, 1, 2)
+    assert torch.equal(gated(0)[0], every[0]) and torch.equal(gated(1)[0], every[1]) and torch.equal(gated(2)[0], every[2])
+    for p in (0.0, 1e-6, 0.4):
+        def linear(*wanted):
+            leaves = [t.clone().requires_grad_(i in wanted) for i, t in enumerate((dh, wg.t().contiguous()))]
+            return torch.autograd.grad(F.linear_dropout_add(*leaves, None, p, 3, 4), [leaves[i] for i in wanted], x)
+
+        both = linear(0, 1)
+        assert torch.equal(linear(0)[0], both[0]) and torch.equal(linear(1)[0], both[1])
