@@ -16,12 +16,13 @@
 
 namespace hgk {
 
+// T: type of the result (partial sums are fp32 whatever it is)
 template <int DT, typename T, int LM, int LN>
 static int run_product(hipStream_t st, GemmArgs& a, const GemmPlan& p, char* slab) {
   a.splits = p.splits;
   a.slab = (float*)slab;
   if (p.splits > 1) {
-    run_tiles<DT, T, LM, LN, E_SLAB>(st, a, p);
+    run_tiles<DT, std::conditional_t<DT == G_F32, float, bf16_t>, LM, LN, E_SLAB>(st, a, p);
     HGK_LAUNCH_CHECK();
     const long n = (long)a.batch * a.M * ((a.N + 7) / 8);
     hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((n + 63) / 64)), dim3(64), 0, st, a);
@@ -65,6 +66,15 @@ struct TypeOf<bf16_t> {
   static constexpr int dt = G_BF16;
   typedef uint16_t raw;
 };
+
+// a weight gradient: T, or fp32
+template <int DT, typename T>
+static int run_wgrad(hipStream_t st, GemmArgs& a, const GemmPlan& p, char* slab, bool f32) {
+  if constexpr (sizeof(T) == 2) {
+    if (f32) return run_product<DT, float, L_COL, L_COL>(st, a, p, slab);
+  }
+  return run_product<DT, T, L_COL, L_COL>(st, a, p, slab);
+}
 
 static inline int es_of(int dtype) { return dtype == HGK_BF16 ? 2 : 4; }
 
@@ -172,7 +182,7 @@ static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* 
 template <typename T>
 static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* wu, const void* dh,
                      void* dx, void* dwg, void* dwu, long M, int C, int F, int act, char* ws,
-                     int dtype) {
+                     int dtype, bool f32_wgrad) {
   constexpr int DT = TypeOf<T>::dt;
   constexpr int es = sizeof(T), ks = 128 / es;
   const GatedWs w = gated_ws(dtype, M, C, F, wanted_code(dx, dwg));
@@ -225,7 +235,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
     b.out = dwg;
     b.out1 = dwu;
     b.vec = C % 8 == 0;
-    if (int rc = run_product<DT, T, L_COL, L_COL>(st, b, w.dw, ws + w.slab)) return rc;
+    if (int rc = run_wgrad<DT, T>(st, b, w.dw, ws + w.slab, f32_wgrad)) return rc;
   }
   return HGK_OK;
 }
@@ -300,7 +310,7 @@ static int linear_fwd(hipStream_t st, const void* x, const void* wt, const void*
 
 template <typename T>
 static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void* dy, void* dx, void* dw,
-                      long M, int K, int N, const DropArgs& d, char* ws, int dtype) {
+                      long M, int K, int N, const DropArgs& d, char* ws, int dtype, bool f32_wgrad) {
   constexpr int DT = TypeOf<T>::dt;
   constexpr int es = sizeof(T), ks = 128 / es;
   typedef typename TypeOf<T>::raw raw;
@@ -357,7 +367,7 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
     b.out = dw;
     b.vec = K % 8 == 0;
     b.alpha = alpha;
-    if (int rc = run_product<DT, T, L_COL, L_COL>(st, b, w.dw, ws + w.slab)) return rc;
+    if (int rc = run_wgrad<DT, T>(st, b, w.dw, ws + w.slab, f32_wgrad)) return rc;
   }
   return HGK_OK;
 }
@@ -410,12 +420,14 @@ int hgk_gated_fwd(hgk_stream_t stream, int dtype, const void* x, const void* wg,
 int hgk_gated_bwd(hgk_stream_t stream, int dtype, const void* x, const void* wg, const void* wu,
                   const void* dh, void* dx, void* dwg, void* dwu, long M, int C, int F, int act,
                   void* workspace, size_t ws_bytes) {
+  const bool f32_wgrad = dtype & HGK_F32_WGRAD;
+  dtype &= ~HGK_F32_WGRAD;
   HGK_CHECK_ROWS("gated", M, C, F);
   HGK_CHECK_ARG(act >= 0 && act < HGK_ACT_COUNT, "gated: unknown activation %d", act);
   HGK_CHECK_ARG((dwg == nullptr) == (dwu == nullptr), "gated: both weight gradients or neither");
   if (M == 0) {
     if (!dwg) return HGK_OK;
-    HGK_DISPATCH_DTYPE(dtype, T, {
+    HGK_DISPATCH_DTYPE(f32_wgrad ? HGK_F32 : dtype, T, {
       if (int rc = zero_out<T>((hipStream_t)stream, dwg, (long)F * C)) return rc;
       return zero_out<T>((hipStream_t)stream, dwu, (long)F * C);
     });
@@ -425,7 +437,7 @@ int hgk_gated_bwd(hgk_stream_t stream, int dtype, const void* x, const void* wg,
                     al16(workspace), "gated: pointers must be 16-byte aligned");
   HGK_CHECK_WORKSPACE("gated", workspace, ws_bytes, hgk_gated_workspace(dtype, M, C, F, wanted_code(dx, dwg)));
   HGK_DISPATCH_DTYPE(dtype, T, return gated_bwd<T>((hipStream_t)stream, x, wg, wu, dh, dx, dwg, dwu, M, C,
-                                                   F, act, (char*)workspace, dtype));
+                                                   F, act, (char*)workspace, dtype, f32_wgrad));
 }
 
 size_t hgk_linear_workspace(int dtype, long M, int K, int N, int dropout, int backward) {
@@ -452,11 +464,13 @@ int hgk_linear_bwd(hgk_stream_t stream, int dtype, const void* x, const void* w,
                    void* dw, long M, int K, int N, double p, unsigned long long seed,
                    unsigned long long offset, const unsigned long long* step, void* workspace,
                    size_t ws_bytes) {
+  const bool f32_wgrad = dtype & HGK_F32_WGRAD;
+  dtype &= ~HGK_F32_WGRAD;
   HGK_CHECK_ROWS("linear", M, K, N);
   HGK_CHECK_ARG(p >= 0.0 && p <= 1.0, "linear: p = %g is no probability", p);
   if (M == 0) {
     if (!dw) return HGK_OK;
-    HGK_DISPATCH_DTYPE(dtype, T, return zero_out<T>((hipStream_t)stream, dw, (long)N * K));
+    HGK_DISPATCH_DTYPE(f32_wgrad ? HGK_F32 : dtype, T, return zero_out<T>((hipStream_t)stream, dw, (long)N * K));
   }
   HGK_CHECK_ARG(x && w && dy, "linear: null pointer");
   HGK_CHECK_ARG(al16(x) && al16(w) && al16(dy) && al16(dx) && al16(dw) && al16(workspace),
@@ -465,6 +479,6 @@ int hgk_linear_bwd(hgk_stream_t stream, int dtype, const void* x, const void* w,
   HGK_CHECK_WORKSPACE("linear", workspace, ws_bytes,
                       hgk_linear_workspace(dtype, M, K, N, d.thr != 0, wanted_code(dx, dw)));
   HGK_DISPATCH_DTYPE(dtype, T, return linear_bwd<T>((hipStream_t)stream, x, w, dy, dx, dw, M, K, N, d,
-                                                    (char*)workspace, dtype));
+                                                    (char*)workspace, dtype, f32_wgrad));
 }
 }

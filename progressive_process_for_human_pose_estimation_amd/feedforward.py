@@ -77,6 +77,12 @@ def _gpu(what, x):
         raise H.HgkError(f"{what}: tensors must live on the GPU")
 
 
+def _weight_type(x, masters):
+    """The type that weights have to be of: x's, or fp32 for a module's masters, which are rounded to x's type
+    for the products and have fp32 gradients"""
+    return torch.float32 if masters and x.dtype is torch.bfloat16 else x.dtype
+
+
 def _check_weights(what, w, v=None):
     if w.dim() != 2 or 0 in w.shape or (v is not None and v.shape != w.shape):
         raise H.HgkError(f"{what}: weights are [out, in], got {[tuple(t.shape) for t in (w, v) if t is not None]}")
@@ -146,14 +152,15 @@ def _once(backward):
 # the function by itself, with other operands.
 
 # ---- the gated product ----
-def _gated_operands(x, w_gate, w_up, activation):
+def _gated_operands(x, w_gate, w_up, activation, masters):
     """(x, w_gate, w_up, activation) as the kernels take them, or HgkError"""
     _check_weights("gated_linear", w_gate, w_up)
-    _check("gated_linear", x, w_gate.shape[1], (w_gate, x.dtype), (w_up, x.dtype))
+    of = _weight_type(x, masters)
+    _check("gated_linear", x, w_gate.shape[1], (w_gate, of), (w_up, of))
     _code("gated_linear", x)
     act = _act(activation)
     _gpu("gated_linear", x)
-    return _dense(x), _dense(w_gate), _dense(w_up), act
+    return _dense(x), _dense(w_gate.to(x.dtype)), _dense(w_up.to(x.dtype)), act
 
 
 def _gated_fwd(x, wg, wu, act):
@@ -168,8 +175,9 @@ def _gated_fwd(x, wg, wu, act):
 
 class _Gated(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, wg, wu, activation):
-        x, wg, wu, act = _gated_operands(x, wg, wu, activation)
+    def forward(ctx, x, wg, wu, activation, masters):
+        ctx.wtype = _weight_type(x, masters)
+        x, wg, wu, act = _gated_operands(x, wg, wu, activation, masters)
         ctx.save_for_backward(x, wg, wu)
         ctx.act = act
         return _gated_fwd(x, wg, wu, act)
@@ -183,32 +191,38 @@ class _Gated(torch.autograd.Function):
         dh = _dense(dh)
         dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
         dw = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
-        dwg, dwu = (torch.empty_like(wg), torch.empty_like(wu)) if dw else (None, None)
+        dwg, dwu = (torch.empty_like(v, dtype=ctx.wtype) for v in (wg, wu)) if dw else (None, None)
         wp, n, own = _workspace(lib.hgk_gated_workspace(dt, M, C, F, _wanted(dx is not None, dw)), x)
+        if ctx.wtype is not x.dtype:
+            dt |= H.F32_WGRAD
         _launch(x, lib.hgk_gated_bwd, dt, x.data_ptr(), wg.data_ptr(), wu.data_ptr(), dh.data_ptr(),
                 H.ptr(dx), H.ptr(dwg), H.ptr(dwu), M, C, F, ctx.act, wp, n)
-        return dx, dwg, dwu, None
+        return dx, dwg, dwu, None, None
+
+
+def _gated(x, w_gate, w_up, activation, masters=False):
+    if _by_function(x, w_gate, w_up):
+        return _Gated.apply(x, w_gate, w_up, activation, masters)
+    return _gated_fwd(*_gated_operands(x, w_gate, w_up, activation, masters))
 
 
 def gated_linear(x, w_gate, w_up, activation="silu"):
     """act(x w_gate^T) * (x w_up^T): x [..., C], w_gate and w_up [F, C] -> [..., F]. Both products, the
     activation and the product of the two in one kernel; the backward computes them again and keeps
     nothing but the inputs. activation: silu, gelu (erf), relu, sigmoid."""
-    if _by_function(x, w_gate, w_up):
-        return _Gated.apply(x, w_gate, w_up, activation)
-    return _gated_fwd(*_gated_operands(x, w_gate, w_up, activation))
+    return _gated(x, w_gate, w_up, activation)
 
 
 # ---- product, dropout and residual ----
-def _linear_operands(x, w, residual, p, seed, offset, step):
+def _linear_operands(x, w, residual, p, seed, offset, step, masters):
     _check_weights("linear_dropout_add", w)
-    _check("linear_dropout_add", x, w.shape[1], (w, x.dtype), (residual, x.dtype))
+    _check("linear_dropout_add", x, w.shape[1], (w, _weight_type(x, masters)), (residual, x.dtype))
     _code("linear_dropout_add", x)
     if residual is not None and residual.shape != (*x.shape[:-1], w.shape[0]):
         raise H.HgkError(f"linear_dropout_add: residual of shape {tuple(residual.shape)}")
     _check_dropout(p, seed, offset, step, x.device)
     _gpu("linear_dropout_add", x)
-    return _dense(x), _dense(w), None if residual is None else _dense(residual)
+    return _dense(x), _dense(w.to(x.dtype)), None if residual is None else _dense(residual)
 
 
 def _linear_fwd(x, w, res, p, seed, offset, step):
@@ -223,8 +237,9 @@ def _linear_fwd(x, w, res, p, seed, offset, step):
 
 class _Linear(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, w, res, p, seed, offset, step):
-        x, w, res = _linear_operands(x, w, res, p, seed, offset, step)
+    def forward(ctx, x, w, res, p, seed, offset, step, masters):
+        ctx.wtype = _weight_type(x, masters)
+        x, w, res = _linear_operands(x, w, res, p, seed, offset, step, masters)
         ctx.save_for_backward(x, w, step)
         ctx.drop = (p, seed, offset)
         return _linear_fwd(x, w, res, p, seed, offset, step)
@@ -240,20 +255,26 @@ class _Linear(torch.autograd.Function):
         if ctx.needs_input_grad[0] or ctx.needs_input_grad[1]:
             g = _dense(dy)
             dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-            dw = torch.empty_like(w) if ctx.needs_input_grad[1] else None
+            dw = torch.empty_like(w, dtype=ctx.wtype) if ctx.needs_input_grad[1] else None
             drops = int(p * 65536 + 0.5) > 0
             wp, n, own = _workspace(lib.hgk_linear_workspace(dt, M, K, N, drops, _wanted(dx is not None, dw is not None)), x)
+            if ctx.wtype is not x.dtype:
+                dt |= H.F32_WGRAD
             _launch(x, lib.hgk_linear_bwd, dt, x.data_ptr(), w.data_ptr(), g.data_ptr(), H.ptr(dx),
                     H.ptr(dw), M, K, N, p, seed, offset, H.ptr(step), wp, n)
-        return dx, dw, dy if ctx.needs_input_grad[2] else None, None, None, None, None
+        return dx, dw, dy if ctx.needs_input_grad[2] else None, None, None, None, None, None
+
+
+def _linear(x, w, residual, p=0.0, seed=0, offset=0, step=None, masters=False):
+    if _by_function(x, w, residual):
+        return _Linear.apply(x, w, residual, p, seed, offset, step, masters)
+    return _linear_fwd(*_linear_operands(x, w, residual, p, seed, offset, step, masters), p, seed, offset, step)
 
 
 def linear_dropout_add(x, w, residual=None, p=0.0, seed=0, offset=0, step=None):
     """residual + dropout(x w^T): x [..., K], w [N, K], residual [..., N] or None -> [..., N]; dropout
     and residual in the product's epilogue. The mask is dropout_add's over the output."""
-    if _by_function(x, w, residual):
-        return _Linear.apply(x, w, residual, p, seed, offset, step)
-    return _linear_fwd(*_linear_operands(x, w, residual, p, seed, offset, step), p, seed, offset, step)
+    return _linear(x, w, residual, p, seed, offset, step)
 
 
 # ---- dropout ----
@@ -498,8 +519,8 @@ class Dropout(_Masks):
 
 class GatedFeedForward(_Masks):
     """x + dropout(w_down (act(w_gate x) * (w_up x))) over channels-last [..., channels]. Parameters
-    are fp32 [out, in] with nn.Linear's initialisation and are cast to x's type in each call, so that
-    bf16 maps train fp32 masters. quantized() gives the block in 8-bit integers for serving."""
+    are fp32 [out, in] with nn.Linear's initialisation; beside bf16 maps they are masters, rounded in each
+    call, whose gradients stay fp32. quantized() gives the block in 8-bit integers for serving."""
 
     def __init__(self, channels, hidden, activation="silu", p=0.0, residual=True):
         super().__init__(p)
@@ -512,9 +533,11 @@ class GatedFeedForward(_Masks):
             nn.init.kaiming_uniform_(w, a=math.sqrt(5))
 
     def forward(self, x):
-        h = gated_linear(x, self.w_gate.to(x.dtype), self.w_up.to(x.dtype), self.activation)
-        return linear_dropout_add(h, self.w_down.to(x.dtype), x if self.residual else None,
-                                  **self.next_mask(x))
+        ws = (self.w_gate, self.w_up, self.w_down)
+        masters = all(w.dtype is torch.float32 for w in ws)
+        wg, wu, wd = (w.to(_weight_type(x, masters)) for w in ws)
+        h = _gated(x, wg, wu, self.activation, masters)
+        return _linear(h, wd, x if self.residual else None, masters=masters, **self.next_mask(x))
 
     def quantized(self):
         return GatedFeedForwardI8(self)

@@ -12,6 +12,7 @@ _PKG = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG, "libhgk.so")
 
 F32, BF16 = 0, 1
+F32_WGRAD = 0x100  # hgk_gated_bwd, hgk_linear_bwd: the weights' gradients in fp32
 UP_BILINEAR_AC, UP_NEAREST = 0, 1
 ABI_VERSION = 41
 

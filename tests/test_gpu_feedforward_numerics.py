@@ -92,3 +92,61 @@ def test_sigmoid_slope_is_right_where_it_is_small(rows, dtype):
         v = part.double()
         want = torch.exp(-v.abs()) / (1 + torch.exp(-v.abs())) ** 2
         R.worst(dx[:, 0], (want, (R.U[dtype] * (1 + e) + e) * want + R.TINY), "slope")
+
+
+def rnd(seed, *shape, dtype=torch.float32, scale=1.0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device=DEV) * scale).to(dtype)
+
+
+def last_rounding_in_fp32(value, bound):
+    """the bound of a result that the oracle rounds to bf16, were it rounded to fp32"""
+    u = R.U[BF16]
+    e = (bound - u * value.abs() - R.TINY) / (1 + u)
+    return value, e + R.U[torch.float32] * (value.abs() + e) + R.TINY
+
+
+# no rows; one K-step of the weight gradients and many, with partial sums (1000, 30000) and without; padded rows
+@pytest.mark.parametrize("M,C,Fh", [(0, 16, 24), (1, 8, 8), (70, 33, 17), (300, 264, 520), (1000, 64, 40), (30000, 128, 72)])
+@pytest.mark.parametrize("p", [0.0, 0.25])
+def test_masters_of_bf16_maps_have_fp32_gradients(M, C, Fh, p):
+    """The block on a bf16 map: its weights' gradients are the kernels' fp32 sums, not those through bf16"""
+    torch.manual_seed(3)
+    block = F.GatedFeedForward(C, Fh, p=p, residual=False).to(DEV)
+    x, dy = rnd(1, M, C, dtype=BF16), rnd(2, M, C, dtype=BF16)
+    block(x).backward(dy)
+    wg, wu, wd = (w.detach().to(BF16) for w in (block.w_gate, block.w_up, block.w_down))
+    mask = {"p": p, "seed": block.seed, "offset": block.offset} if p else {}
+    leaves = [t.requires_grad_() for t in (wg, wu, wd)]
+    h = F.gated_linear(x, wg, wu)
+    grads = torch.autograd.grad(F.linear_dropout_add(h, wd, None, **mask), leaves, dy)
+    for w, g in zip((block.w_gate, block.w_up, block.w_down), grads):
+        assert w.grad.dtype is torch.float32 and torch.equal(w.grad.to(BF16), g)
+        assert M == 0 or not torch.equal(w.grad, g.float())
+    if M == 0:
+        return
+    keep = R.kept(M, C, p, block.seed, block.offset).to(DEV) if p else torch.ones(M, C, dtype=torch.bool, device=DEV)
+    d = [t.detach().double() for t in (x, wg, wu, wd, dy, h)]
+    _, _, (dwd, e) = R.linear(d[5], d[3], None, keep, p, BF16, d[4])
+    R.worst(block.w_down.grad, last_rounding_in_fp32(dwd, e), "dw_down")
+    hh = h.detach().requires_grad_()
+    dh, = torch.autograd.grad(F.linear_dropout_add(hh, wd, None, **mask), hh, dy)
+    _, _, dwg, dwu = R.gated(d[0], d[1], d[2], "silu", BF16, dh.double())
+    R.worst(block.w_gate.grad, last_rounding_in_fp32(*dwg), "dw_gate")
+    R.worst(block.w_up.grad, last_rounding_in_fp32(*dwu), "dw_up")
+
+
+def test_parameters_in_other_types_are_cast_as_before():
+    x = rnd(1, 100, 64, dtype=BF16)
+    block = F.GatedFeedForward(64, 40).to(DEV)
+    want = block(x)
+    low = F.GatedFeedForward(64, 40).to(DEV, BF16)
+    low.load_state_dict(block.state_dict())
+    assert torch.equal(low(x), want)
+    low(x).sum().backward()
+    assert low.w_gate.grad.dtype is BF16
+    assert low(x.float()).dtype is torch.float32  # bf16 parameters on an fp32 map
+    low.w_up = torch.nn.Parameter(low.w_up.float())
+    assert torch.equal(low(x), want)
+    low(x).sum().backward()
+    assert low.w_up.grad.dtype is torch.float32
