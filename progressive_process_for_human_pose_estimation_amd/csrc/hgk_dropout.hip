@@ -149,28 +149,29 @@ static inline bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 template <typename T>
 static int launch_dropout(hipStream_t st, const DropoutArgs& a) {
   const bool al = al16(a.x) && al16(a.res) && al16(a.y);
+  HGK_CHECK_ARG(a.rows < (1l << 62) / a.groups, "dropout: too many rows (%ld)", a.rows);
   if (a.C % 8 == 0 && al) {
     if (a.rows_per_mask > 1) {
       const long n = ((a.rows + 3) / 4) * a.groups;
-      HGK_CHECK_ARG((n + 255) / 256 < (1l << 31), "dropout: too many elements");
+      HGK_CHECK_THREADS("dropout", (n + 255) / 256, 256);
       hipLaunchKernelGGL((dropout_vec_kernel<T, 4>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
     } else {
       const long n = a.rows * a.groups;
-      HGK_CHECK_ARG((n + 255) / 256 < (1l << 31), "dropout: too many elements");
+      HGK_CHECK_THREADS("dropout", (n + 255) / 256, 256);
       hipLaunchKernelGGL((dropout_vec_kernel<T, 1>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
     }
   } else if (a.groups * 8 <= kDropLds) {
     // RB rows: a multiple of 8, about 8192 elements a workgroup, mask bytes within the LDS
     int RB = 8 * std::max(1, std::min(kDropLds / (8 * a.groups), 8192 / (8 * a.C)));
     const long nb = (a.rows + RB - 1) / RB;
-    HGK_CHECK_ARG(nb < (1l << 31), "dropout: too many rows");
+    HGK_CHECK_THREADS("dropout", nb, 256);
     if (al)
       hipLaunchKernelGGL((dropout_flat_kernel<T, true>), dim3((unsigned)nb), dim3(256), 0, st, a, RB);
     else
       hipLaunchKernelGGL((dropout_flat_kernel<T, false>), dim3((unsigned)nb), dim3(256), 0, st, a, RB);
   } else {
     const long n = a.rows * a.groups;
-    HGK_CHECK_ARG((n + 255) / 256 < (1l << 31), "dropout: too many elements");
+    HGK_CHECK_THREADS("dropout", (n + 255) / 256, 256);
     hipLaunchKernelGGL((dropout_long_kernel<T>), dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, a);
   }
   HGK_LAUNCH_CHECK();

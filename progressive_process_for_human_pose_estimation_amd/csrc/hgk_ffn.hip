@@ -22,15 +22,13 @@ static int run_product(hipStream_t st, GemmArgs& a, const GemmPlan& p, char* sla
   a.splits = p.splits;
   a.slab = (float*)slab;
   if (p.splits > 1) {
-    run_tiles<DT, std::conditional_t<DT == G_F32, float, bf16_t>, LM, LN, E_SLAB>(st, a, p);
-    HGK_LAUNCH_CHECK();
+    if (int rc = run_tiles<DT, std::conditional_t<DT == G_F32, float, bf16_t>, LM, LN, E_SLAB>(st, a, p)) return rc;
     const long n = (long)a.batch * a.M * ((a.N + 7) / 8);
     hipLaunchKernelGGL((gemm_join_kernel<T>), dim3((unsigned)((n + 63) / 64)), dim3(64), 0, st, a);
-  } else {
-    run_tiles<DT, T, LM, LN, E_OUT>(st, a, p);
+    HGK_LAUNCH_CHECK();
+    return HGK_OK;
   }
-  HGK_LAUNCH_CHECK();
-  return HGK_OK;
+  return run_tiles<DT, T, LM, LN, E_OUT>(st, a, p);
 }
 
 // Up to this many rows stream the weights (skinny_kernel), more take tiles. The linear's tiles can split k, so
@@ -138,7 +136,7 @@ static bool al16(const void* p) { return ((uintptr_t)p & 15) == 0; }
                 what ": bad sizes (%ld rows, %d, %d)", (long)(M), (int)(A), (int)(B))
 
 template <typename T>
-static void gated_operands(hipStream_t st, GemmArgs& a, const GatedWs& w, char* ws, const void* x,
+static int gated_operands(hipStream_t st, GemmArgs& a, const GatedWs& w, char* ws, const void* x,
                            const void* wg, const void* wu, long M, int C, int F) {
   typedef typename TypeOf<T>::raw raw;
   if (w.pad) {
@@ -146,7 +144,7 @@ static void gated_operands(hipStream_t st, GemmArgs& a, const GatedWs& w, char* 
     p.add(x, ws + w.x, M, C, w.Cp, sizeof(T));
     p.add(wg, ws + w.wg, F, C, w.Cp, sizeof(T));
     p.add(wu, ws + w.wu, F, C, w.Cp, sizeof(T));
-    p.launch<raw>(st);
+    if (int rc = p.launch<raw>(st)) return rc;
   }
   a.m0 = a.m1 = w.pad ? ws + w.x : (const char*)x;
   a.n0 = w.pad ? ws + w.wg : (const char*)wg;
@@ -156,6 +154,7 @@ static void gated_operands(hipStream_t st, GemmArgs& a, const GatedWs& w, char* 
   a.N = F;
   a.km = a.kn = w.Cp;
   a.spseg = (int)up_to((long)w.Cp * sizeof(T), 128) / 128;
+  return HGK_OK;
 }
 
 template <typename T>
@@ -165,18 +164,17 @@ static int gated_fwd(hipStream_t st, const void* x, const void* wg, const void* 
   if (gated_rows_ok(dtype, M, C, F, false)) return gated_rows_fwd(st, x, wg, wu, h, M, C, F, act);
   const GatedWs w = gated_ws(dtype, M, C, F, 0);
   GemmArgs a = gemm_args();
-  gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
+  if (int rc = gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F)) return rc;
   a.out = h;
   a.act = act;
   a.vec = F % 8 == 0;
   if (M <= skinny_rows<T>(true)) {
     run_skinny<DT, T, true>(st, a);
-  } else {
-    const GemmPlan p = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, F, 2, a.spseg, 1, false);
-    run_tiles<DT, T, L_ROW, L_ROW, E_GATED>(st, a, p);
+    HGK_LAUNCH_CHECK();
+    return HGK_OK;
   }
-  HGK_LAUNCH_CHECK();
-  return HGK_OK;
+  const GemmPlan p = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, F, 2, a.spseg, 1, false);
+  return run_tiles<DT, T, L_ROW, L_ROW, E_GATED>(st, a, p);
 }
 
 template <typename T>
@@ -187,7 +185,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
   constexpr int es = sizeof(T), ks = 128 / es;
   const GatedWs w = gated_ws(dtype, M, C, F, wanted_code(dx, dwg));
   GemmArgs a = gemm_args();
-  gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F);
+  if (int rc = gated_operands<T>(st, a, w, ws, x, wg, wu, M, C, F)) return rc;
   const char *xp = a.m0, *wgp = a.n0, *wup = a.n1;
   if (w.rows) {  // Fp is F, Cp is C
     if (int rc = gated_rows_bwd(st, x, wg, wu, dh, dwg ? ws + w.dg : nullptr, ws + w.du, dx, M, C, F, act)) return rc;
@@ -199,8 +197,7 @@ static int gated_bwd(hipStream_t st, const void* x, const void* wg, const void* 
     a.act = act;
     a.vec = F % 8 == 0;
     const GemmPlan p = plan_gemm(dtype == HGK_BF16 ? G_BF16 : G_F32, M, F, 2, a.spseg, 1, false);
-    run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p);
-    HGK_LAUNCH_CHECK();
+    if (int rc = run_tiles<DT, T, L_ROW, L_ROW, E_GATED_BWD>(st, a, p)) return rc;
   }
   if (dx && !w.rows) {
     GemmArgs b = gemm_args();
@@ -285,7 +282,7 @@ static int linear_fwd(hipStream_t st, const void* x, const void* wt, const void*
     Pads p;
     p.add(x, ws + w.x, M, K, w.Kp, sizeof(T));
     p.add(wt, ws + w.w, N, K, w.Kp, sizeof(T));
-    p.launch<raw>(st);
+    if (int rc = p.launch<raw>(st)) return rc;
   }
   GemmArgs a = gemm_args();
   a.m0 = w.pad_k ? ws + w.x : (const char*)x;
@@ -335,8 +332,7 @@ static int linear_bwd(hipStream_t st, const void* x, const void* wt, const void*
     xp = ws + w.x;
     wp = ws + w.w;
   }
-  p.launch<raw>(st);
-  HGK_LAUNCH_CHECK();
+  if (int rc = p.launch<raw>(st)) return rc;
   const float alpha = drop ? d.scale : 1.f;
   if (dx && !w.rows) {
     GemmArgs b = gemm_args();

@@ -260,26 +260,27 @@ bool gated_rows_ok(int dtype, long M, int C, int F, bool bwd) {
 }
 
 template <int NK, bool BWD, int ACT, int RW>
-static void launch_rows_as(hipStream_t st, const RowsArgs& a) {
+static int launch_rows_as(hipStream_t st, const RowsArgs& a) {
   constexpr int rows = 128 * RW;
+  HGK_CHECK_THREADS("gated", ((long)a.M + rows - 1) / rows, 512);
   hipLaunchKernelGGL((gated_rows_kernel<NK, BWD, ACT, RW>), dim3((unsigned)((a.M + rows - 1) / rows)), dim3(512), 0, st, a);
+  HGK_LAUNCH_CHECK();
+  return HGK_OK;
 }
 template <bool BWD, int ACT>
-static void launch_rows_act(hipStream_t st, const RowsArgs& a) {
-  if (a.C <= 64) launch_rows_as<2, BWD, ACT, 1>(st, a);
-  else if constexpr (BWD) a.C <= 128 ? launch_rows_as<4, true, ACT, 1>(st, a) : launch_rows_as<8, true, ACT, 1>(st, a);
-  else if (a.C > 128) launch_rows_as<8, false, ACT, 2>(st, a);
-  else if (a.M >= kTwoGroups) launch_rows_as<4, false, ACT, 2>(st, a);
-  else launch_rows_as<4, false, ACT, 1>(st, a);
+static int launch_rows_act(hipStream_t st, const RowsArgs& a) {
+  if (a.C <= 64) return launch_rows_as<2, BWD, ACT, 1>(st, a);
+  if constexpr (BWD) return a.C <= 128 ? launch_rows_as<4, true, ACT, 1>(st, a) : launch_rows_as<8, true, ACT, 1>(st, a);
+  else if (a.C > 128) return launch_rows_as<8, false, ACT, 2>(st, a);
+  else if (a.M >= kTwoGroups) return launch_rows_as<4, false, ACT, 2>(st, a);
+  else return launch_rows_as<4, false, ACT, 1>(st, a);
 }
 template <bool BWD>
 static int launch_rows(hipStream_t st, const RowsArgs& a) {
-  if (a.act == kActSilu) launch_rows_act<BWD, kActSilu>(st, a);
-  else if (a.act == kActGelu) launch_rows_act<BWD, kActGelu>(st, a);
-  else if (a.act == kActRelu) launch_rows_act<BWD, kActRelu>(st, a);
-  else launch_rows_act<BWD, kActSigmoid>(st, a);
-  HGK_LAUNCH_CHECK();
-  return HGK_OK;
+  if (a.act == kActSilu) return launch_rows_act<BWD, kActSilu>(st, a);
+  if (a.act == kActGelu) return launch_rows_act<BWD, kActGelu>(st, a);
+  if (a.act == kActRelu) return launch_rows_act<BWD, kActRelu>(st, a);
+  return launch_rows_act<BWD, kActSigmoid>(st, a);
 }
 
 int gated_rows_fwd(hipStream_t st, const void* x, const void* wg, const void* wu, void* h, long M, int C, int F,

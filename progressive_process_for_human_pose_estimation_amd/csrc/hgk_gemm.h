@@ -954,9 +954,12 @@ struct Pads {
     a.chunks += rows * ((long)Kp * es / 16);
   }
   template <typename E>
-  void launch(hipStream_t st) {
-    if (a.n)
-      hipLaunchKernelGGL((pad_rows_kernel<E>), dim3((unsigned)((a.chunks + 255) / 256)), dim3(256), 0, st, a);
+  int launch(hipStream_t st) {
+    if (!a.n) return HGK_OK;
+    HGK_CHECK_THREADS("padded rows", (a.chunks + 255) / 256, 256);
+    hipLaunchKernelGGL((pad_rows_kernel<E>), dim3((unsigned)((a.chunks + 255) / 256)), dim3(256), 0, st, a);
+    HGK_LAUNCH_CHECK();
+    return HGK_OK;
   }
 };
 
@@ -1019,18 +1022,22 @@ static inline GemmArgs gemm_args() {
 }
 
 template <int DT, typename T, int LM, int LN, int EPI>
-static void run_tiles(hipStream_t st, GemmArgs& a, const GemmPlan& p) {
+static int run_tiles(hipStream_t st, GemmArgs& a, const GemmPlan& p) {
   a.tiles_m = p.tiles_m;
   a.tiles_n = p.tiles_n;
+  HGK_CHECK_THREADS("product", (long)a.tiles_m * a.tiles_n * a.batch * a.splits, p.tile == 256 ? 512 : 256);
   const dim3 grid((unsigned)((long)a.tiles_m * a.tiles_n * a.batch * a.splits));
   if constexpr (DT != G_F32) {
     if (p.tile == 256) {
       hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 256, 4, 2, EPI>), grid, dim3(512), 0, st, a);
-      return;
+      HGK_LAUNCH_CHECK();
+      return HGK_OK;
     }
   }
   if (p.tile == 128) hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 128, 2, 2, EPI>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((gemm_kernel<DT, T, LM, LN, 64, 4, 1, EPI>), grid, dim3(256), 0, st, a);
+  HGK_LAUNCH_CHECK();
+  return HGK_OK;
 }
 
 }  // namespace hgk

@@ -92,9 +92,16 @@ template <typename T, bool VEC>
 static void launch_quant_as(hipStream_t st, const T* x, int8_t* q, float* s, long rows, int K, int Kp) {
   const int nc = VEC ? K / Vec16<T>::N : K;
   const dim3 blk(256);
-  auto grid = [&](int L) { return dim3((unsigned)((rows * L + 255) / 256)); };
-#define HGK_QUANT(L, NCH) \
-  hipLaunchKernelGGL((quant_rows_kernel<T, L, NCH, VEC>), grid(L), blk, 0, st, x, q, s, rows, K, Kp)
+  // in runs of rows: a launch holds less than 2^32 threads
+  auto runs = [&](int threads, auto&& launch) {
+    const long most = (1l << 31) / threads;
+    for (long r = 0; r < rows; r += most) launch(x + r * K, q + r * Kp, s + r, std::min(most, rows - r));
+  };
+#define HGK_QUANT(L, NCH)                                                                                              \
+  runs(L, [&](const T* xr, int8_t* qr, float* sr, long n) {                                                            \
+    hipLaunchKernelGGL((quant_rows_kernel<T, L, NCH, VEC>), dim3((unsigned)((n * L + 255) / 256)), blk, 0, st, xr, qr, \
+                       sr, n, K, Kp);                                                                                  \
+  })
   if (nc <= 8) HGK_QUANT(8, 1);
   else if (nc <= 16) HGK_QUANT(16, 1);
   else if (nc <= 32) HGK_QUANT(16, 2);
@@ -102,7 +109,10 @@ static void launch_quant_as(hipStream_t st, const T* x, int8_t* q, float* s, lon
   else if (nc <= 128) HGK_QUANT(64, 2);
   else if (nc <= 256) HGK_QUANT(64, 4);
   else if (nc <= 512) HGK_QUANT(64, 8);
-  else if constexpr (VEC) hipLaunchKernelGGL((quant_long_kernel<T>), dim3((unsigned)rows), blk, 0, st, x, q, s, K, Kp);
+  else if constexpr (VEC)
+    runs(256, [&](const T* xr, int8_t* qr, float* sr, long n) {
+      hipLaunchKernelGGL((quant_long_kernel<T>), dim3((unsigned)n), blk, 0, st, xr, qr, sr, K, Kp);
+    });
   else HGK_QUANT(64, 0);
 #undef HGK_QUANT
 }
@@ -323,8 +333,7 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
       p.add(w1, ws + w.w1, N, K, w.Kp, 1);
       a.n1 = ws + w.w1;
     }
-    p.launch<uint8_t>(st);
-    HGK_LAUNCH_CHECK();
+    if (int rc = p.launch<uint8_t>(st)) return rc;
   }
   constexpr int EPI = GATED ? E_GATED : E_OUT, per = GATED ? 2 : 1;
   if (way == W_FEW) {
@@ -333,7 +342,7 @@ static int linear_i8(hipStream_t st, const void* x, const void* w0, const float*
     else if (M <= 32) hipLaunchKernelGGL((skinny_kernel<G_I8, T, 2, GATED>), grid, dim3(512), 0, st, a);
     else hipLaunchKernelGGL((skinny_kernel<G_I8, T, 4, GATED>), grid, dim3(512), 0, st, a);
   } else {
-    run_tiles<G_I8, T, L_ROW, L_ROW, EPI>(st, a, plan_gemm(G_I8, M, N, per, a.spseg, 1, false));
+    return run_tiles<G_I8, T, L_ROW, L_ROW, EPI>(st, a, plan_gemm(G_I8, M, N, per, a.spseg, 1, false));
   }
   HGK_LAUNCH_CHECK();
   return HGK_OK;

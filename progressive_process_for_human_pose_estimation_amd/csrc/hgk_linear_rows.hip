@@ -167,9 +167,12 @@ bool linear_rows_ok(int dtype, long M, int K, int N, bool drop) {
 }
 
 template <int NK, int RW>
-static void launch_as(hipStream_t st, const LinearRowsArgs& a) {
+static int launch_as(hipStream_t st, const LinearRowsArgs& a) {
   constexpr int rows = 128 * RW;
+  HGK_CHECK_THREADS("linear", ((long)a.M + rows - 1) / rows, 512);
   hipLaunchKernelGGL((linear_rows_kernel<NK, RW>), dim3((unsigned)((a.M + rows - 1) / rows)), dim3(512), 0, st, a);
+  HGK_LAUNCH_CHECK();
+  return HGK_OK;
 }
 int linear_rows_bwd(hipStream_t st, const void* dy, const void* w, void* dz, void* dx, long M, int K, int N,
                     const DropArgs& d) {
@@ -184,12 +187,10 @@ int linear_rows_bwd(hipStream_t st, const void* dy, const void* w, void* dz, voi
   a.drop = d.thr != 0;
   a.alpha = a.drop ? d.scale : 1.f;
   a.d = d;
-  if (N <= 64) launch_as<2, 1>(st, a);
-  else if (N <= 128) launch_as<4, 1>(st, a);
-  else if (M < kTwoGroups) launch_as<8, 1>(st, a);
-  else launch_as<8, 2>(st, a);
-  HGK_LAUNCH_CHECK();
-  return HGK_OK;
+  if (N <= 64) return launch_as<2, 1>(st, a);
+  if (N <= 128) return launch_as<4, 1>(st, a);
+  if (M < kTwoGroups) return launch_as<8, 1>(st, a);
+  return launch_as<8, 2>(st, a);
 }
 
 }  // namespace hgk

@@ -26,6 +26,10 @@ __device__ __forceinline__ uint4 philox4x32_10(uint4 c, uint32_t k0, uint32_t k1
   return c;
 }
 
+// a launch holds less than 2^32 threads
+#define HGK_CHECK_THREADS(what, workgroups, threads) \
+  HGK_CHECK_ARG((workgroups) < (1l << 32) / (threads), what ": too many workgroups (%ld of %d threads)", (long)(workgroups), (int)(threads))
+
 struct DropArgs {
   uint32_t thr;  // 0 .. 65536; 0: everything kept
   float scale;   // 65536 / (65536 - thr); 0 at thr = 65536

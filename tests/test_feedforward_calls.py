@@ -305,3 +305,28 @@ def test_backward_refuses_a_workspace_for_fewer_gradients():
     assert L.hgk_gated_bwd(None, 1, A, A, A, A, A, A, A, M, C, Fh, 0, A, n) == -1 and b"too small" in L.hgk_last_error()
     n = L.hgk_linear_workspace(1, M, Fh, C, 1, 2)
     assert L.hgk_linear_bwd(None, 1, A, A, A, A, A, M, Fh, C, 0.5, 0, 0, None, A, n) == -1 and b"too small" in L.hgk_last_error()
+
+
+def test_launches_of_more_threads_than_there_are_numbers_are_refused():
+    """A launch holds less than 2^32 threads. Sizes that would take more, and that a card could hold, are refused before
+    anything runs."""
+    L, A = H.lib(), 1 << 20  # an address on a 16-byte border, never read
+    big = 1 << 62
+
+    def refused(rc):
+        msg = L.hgk_last_error()
+        return rc == -1 and b"too many" in msg
+
+    M = 1 << 30
+    assert refused(L.hgk_dropout_add(None, 1, A, None, A, 1 << 32, 8, 1, 0.5, 0, 0, None))
+    assert refused(L.hgk_dropout_add(None, 1, A, None, A, 1 << 34, 8, 1 << 20, 0.5, 0, 0, None))
+    assert refused(L.hgk_dropout_add(None, 1, A, None, A, 1 << 38, 1, 1, 0.5, 0, 0, None))
+    assert refused(L.hgk_dropout_add(None, 1, A, None, A, (1 << 22) + 1, 8193, 1, 0.5, 0, 0, None))
+    assert refused(L.hgk_dropout_add(None, 1, A, None, A, 1 << 62, 64, 1, 0.5, 0, 0, None))  # rows * groups leave 64 bits
+    assert refused(L.hgk_gated_fwd(None, 1, A, A, A, A, M, 8, 8, 0, None, 0))
+    assert refused(L.hgk_gated_fwd(None, 1, A, A, A, A, M, 33, 8, 0, A, big))
+    assert refused(L.hgk_gated_bwd(None, 1, A, A, A, A, A, None, None, M, 8, 8, 0, A, big))
+    assert refused(L.hgk_gated_bwd(None, 1, A, A, A, A, None, A, A, M, 8, 16, 0, A, big))
+    assert refused(L.hgk_linear_fwd(None, 1, A, A, None, A, M, 8, 8, 0.0, 0, 0, None, A, big))
+    assert refused(L.hgk_linear_bwd(None, 1, A, A, A, A, None, M, 8, 8, 0.0, 0, 0, None, A, big))
+    assert refused(L.hgk_linear_bwd(None, 1, A, A, A, None, A, M, 8, 33, 0.0, 0, 0, None, A, big))

@@ -176,3 +176,15 @@ def test_one_gradient_at_a_time(M, C, Fh, dtype):
 
         both = linear(0, 1)
         assert torch.equal(linear(0)[0], both[0]) and torch.equal(linear(1)[0], both[1])
+
+
+def test_rows_past_one_launch_are_quantised():
+    """8 threads a row: runs of 2^28 rows"""
+    M = (1 << 28) + 37
+    x = torch.zeros(M, 8, device=DEV, dtype=torch.bfloat16)
+    some = torch.tensor([0, 1, (1 << 28) - 2, (1 << 28) - 1, 1 << 28, (1 << 28) + 1, M - 1], device=DEV)
+    x[some] = rnd(1, len(some), 8, dtype=torch.bfloat16)
+    q, s = F.quantize_rows(x)
+    want_q, want_s = F.quantize_rows(x[some])
+    assert torch.equal(q[some], want_q) and torch.equal(s[some], want_s)
+    assert int(s.count_nonzero()) == len(some)
