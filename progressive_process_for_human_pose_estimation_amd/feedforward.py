@@ -34,7 +34,7 @@ ACTIVATIONS = {"silu": 0, "gelu": 1, "relu": 2, "sigmoid": 3}
 _DTYPES = {torch.float32: H.F32, torch.bfloat16: H.BF16}
 _U64 = 1 << 64
 _PROXY = torch._C._TorchDispatchModeKey.PROXY
-_dispatch_mode, _tracing_state = torch._C._get_dispatch_mode, torch._C._get_tracing_state
+_dispatch_mode, _tracing = torch._C._get_dispatch_mode, torch._C._is_tracing
 
 
 def _code(what, x):
@@ -98,20 +98,17 @@ def _check_dropout(p, seed, offset, step, device):
         raise H.HgkError(f"dropout: step is an int64 tensor of one element on {device}")
 
 
-def _grads(*operands):
-    if not torch.is_grad_enabled():
-        return False
-    for t in operands:
-        if t is not None and t.requires_grad:
-            return True
-    return False
-
-
 def _by_function(*operands):
     """Whether a call goes through its autograd function: where a gradient is wanted, under torch.jit.trace
     (which records functions; of a bare launch it would record the allocation of the result) and in forward
     mode (where a function refuses the tangent that a bare launch would lose)"""
-    return _grads(*operands) or _tracing_state() is not None or forward_ad._current_level >= 0
+    if _tracing() or forward_ad._current_level >= 0:
+        return True
+    if torch.is_grad_enabled():
+        for t in operands:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 def _launch(x, fn, *args):
@@ -155,12 +152,14 @@ def _once(backward):
 def _gated_operands(x, w_gate, w_up, activation, masters):
     """(x, w_gate, w_up, activation) as the kernels take them, or HgkError"""
     _check_weights("gated_linear", w_gate, w_up)
-    of = _weight_type(x, masters)
+    of = _weight_type(x, masters) if masters else x.dtype
     _check("gated_linear", x, w_gate.shape[1], (w_gate, of), (w_up, of))
     _code("gated_linear", x)
     act = _act(activation)
     _gpu("gated_linear", x)
-    return _dense(x), _dense(w_gate.to(x.dtype)), _dense(w_up.to(x.dtype)), act
+    if of is not x.dtype:
+        w_gate, w_up = w_gate.to(x.dtype), w_up.to(x.dtype)
+    return _dense(x), _dense(w_gate), _dense(w_up), act
 
 
 def _gated_fwd(x, wg, wu, act):
@@ -216,13 +215,16 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
 # ---- product, dropout and residual ----
 def _linear_operands(x, w, residual, p, seed, offset, step, masters):
     _check_weights("linear_dropout_add", w)
-    _check("linear_dropout_add", x, w.shape[1], (w, _weight_type(x, masters)), (residual, x.dtype))
+    of = _weight_type(x, masters) if masters else x.dtype
+    _check("linear_dropout_add", x, w.shape[1], (w, of), (residual, x.dtype))
     _code("linear_dropout_add", x)
     if residual is not None and residual.shape != (*x.shape[:-1], w.shape[0]):
         raise H.HgkError(f"linear_dropout_add: residual of shape {tuple(residual.shape)}")
     _check_dropout(p, seed, offset, step, x.device)
     _gpu("linear_dropout_add", x)
-    return _dense(x), _dense(w.to(x.dtype)), None if residual is None else _dense(residual)
+    if of is not x.dtype:
+        w = w.to(x.dtype)
+    return _dense(x), _dense(w), None if residual is None else _dense(residual)
 
 
 def _linear_fwd(x, w, res, p, seed, offset, step):
@@ -389,7 +391,8 @@ def _linear_i8(x, w, w_scale, bias, residual):
         _check_scale("linear_i8", bias, N)
     _gpu("linear_i8", x)
     x, w, w_scale = _dense(x), _dense(w), _dense(w_scale)
-    bias, residual = (None if t is None else _dense(t) for t in (bias, residual))
+    bias = None if bias is None else _dense(bias)
+    residual = None if residual is None else _dense(residual)
     M, lib = x.numel() // K, H.lib()
     y = x.new_empty((*x.shape[:-1], N))
     wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, K, N, 0), x)
@@ -424,7 +427,7 @@ def _gated_i8(x, wg, sg, wu, su, activation):
     _check_scale("gated_linear_i8", sg, F)
     _check_scale("gated_linear_i8", su, F)
     _gpu("gated_linear_i8", x)
-    x, wg, sg, wu, su = (_dense(t) for t in (x, wg, sg, wu, su))
+    x, wg, sg, wu, su = _dense(x), _dense(wg), _dense(sg), _dense(wu), _dense(su)
     M, lib = x.numel() // C, H.lib()
     h = x.new_empty((*x.shape[:-1], F))
     wp, n, own = _workspace(lib.hgk_linear_i8_workspace(M, C, F, 1), x)
@@ -473,7 +476,7 @@ class _Masks(nn.Module):
         """keyword arguments of the next use, on x's device"""
         if not self.training or self.p == 0.0:
             return {"p": 0.0}
-        tracing = _tracing_state() is not None
+        tracing = _tracing()
         self.offset = 0 if tracing else self._draw()  # a trace is compared with another one: no number of its own
         return {"p": self.p, "seed": self.seed, "offset": self.offset, "step": self._recorded_step(x, tracing)}
 
