@@ -123,8 +123,8 @@ __global__ __launch_bounds__(256) void dropout_flat_kernel(DropoutArgs a, int RB
   }
 }
 
-// rows whose masks are not more than kDropLds bytes go row by row through the flat kernel; longer
-// rows (C > 65536) take one group of one row a thread
+// Runs of 8 rows whose masks are more than kDropLds bytes (C > 8192, off the 16-byte borders): one group of
+// one row a thread, element by element
 template <typename T>
 __global__ __launch_bounds__(256) void dropout_long_kernel(DropoutArgs a) {
   const long t = (long)blockIdx.x * 256 + threadIdx.x;

@@ -127,7 +127,7 @@ __device__ __forceinline__ void dma16s(const char* base, uint32_t off, char* lds
 }
 
 // ---- activations: value and slope. `FAST`: bf16 results (hardware exponential and reciprocal,
-// 1 ulp of fp32, against a half step of 2^-9); fp32 results take the full-precision functions ----
+// 1 ulp of fp32, against a half step of 2^-8); fp32 results take the full-precision functions ----
 template <bool FAST>
 __device__ __forceinline__ float sigmoid_f(float g) {
   if (FAST) return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(g * -1.44269504f));

@@ -2,7 +2,9 @@
 // for each output channel, how the block's products are served:
 //   s_m = max_k |x[m][k]| / 127 (fp32),  q[m][k] = rint(x[m][k] / s_m)
 //   y[m][n] = s_m w_n sum_k q[m][k] wq[n][k] (+ b[n]);   gated: a(G) U of two such products
-// The sums are exact: int32 accumulators (K <= 2^17 keeps |sum| < 2^31), scaled once in fp32.
+// The sums are exact: int32 accumulators (K <= 2^17 keeps |sum| < 2^31). A sum is then rounded to fp32
+// (none below 2^24, K = 1040) and multiplied by the two scales in fp32: three roundings of 2^-24, a share of
+// 2^-14 of the one to bf16. 64-bit products would run at a small part of the epilogue's rate.
 // v_mfma_i32_16x16x64_i8 runs at twice the bf16 rate and the weights are half its bytes.
 #include "hgk_gemm.h"
 

@@ -11,8 +11,10 @@ hgk_dropout.hip, hgk_linear_i8.hip), for training and, in 8-bit integers, for se
 
 Activations are channels-last: [..., C] fp32 or bf16 on the GPU (an NCHW map in channels_last
 memory is `x.permute(0, 2, 3, 1)`, without a copy). Weights are [out, in] in the activations' type;
-gradients have the type of what they belong to. Sums are fp32 (int32 in the 8-bit products), rounded
-once. Other strides, and views that do not start on a 16-byte border, are copied first.
+gradients have the type of what they belong to. Sums are fp32 (int32 in the 8-bit products) and results
+are rounded once; the gated product's backward rounds the gradients of its two inner products to the
+operands' type on the way. Other strides, and views that do not start on a 16-byte border, are copied
+first.
 
 Dropout's mask is a function of (seed, offset, element) and never stored: the backward draws it
 again. An element is dropped with probability p to the nearest 2^-16 and the rest is scaled by the
@@ -20,7 +22,8 @@ inverse of the probability that is kept. The same (seed, offset) gives the same 
 offset for each use. `step`, an int64 GPU tensor of one element, is added to the offset on the
 device, so that a captured graph draws other masks at each replay; it must not change between a
 forward and its backward. Everything here can be captured (a backward together with its forward, on
-leaves of which no eager graph is alive); there is no CPU fallback.
+leaves of which no eager graph is alive) and traced by torch.jit.trace; forward mode, make_fx and a
+second derivative are refused. There is no CPU fallback.
 """
 import math
 
