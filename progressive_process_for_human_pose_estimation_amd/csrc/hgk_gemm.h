@@ -978,10 +978,11 @@ struct GemmPlan {
 // hide all of that. A CU with one or two workgroups waits for memory instead: 0.16 us and 0.8 of its
 // products a step. A round ends with its epilogue, 4 us of a 256-wide tile. Against the tile stand the
 // rounds: tiles are dealt to 256 CUs whole. Splitting k costs the partial sums' way to memory and back
-// (4.6 TB/s) and a second launch (4.7 us). The constants of waiting and splitting are fitted to 29 weight
-// gradients (64 x 256 .. 2048 x 512 over 2000 .. 131072 rows, all tiles, 4 to 256 splits): what they choose
-// is 1 % slower on average than the best of each (256 x 1024 over 32768 rows: 30.7 us in 16 splits of
-// 128-wide tiles, 35.6 in 32, 38.6 in 64-wide tiles).
+// (4.6 TB/s) and a second launch (4.7 us). The constants of waiting and splitting are fitted to weight
+// gradients of 64 x 256 .. 2048 x 512 over 2000 .. 131072 rows. Measured over 28 of those, every tile and 1 to 128
+// splits: what they choose is 3 % slower on average than the best of each (256 x 1024 over 32768 rows: 32 us in
+// 16 splits of 128-wide tiles, 40 in 64-wide ones), 26 % at worst (the same over 131072 rows: 115 us for 92 of 64
+// splits of 256-wide tiles).
 static inline GemmPlan plan_gemm(int dt, long M, long N, int per, int steps, int batch, bool can_split) {
   GemmPlan best;
   double least = 1e30;
