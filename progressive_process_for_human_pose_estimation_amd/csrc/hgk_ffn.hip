@@ -397,6 +397,7 @@ using namespace hgk;
 extern "C" {
 
 size_t hgk_gated_workspace(int dtype, long M, int C, int F, int backward) {
+  dtype &= ~HGK_F32_WGRAD;
   if (M <= 0 || C <= 0 || F <= 0 || (dtype != HGK_F32 && dtype != HGK_BF16)) return 0;
   return (size_t)gated_ws(dtype, M, C, F, backward).total;
 }
@@ -438,6 +439,7 @@ int hgk_gated_bwd(hgk_stream_t stream, int dtype, const void* x, const void* wg,
 }
 
 size_t hgk_linear_workspace(int dtype, long M, int K, int N, int dropout, int backward) {
+  dtype &= ~HGK_F32_WGRAD;
   if (M <= 0 || K <= 0 || N <= 0 || (dtype != HGK_F32 && dtype != HGK_BF16)) return 0;
   return (size_t)linear_ws(dtype, M, K, N, dropout != 0, backward).total;
 }

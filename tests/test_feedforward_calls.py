@@ -330,3 +330,10 @@ def test_launches_of_more_threads_than_there_are_numbers_are_refused():
     assert refused(L.hgk_linear_fwd(None, 1, A, A, None, A, M, 8, 8, 0.0, 0, 0, None, A, big))
     assert refused(L.hgk_linear_bwd(None, 1, A, A, A, A, None, M, 8, 8, 0.0, 0, 0, None, A, big))
     assert refused(L.hgk_linear_bwd(None, 1, A, A, A, None, A, M, 8, 33, 0.0, 0, 0, None, A, big))
+
+
+def test_workspace_queries_take_the_dtype_that_the_backward_takes():
+    L = H.lib()
+    assert L.hgk_gated_workspace(1 | H.F32_WGRAD, 500, 100, 200, 1) == L.hgk_gated_workspace(1, 500, 100, 200, 1) > 0
+    assert L.hgk_linear_workspace(1 | H.F32_WGRAD, 500, 100, 200, 1, 1) == L.hgk_linear_workspace(1, 500, 100, 200, 1, 1) > 0
+    assert L.hgk_gated_fwd(None, 1 | H.F32_WGRAD, 1 << 20, 1 << 20, 1 << 20, 1 << 20, 4, 8, 8, 0, None, 0) == -1
