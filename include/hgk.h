@@ -680,7 +680,7 @@ int hgk_gated_fwd(hgk_stream_t stream, int dtype, const void* x, const void* wg,
 /* `dtype` of hgk_gated_bwd and hgk_linear_bwd with this bit set: the weights' gradients are written in
  * fp32, whatever the operands' type (fp32 masters of bf16 weights; ABI 41) */
 enum { HGK_F32_WGRAD = 0x100 };
-/* its backward from dh [M][F]; nothing is kept from the forward (both products are computed again).
+/* hgk_gated_fwd's backward from dh [M][F]; nothing is kept from the forward (both products are computed again).
  * dx [M][C] nullable; dwg / dwu [F][C] both or neither. Overwrites its outputs. */
 int hgk_gated_bwd(hgk_stream_t stream, int dtype, const void* x, const void* wg, const void* wu,
                   const void* dh, void* dx, void* dwg, void* dwu, long M, int C, int F, int act,

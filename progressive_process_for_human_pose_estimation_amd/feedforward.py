@@ -65,8 +65,9 @@ def _check(what, x, k, *others):
     """x [..., k] and the other operands: on one device, each of its type"""
     if _dispatch_mode(_PROXY) is not None:
         raise H.HgkError(f"{what}: make_fx cannot record it (torch.jit.trace can)")
-    if x.dim() < 1 or x.shape[-1] != k:
-        raise H.HgkError(f"{what}: expected rows of {k} channels, got shape {tuple(x.shape)}")
+    shape = x.shape
+    if not shape or shape[-1] != k:
+        raise H.HgkError(f"{what}: expected rows of {k} channels, got shape {tuple(shape)}")
     device = x.device
     for t, dtype in others:
         if t is not None and (t.dtype is not dtype or t.device != device):
@@ -87,9 +88,10 @@ def _weight_type(x, masters):
 
 
 def _check_weights(what, w, v=None):
-    if w.dim() != 2 or 0 in w.shape or (v is not None and v.shape != w.shape):
+    shape = w.shape
+    if len(shape) != 2 or 0 in shape or (v is not None and v.shape != shape):
         raise H.HgkError(f"{what}: weights are [out, in], got {[tuple(t.shape) for t in (w, v) if t is not None]}")
-    return w.shape
+    return shape
 
 
 def _check_dropout(p, seed, offset, step, device):
@@ -154,9 +156,9 @@ def _once(backward):
 # ---- the gated product ----
 def _gated_operands(x, w_gate, w_up, activation, masters):
     """(x, w_gate, w_up, activation) as the kernels take them, or HgkError"""
-    _check_weights("gated_linear", w_gate, w_up)
+    C = _check_weights("gated_linear", w_gate, w_up)[1]
     of = _weight_type(x, masters) if masters else x.dtype
-    _check("gated_linear", x, w_gate.shape[1], (w_gate, of), (w_up, of))
+    _check("gated_linear", x, C, (w_gate, of), (w_up, of))
     _code("gated_linear", x)
     act = _act(activation)
     _gpu("gated_linear", x)
@@ -217,11 +219,11 @@ def gated_linear(x, w_gate, w_up, activation="silu"):
 
 # ---- product, dropout and residual ----
 def _linear_operands(x, w, residual, p, seed, offset, step, masters):
-    _check_weights("linear_dropout_add", w)
+    N, K = _check_weights("linear_dropout_add", w)
     of = _weight_type(x, masters) if masters else x.dtype
-    _check("linear_dropout_add", x, w.shape[1], (w, of), (residual, x.dtype))
+    _check("linear_dropout_add", x, K, (w, of), (residual, x.dtype))
     _code("linear_dropout_add", x)
-    if residual is not None and residual.shape != (*x.shape[:-1], w.shape[0]):
+    if residual is not None and residual.shape != (*x.shape[:-1], N):
         raise H.HgkError(f"linear_dropout_add: residual of shape {tuple(residual.shape)}")
     _check_dropout(p, seed, offset, step, x.device)
     _gpu("linear_dropout_add", x)
@@ -382,8 +384,7 @@ def _check_scale(what, s, n):
 
 
 def _linear_i8(x, w, w_scale, bias, residual):
-    _check_weights("linear_i8", w)
-    N, K = w.shape
+    N, K = _check_weights("linear_i8", w)
     _check("linear_i8", x, K, (w, torch.int8), (w_scale, torch.float32), (bias, torch.float32),
            (residual, x.dtype))
     _code("linear_i8", x)
@@ -422,8 +423,7 @@ def linear_i8(x, w, w_scale, bias=None, residual=None):
 
 
 def _gated_i8(x, wg, sg, wu, su, activation):
-    _check_weights("gated_linear_i8", wg, wu)
-    F, C = wg.shape
+    F, C = _check_weights("gated_linear_i8", wg, wu)
     _check("gated_linear_i8", x, C, (wg, torch.int8), (wu, torch.int8), (sg, torch.float32), (su, torch.float32))
     _code("gated_linear_i8", x)
     act = _act(activation)
